@@ -113,6 +113,14 @@ _SIGS = {
     "sigmoid_gate_backward_hip": (i32, [vp, vp, vp, sz, sz, sz, vp]),
     "adamw_step_hip": (i32, [vp, vp, vp, vp, sz, f32, f32, f32, f32, f32, sz, vp]),
     "adamw_step_master_hip": (i32, [vp, vp, vp, vp, vp, sz, f32, f32, f32, f32, f32, sz, vp]),
+    "adamw_step_master_scaled_hip": (i32, [vp, vp, vp, vp, vp, vp, sz, f32, f32, f32, f32, f32,
+                                           sz, vp]),
+    # gradient norm and clipping
+    "grad_list_create_hip": (i32, [ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(vp),
+                                   ctypes.POINTER(sz), ctypes.POINTER(i32), sz]),
+    "grad_list_destroy_hip": (i32, [vp]),
+    "grad_norm_hip": (i32, [vp, f32, vp, vp, vp]),
+    "grad_clip_hip": (i32, [vp, f32, vp, vp]),
     # embedding, cross-entropy
     "embedding_forward_hip": (i32, [vp, vp, vp, sz, sz, vp]),
     "embedding_forward_checked_hip": (i32, [vp, vp, vp, sz, sz, sz, vp]),
@@ -120,6 +128,12 @@ _SIGS = {
     "cross_entropy_forward_hip": (i32, [vp, vp, vp, sz, sz, f32, vp]),
     "cross_entropy_backward_hip": (i32, [vp, vp, vp, vp, sz, sz, f32, vp]),
     "cross_entropy_forward_backward_hip": (i32, [vp, vp, vp, vp, vp, sz, sz, f32, vp]),
+    # policy and preference losses
+    "token_logprob_forward_hip": (i32, [vp, vp, vp, vp, sz, sz, sz, i32, vp]),
+    "policy_loss_forward_backward_hip": (i32, [vp] * 10 + [sz] * 4 + [f32] * 3 + [i32, vp]),
+    "preference_loss_workspace_size": (sz, [sz]),
+    "preference_loss_forward_backward_hip": (i32, [vp] * 9 + [sz] * 5 + [f32] * 2 +
+                                             [i32, vp, sz, vp]),
     # sequence packing (host)
     "efla_pack_sequences": (i32, [vp, vp, sz, sz, vp, vp, vp, vp, ctypes.POINTER(sz),
                                   ctypes.POINTER(sz)]),

@@ -132,7 +132,9 @@ __global__ void __launch_bounds__(NTH) adamw_master_kernel(float* __restrict__ p
                                                            float* __restrict__ m,
                                                            float* __restrict__ v,
                                                            bf16* __restrict__ pcopy, long n,
-                                                           long n8, AdamArgs a) {
+                                                           long n8, AdamArgs a,
+                                                           const float* __restrict__ gscale) {
+    const float gs = gscale ? *gscale : 1.f;
     for (long i = gid(); i < n8; i += gstride()) {
         f32x4 p0 = reinterpret_cast<f32x4*>(p)[2 * i], p1 = reinterpret_cast<f32x4*>(p)[2 * i + 1];
         f32x4 m0 = reinterpret_cast<f32x4*>(m)[2 * i], m1 = reinterpret_cast<f32x4*>(m)[2 * i + 1];
@@ -141,8 +143,8 @@ __global__ void __launch_bounds__(NTH) adamw_master_kernel(float* __restrict__ p
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float pa = p0[j], ma = m0[j], va = v0[j], pb = p1[j], mb = m1[j], vb = v1[j];
-            adam1(pa, (float)gv[j], ma, va, a);
-            adam1(pb, (float)gv[4 + j], mb, vb, a);
+            adam1(pa, gs * (float)gv[j], ma, va, a);
+            adam1(pb, gs * (float)gv[4 + j], mb, vb, a);
             p0[j] = pa, m0[j] = ma, v0[j] = va, p1[j] = pb, m1[j] = mb, v1[j] = vb;
         }
         reinterpret_cast<f32x4*>(p)[2 * i] = p0;
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(NTH) adamw_master_kernel(float* __restrict__ p
         }
     }
     for (long i = n8 * 8 + gid(); i < n; i += gstride()) {
-        adam1(p[i], (float)g[i], m[i], v[i], a);
+        adam1(p[i], gs * (float)g[i], m[i], v[i], a);
         if (pcopy) pcopy[i] = (bf16)p[i];
     }
 }
@@ -326,12 +328,11 @@ extern "C" int adamw_step_hip(void* param, const void* grad, void* exp_avg, void
     return (int)hipPeekAtLastError();
 }
 
-extern "C" int adamw_step_master_hip(float* param, const void* grad, float* exp_avg,
-                                     float* exp_avg_sq, void* param_bf16, size_t numel, float lr,
-                                     float beta1, float beta2, float eps, float weight_decay,
-                                     size_t step, hipStream_t stream) {
-    if (numel == 0) return kSuccess;
-    if (!param || !grad || !exp_avg || !exp_avg_sq) return kInvalidValue;
+// grad_scale (may be NULL): a factor on the gradient, read on the device
+static int adamw_master(float* param, const void* grad, const float* grad_scale, float* exp_avg,
+                        float* exp_avg_sq, void* param_bf16, size_t numel, float lr, float beta1,
+                        float beta2, float eps, float weight_decay, size_t step,
+                        hipStream_t stream) {
     ew::AdamArgs a;
     const int rc = ew::adam_args(lr, beta1, beta2, eps, weight_decay, step, &a);
     if (rc != kSuccess) return rc;
@@ -342,6 +343,28 @@ extern "C" int adamw_step_master_hip(float* param, const void* grad, float* exp_
                  ew::aligned16(exp_avg_sq) && ew::aligned16(param_bf16),
              &n8, &grid, 4 * ew::kMaxBlocks);  // 2-3 % faster than 4096 on 368M values
     EFLA_LAUNCH("adamw_master", ew::adamw_master_kernel, grid, dim3(ew::NTH), stream, param,
-                (const bf16*)grad, exp_avg, exp_avg_sq, (bf16*)param_bf16, (long)numel, n8, a);
+                (const bf16*)grad, exp_avg, exp_avg_sq, (bf16*)param_bf16, (long)numel, n8, a,
+                grad_scale);
     return (int)hipPeekAtLastError();
+}
+
+extern "C" int adamw_step_master_hip(float* param, const void* grad, float* exp_avg,
+                                     float* exp_avg_sq, void* param_bf16, size_t numel, float lr,
+                                     float beta1, float beta2, float eps, float weight_decay,
+                                     size_t step, hipStream_t stream) {
+    if (numel == 0) return kSuccess;
+    if (!param || !grad || !exp_avg || !exp_avg_sq) return kInvalidValue;
+    return adamw_master(param, grad, nullptr, exp_avg, exp_avg_sq, param_bf16, numel, lr, beta1,
+                        beta2, eps, weight_decay, step, stream);
+}
+
+extern "C" int adamw_step_master_scaled_hip(float* param, const void* grad,
+                                            const float* grad_scale, float* exp_avg,
+                                            float* exp_avg_sq, void* param_bf16, size_t numel,
+                                            float lr, float beta1, float beta2, float eps,
+                                            float weight_decay, size_t step, hipStream_t stream) {
+    if (numel == 0) return kSuccess;
+    if (!param || !grad || !grad_scale || !exp_avg || !exp_avg_sq) return kInvalidValue;
+    return adamw_master(param, grad, grad_scale, exp_avg, exp_avg_sq, param_bf16, numel, lr, beta1,
+                        beta2, eps, weight_decay, step, stream);
 }

@@ -8,6 +8,8 @@ and the GELU / AdamW kernels of kernels/cuda/include/kernels.h:171-189, 309-322.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from ._lib import check, lib
@@ -320,9 +322,11 @@ def adamw_step(param, grad, exp_avg, exp_avg_sq, lr, beta1=0.9, beta2=0.999, eps
 
 
 def adamw_step_master(param, grad, exp_avg, exp_avg_sq, lr, beta1=0.9, beta2=0.999, eps=1e-8,
-                      weight_decay=0.0, step=1, param_bf16=None) -> None:
+                      weight_decay=0.0, step=1, param_bf16=None, grad_scale=None) -> None:
     """In-place AdamW step on fp32 master weights / moments with a bf16 gradient;
-    ``param_bf16`` (optional) receives the new weights in bf16."""
+    ``param_bf16`` (optional) receives the new weights in bf16.  ``grad_scale``
+    (optional, one fp32 device value, as ``grad_norm`` returns it) multiplies the
+    gradient."""
     for t, n in ((param, "param"), (exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq")):
         _require(t, n, torch.float32, param.device)
     _require(grad, "grad", torch.bfloat16, param.device)
@@ -331,6 +335,16 @@ def adamw_step_master(param, grad, exp_avg, exp_avg_sq, lr, beta1=0.9, beta2=0.9
     for t in (grad, exp_avg, exp_avg_sq, param_bf16):
         if t is not None and t.numel() != param.numel():
             raise ValueError("adamw_step_master: sizes differ")
+    if grad_scale is not None:
+        _require(grad_scale, "grad_scale", torch.float32, param.device)
+        if grad_scale.numel() != 1:
+            raise ValueError("adamw_step_master: grad_scale must be one value")
+        rc = lib().adamw_step_master_scaled_hip(
+            _p(param), _p(grad), _p(grad_scale), _p(exp_avg), _p(exp_avg_sq), _p(param_bf16),
+            param.numel(), float(lr), float(beta1), float(beta2), float(eps),
+            float(weight_decay), int(step), _stream(param))
+        check(rc, "adamw_step_master_scaled_hip")
+        return
     rc = lib().adamw_step_master_hip(_p(param), _p(grad), _p(exp_avg), _p(exp_avg_sq),
                                      _p(param_bf16), param.numel(), float(lr), float(beta1),
                                      float(beta2), float(eps), float(weight_decay), int(step),
@@ -413,3 +427,197 @@ def cross_entropy_backward(grad_loss: torch.Tensor, logits: torch.Tensor, target
                                           float(label_smoothing), _stream(logits))
     check(rc, "cross_entropy_backward_hip")
     return g
+
+
+# ---------------------------------------------------------------------------
+# losses on rewards and preferences
+# ---------------------------------------------------------------------------
+def _loss_rows(logits, targets, **rows):
+    """(rows, vocab, row stride, dtype code) of 2-D logits whose rows are contiguous,
+    after checking the per-row operands given by name (None: absent)."""
+    _require(logits, "logits", contiguous=False)
+    if logits.dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {logits.dtype}")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be 2-D with contiguous rows")
+    N, V = logits.shape
+    # a single row's stride says nothing
+    ld = logits.stride(0) if N > 1 else max(V, 1)
+    if ld < V:
+        raise ValueError("logits rows overlap")
+    dev = logits.device
+    _require(targets, "targets", torch.int32, dev)
+    if targets.shape != (N,):
+        raise ValueError("targets must hold one token per row of logits")
+    for name, t in rows.items():
+        if t is not None:
+            _require(t, name, torch.float32, dev)
+            if t.shape != (N,):
+                raise ValueError(f"{name} must hold one value per row of logits")
+    return N, V, ld, DTYPE_CODES[logits.dtype]
+
+
+def _loss_grad(logits, need_grad, in_place, ld):
+    """The gradient's tensor (None without one) and its row stride."""
+    if not need_grad:
+        if in_place:
+            raise ValueError("in_place needs need_grad")
+        return None, 0
+    if in_place:
+        return logits, ld
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
+
+
+def token_logprob_forward(logits: torch.Tensor, targets: torch.Tensor,
+                          weights=None) -> torch.Tensor:
+    """log softmax(logits)[i, targets[i]], fp32 (rows,), for (rows, vocab) logits in
+    bf16, fp16 or fp32 (a row stride is fine).  A row whose weight (fp32 (rows,),
+    None: all count) is 0 is not read and gives 0."""
+    N, V, ld, dt = _loss_rows(logits, targets, weights=weights)
+    logp = torch.empty(N, dtype=torch.float32, device=logits.device)
+    rc = lib().token_logprob_forward_hip(_p(logits), _p(targets), _p(weights), _p(logp), N, V, ld,
+                                         dt, _stream(logits))
+    check(rc, "token_logprob_forward_hip")
+    return logp
+
+
+def policy_loss_forward_backward(logits: torch.Tensor, targets: torch.Tensor,
+                                 advantages: torch.Tensor, old_logp=None, ref_logp=None,
+                                 weights=None, clip_low: float = 0.2, clip_high: float = 0.2,
+                                 kl_coef: float = 0.0, in_place: bool = False,
+                                 need_grad: bool = True):
+    """(loss, logp, kl or None, dL/dlogits or None) of the clipped policy loss with a
+    KL term, from one read of the logits; L = loss.sum().
+
+    Per row, r = exp(logp - old_logp) and kl = exp(d) - 1 - d with d = ref_logp - logp:
+    ``loss = weight * (kl_coef * kl - min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A))``.
+    Without ``old_logp`` the sampling policy is this one (r = 1, with its gradient);
+    without ``ref_logp`` there is no kl; without ``weights`` every row has 1 / rows.
+    Rows of weight 0 are not read.  With ``in_place`` the gradient overwrites the logits."""
+    N, V, ld, dt = _loss_rows(logits, targets, advantages=advantages, old_logp=old_logp,
+                              ref_logp=ref_logp, weights=weights)
+    if advantages is None:
+        raise TypeError("advantages must be a tensor")
+    if ref_logp is None and kl_coef != 0:
+        raise ValueError("kl_coef needs ref_logp")
+    out = torch.empty(3 if ref_logp is not None else 2, N, dtype=torch.float32,
+                      device=logits.device)
+    loss, logp = out[0], out[1]
+    kl = out[2] if ref_logp is not None else None
+    g, ldg = _loss_grad(logits, need_grad, in_place, ld)
+    rc = lib().policy_loss_forward_backward_hip(
+        _p(logits), _p(targets), _p(advantages), _p(old_logp), _p(ref_logp), _p(weights),
+        _p(loss), _p(logp), _p(kl), _p(g), N, V, ld, ldg, float(clip_low), float(clip_high),
+        float(kl_coef), dt, _stream(logits))
+    check(rc, "policy_loss_forward_backward_hip")
+    return loss, logp, kl, g
+
+
+def preference_loss_forward_backward(logits: torch.Tensor, targets: torch.Tensor,
+                                     cu_seqlens: torch.Tensor, ref_logp=None, weights=None,
+                                     beta: float = 0.1, label_smoothing: float = 0.0,
+                                     in_place: bool = False, need_grad: bool = True):
+    """(loss (pairs,), rewards (2 pairs,), logp (rows,), dL/dlogits or None) of the
+    preference loss; L = loss.sum(), the mean over the pairs.
+
+    ``cu_seqlens`` (int32, 2 pairs + 1) packs the sequences, chosen and rejected in turn.
+    ``rewards[s] = beta * sum(weight * (logp - ref_logp))`` over sequence s and, with x a
+    pair's difference of rewards,
+    ``loss = (-(1 - e) log sigmoid(x) - e log sigmoid(-x)) / pairs``, e the label smoothing.
+    Rows of weight 0 (prompts, padding) are not read; without ``weights`` all count.
+    With ``in_place`` the gradient overwrites the logits."""
+    N, V, ld, dt = _loss_rows(logits, targets, ref_logp=ref_logp, weights=weights)
+    dev = logits.device
+    _require(cu_seqlens, "cu_seqlens", torch.int32, dev)
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() % 2 == 0:
+        raise ValueError("cu_seqlens must hold 2 pairs + 1 offsets")
+    P = cu_seqlens.numel() // 2
+    loss = torch.empty(P, dtype=torch.float32, device=dev)
+    rewards = torch.empty(2 * P, dtype=torch.float32, device=dev)
+    logp = torch.empty(N, dtype=torch.float32, device=dev)
+    g, ldg = _loss_grad(logits, need_grad, in_place, ld)
+    ws, wsb = None, 0
+    if need_grad and N:
+        wsb = lib().preference_loss_workspace_size(N)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    rc = lib().preference_loss_forward_backward_hip(
+        _p(logits), _p(targets), _p(ref_logp), _p(weights), _p(cu_seqlens), _p(loss),
+        _p(rewards), _p(logp), _p(g), P, N, V, ld, ldg, float(beta), float(label_smoothing), dt,
+        _p(ws), wsb, _stream(logits))
+    check(rc, "preference_loss_forward_backward_hip")
+    return loss, rewards, logp, g
+
+
+# ---------------------------------------------------------------------------
+# gradient norm and clipping
+# ---------------------------------------------------------------------------
+class GradList:
+    """The gradients that a training loop clips at every step, laid out once.
+
+    It keeps the tensors (contiguous, bf16, fp16 or fp32, on one device) and the device
+    table of their addresses; what they hold is read at each call.  Clipping writes into
+    ``outs`` (shaped and typed like the gradients), or in place without.  One call at a
+    time may use a list: two streams need two."""
+
+    def __init__(self, grads, outs=None):
+        self.grads = list(grads)
+        self.outs = None if outs is None else list(outs)
+        self._handle = None
+        if not self.grads:
+            raise ValueError("no gradients")
+        dev = self.grads[0].device
+        for t in self.grads:
+            _require(t, "a gradient", None, dev)
+            if t.dtype not in DTYPE_CODES:
+                raise ValueError(f"unsupported dtype {t.dtype}")
+        if self.outs is not None:
+            if len(self.outs) != len(self.grads):
+                raise ValueError("grads and outs differ in number")
+            for t, g in zip(self.outs, self.grads):
+                _require(t, "an output", g.dtype, dev)
+                if t.shape != g.shape:
+                    raise ValueError("an output's shape differs from its gradient's")
+        n = len(self.grads)
+        self.device = dev
+        ptrs = (ctypes.c_void_p * n)(*[_p(t) for t in self.grads])
+        outp = None if self.outs is None else (ctypes.c_void_p * n)(*[_p(t) for t in self.outs])
+        numels = (ctypes.c_size_t * n)(*[t.numel() for t in self.grads])
+        dts = (ctypes.c_int * n)(*[DTYPE_CODES[t.dtype] for t in self.grads])
+        handle = ctypes.c_void_p()
+        with torch.cuda.device(dev):
+            rc = lib().grad_list_create_hip(ctypes.byref(handle), ptrs, outp, numels, dts, n)
+        check(rc, "grad_list_create_hip")
+        self._handle = handle
+
+    def __del__(self):
+        if getattr(self, "_handle", None):
+            lib().grad_list_destroy_hip(self._handle)
+            self._handle = None
+
+
+def _grad_list(grads) -> GradList:
+    return grads if isinstance(grads, GradList) else GradList(grads)
+
+
+def grad_norm(grads, max_norm: float = float("inf")):
+    """(norm, coef) of a ``GradList`` (or tensors, for which one is made): the 2-norm over
+    every element and ``min(1, max_norm / (norm + 1e-6))``, fp32 device values of one
+    element.  ``coef`` goes to ``adamw_step_master(grad_scale=coef)``."""
+    gl = _grad_list(grads)
+    out = torch.empty(2, dtype=torch.float32, device=gl.device)
+    norm, coef = out[:1], out[1:]
+    rc = lib().grad_norm_hip(gl._handle, float(max_norm), _p(norm), _p(coef),
+                             _stream(out))
+    check(rc, "grad_norm_hip")
+    return norm.view(()), coef.view(())
+
+
+def clip_grad_norm(grads, max_norm: float) -> torch.Tensor:
+    """Scales the gradients of a ``GradList`` (or tensors, in place) by
+    ``min(1, max_norm / (norm + 1e-6))``; returns their norm (before), an fp32 device
+    value.  A list's ``outs`` receive the scaled gradients where it has them."""
+    gl = _grad_list(grads)
+    norm = torch.empty((), dtype=torch.float32, device=gl.device)
+    rc = lib().grad_clip_hip(gl._handle, float(max_norm), _p(norm), _stream(norm))
+    check(rc, "grad_clip_hip")
+    return norm

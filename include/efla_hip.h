@@ -472,6 +472,51 @@ int adamw_step_master_hip(float* param, const void* grad, float* exp_avg, float*
                           void* param_bf16, size_t numel, float lr, float beta1, float beta2,
                           float eps, float weight_decay, size_t step, hipStream_t stream);
 
+/* adamw_step_master_hip with the gradient taken times *grad_scale, a device value
+ * read when the kernel runs (grad_norm_hip's coef: the step on clipped gradients
+ * without the pass that writes them; the product is not rounded to bf16).  A factor
+ * of 1 gives adamw_step_master_hip's bits.  grad_scale NULL -> 1, else the same
+ * return codes. */
+int adamw_step_master_scaled_hip(float* param, const void* grad, const float* grad_scale,
+                                 float* exp_avg, float* exp_avg_sq, void* param_bf16,
+                                 size_t numel, float lr, float beta1, float beta2, float eps,
+                                 float weight_decay, size_t step, hipStream_t stream);
+
+/* ========================================================================
+ * Gradient norm and clipping (the reference's clip, optim.cu:221-232, 765-775,
+ * goes through the host between its reduction and its scaling)
+ *
+ * A list is what a training loop clips at every step: `count` gradients, each
+ * numels[i] elements of dtypes[i] (EFLA_DTYPE_*), contiguous, at any multiple
+ * of the element's size.  It holds their addresses (and a small device table,
+ * allocated here), so they have to stay where they are for as long as it is used;
+ * their values are read at each call.  One call at a time uses a list: its scratch
+ * is its own.
+ * ======================================================================== */
+
+/* Makes a list for the current device.  Clipping writes to outs[i], which may be
+ * grads[i] (outs NULL: all in place); an output that overlaps any other gradient
+ * or output is undefined.  A gradient of no element may be NULL.  NULL arguments,
+ * an unknown dtype or a misaligned pointer -> 1; more than 2^45 elements in all
+ * -> 9.  Waits for its copy to the device: not for use under stream capture. */
+int grad_list_create_hip(void** list, const void* const* grads, void* const* outs,
+                         const size_t* numels, const int* dtypes, size_t count);
+/* Frees it (NULL -> 0), after waiting for the device. */
+int grad_list_destroy_hip(void* list);
+
+/* norm[0] = sqrt(sum g^2) over every element of every gradient, and, unless coef is
+ * NULL, coef[0] = min(1, max_norm / (norm + 1e-6)); device values, fp32.  Squares
+ * and sums are 64 bits, in a fixed order.  No gradient: norm 0, coef 1.  An
+ * infinite or NaN gradient: norm and coef as the formula (coef 0 or NaN).
+ * NULL list or norm, max_norm negative or NaN -> 1; another device current than
+ * the list's -> 101. */
+int grad_norm_hip(const void* list, float max_norm, float* norm, float* coef,
+                  hipStream_t stream);
+
+/* The norm, and outs[i] = coef grads[i] in fp32, rounded once to the gradient's
+ * type.  Where coef is 1 nothing is written in place.  Same return codes. */
+int grad_clip_hip(const void* list, float max_norm, float* norm, hipStream_t stream);
+
 /* No reference counterpart: the per-token beta gate of a model whose fused
  * projection row ends in `cols` beta logits (the config-4 model, one logit
  * per head).  beta[r*cols + c] = bf16(sigmoid(float(logits[r*ld + c]))) for
@@ -539,6 +584,70 @@ int cross_entropy_forward_backward_hip(const void* logits, const int32_t* target
                                        const float* grad_loss, float* loss, void* grad_logits,
                                        size_t batch_size, size_t vocab_size,
                                        float label_smoothing, hipStream_t stream);
+
+/* ========================================================================
+ * Losses of training on rewards and preferences (no reference counterpart)
+ *
+ * Logits (rows, vocab), dtype EFLA_DTYPE_F32, _F16 or _BF16, `ld` elements from a row
+ * to the next (ld >= vocab), at any multiple of the element's size.  targets int32:
+ * the token whose log-probability
+ *   logp[i] = z_i,t - logsumexp(z_i)
+ * counts.  weights (rows) fp32: a row of weight 0 is not read, and its outputs and
+ * gradient are 0 whatever else is there.  In another row a target outside [0,
+ * vocab) gives NaN and a zero gradient row; a +inf or NaN logit, or nothing but -inf,
+ * gives NaN for the row's outputs and gradient.  The arithmetic is fp32 or more;
+ * gradients are rounded once, to the logits' type.  grad_logits (rows, vocab) with
+ * ld_grad elements a row may be the logits themselves (then ld_grad == ld), or NULL
+ * for the loss alone; columns past vocab are not touched.  Results do not depend on
+ * scheduling.  rows == 0 -> 0; a NULL or misaligned pointer, an unknown dtype, vocab
+ * == 0 or ld < vocab -> 1; rows or vocab past 2^31 - 1 -> 9.
+ * ======================================================================== */
+
+/* logp (rows) fp32 of the targets: the frozen model's or the sampling policy's side of
+ * the losses below.  weights may be NULL (every row counts). */
+int token_logprob_forward_hip(const void* logits, const int32_t* targets, const float* weights,
+                              float* logp, size_t rows, size_t vocab_size, size_t ld, int dtype,
+                              hipStream_t stream);
+
+/* The clipped policy loss with a KL term, per row
+ *   r = e^(logp - old_logp),  kl = e^(ref_logp - logp) - 1 - (ref_logp - logp)
+ *   loss[i] = w_i (kl_coef kl - min(r A_i, clip(r, 1 - clip_low, 1 + clip_high) A_i))
+ * and d sum(loss) / d logits from one read of the logits (two where a row is more than
+ * a workgroup's registers hold).  old_logp NULL: the policy itself (r = 1, with
+ * the gradient of r).  At a border of the clipping the gradient is the unclipped
+ * side's.  weights NULL: 1 / rows each, so that sum(loss) is the mean.  loss, logp and
+ * kl (may be NULL; else it needs ref_logp) are fp32 (rows).  clip_low outside
+ * [0, 1], clip_high or kl_coef negative, NaN, or kl_coef infinite or without
+ * ref_logp -> 1. */
+int policy_loss_forward_backward_hip(const void* logits, const int32_t* targets,
+                                     const float* advantages, const float* old_logp,
+                                     const float* ref_logp, const float* weights, float* loss,
+                                     float* logp, float* kl, void* grad_logits, size_t rows,
+                                     size_t vocab_size, size_t ld, size_t ld_grad,
+                                     float clip_low, float clip_high, float kl_coef, int dtype,
+                                     hipStream_t stream);
+
+/* Bytes of preference_loss_forward_backward_hip's workspace (16-byte aligned). */
+size_t preference_loss_workspace_size(size_t rows);
+
+/* The preference loss over packed sequences: cu_seqlens int32 (2 pairs + 1), the rows
+ * of sequence s are [cu_seqlens[s], cu_seqlens[s + 1]), sequence 2p the chosen and 2p + 1
+ * the rejected one of pair p.  With D_s = sum over its rows of w (logp - ref_logp),
+ *   rewards[s] = beta D_s,  x = rewards[2p] - rewards[2p + 1],
+ *   loss[p] = (-(1 - eps) log sigmoid(x) - eps log sigmoid(-x)) / pairs
+ * and d sum(loss) / d logits.  ref_logp NULL: 0; weights NULL: 1 each (1 / length
+ * gives means instead of sums).  Sums are 64 bits, in a fixed order.  Sequences may
+ * be empty; offsets are clamped to the rows and to their predecessors; rows outside
+ * of every sequence have gradient 0.  A NaN in one row makes its pair's loss, rewards
+ * and gradient NaN.  workspace NULL: the stream's cached one (only a call with
+ * grad_logits needs any).  beta not positive and finite, eps outside [0, 1), or a
+ * workspace that is too small -> 1. */
+int preference_loss_forward_backward_hip(
+    const void* logits, const int32_t* targets, const float* ref_logp, const float* weights,
+    const int32_t* cu_seqlens, float* loss, float* rewards, float* logp, void* grad_logits,
+    size_t pairs, size_t rows, size_t vocab_size, size_t ld, size_t ld_grad, float beta,
+    float label_smoothing, int dtype, void* workspace, size_t workspace_bytes,
+    hipStream_t stream);
 
 /* ========================================================================
  * Sequence packing (host, no GPU)

@@ -30,6 +30,11 @@ Contents and what pins each part (tests/test_oracle_*.py):
 * ``layernorm_fwd`` / ``layernorm_bwd`` -- layernorm.cu:133-183 and the
   textbook gradient.  Pinned by the per-row mean 0 / variance 1 invariant and
   torch fp64 autograd.
+* ``token_logprob`` / ``policy_loss`` / ``preference_loss`` / ``clip_coef`` -- fp64
+  numpy of the losses on rewards and preferences (no reference counterpart)
+  and of gradient clipping.  Pinned by torch fp64 autograd of the losses as
+  written with its own log_softmax / logsigmoid / clamp, central differences and
+  torch's clip_grad_norm_.
 * ``rmsnorm_fwd`` / ``rmsnorm_bwd`` -- layernorm.cu:15-127 with the exact
   gradient (the reference's dx drops a factor rs^2).  Pinned by the per-row
   mean(y^2) = 1 invariant (w = 1, eps = 0), torch's rms_norm and fp64
@@ -615,6 +620,99 @@ def cross_entropy_bwd(grad_loss, logits, targets, label_smoothing=0.0):
     p[np.arange(B)[ok], t[ok]] -= 1.0
     coef = np.where(ok, np.asarray(grad_loss, dtype=np.float64) * (1 - label_smoothing) / B, 0.0)
     return p * coef[:, None]
+
+
+def _row_parts(logits, targets, weights):
+    """(logp, softmax, rows that count, rows whose target is a token), fp64; logp 0 in
+    rows of weight 0, NaN where the target is none."""
+    z = np.asarray(logits, dtype=np.float64)
+    t = np.asarray(targets).astype(np.int64)
+    N, V = z.shape
+    on = np.ones(N, bool) if weights is None else np.asarray(weights) != 0
+    tok = (t >= 0) & (t < V)
+    z = np.where(on[:, None], z, 0.0)
+    with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
+        m = z.max(axis=1, keepdims=True)
+        e = np.exp(z - np.where(np.isinf(m) & (m < 0), 0.0, m))
+        s = e.sum(axis=1, keepdims=True)
+        zt = z[np.arange(N), np.where(tok, t, 0)]
+        logp = np.where(tok, (zt - m[:, 0]) - np.log(s[:, 0]), np.nan)
+        p = e / s
+    return np.where(on, logp, 0.0), p, on, tok
+
+
+def token_logprob(logits, targets, weights=None):
+    """log softmax(z_i)[t_i], fp64: 0 in rows of weight 0, NaN for a target outside
+    the vocabulary."""
+    return _row_parts(logits, targets, weights)[0]
+
+
+def _row_gradient(p, targets, on, tok, dlogp):
+    """dlogp_i ([j = t_i] - softmax_ij); zero rows without weight or target."""
+    rows = np.flatnonzero(on & tok)
+    g = np.zeros_like(p)
+    g[rows] = -dlogp[rows, None] * p[rows]
+    g[rows, np.asarray(targets).astype(np.int64)[rows]] += dlogp[rows]
+    return g
+
+
+def policy_loss(logits, targets, advantages, old_logp=None, ref_logp=None, weights=None,
+                clip_low=0.2, clip_high=0.2, kl_coef=0.0):
+    """(loss, logp, kl, dlogp, dlogits) of the clipped policy loss with the KL estimate
+    e^d - 1 - d, d = ref - logp; per row, fp64.  No counterpart in the reference."""
+    logp, p, on, tok = _row_parts(logits, targets, weights)
+    N = len(logp)
+    w = np.full(N, 1.0 / N) if weights is None else np.asarray(weights, dtype=np.float64)
+    a = np.asarray(advantages, dtype=np.float64)
+    with np.errstate(invalid="ignore", over="ignore"):
+        r = np.ones(N) if old_logp is None else np.exp(logp - np.asarray(old_logp, np.float64))
+        low, high = 1.0 - clip_low, 1.0 + clip_high
+        loss = -np.minimum(r * a, np.clip(r, low, high) * a)
+        d = np.where(np.where(a >= 0, r <= high, r >= low), -a * r, 0.0)
+        kl = np.zeros(N)
+        if ref_logp is not None:
+            x = np.asarray(ref_logp, np.float64) - logp
+            kl = np.expm1(x) - x
+            if kl_coef != 0:
+                loss, d = loss + kl_coef * kl, d - kl_coef * np.expm1(x)
+        loss, d = w * loss, w * d
+    loss = np.where(on, np.where(tok, loss, np.nan), 0.0)
+    kl = np.where(on, np.where(tok, kl, np.nan), 0.0)
+    d = np.where(on & tok, d, 0.0)
+    return loss, logp, kl, d, _row_gradient(p, targets, on, tok, d)
+
+
+def preference_loss(logits, targets, cu_seqlens, ref_logp=None, weights=None, beta=0.1,
+                    label_smoothing=0.0):
+    """(loss, rewards, logp, dlogp, dlogits) of the preference loss over packed
+    sequences, chosen and rejected in turn, fp64.  No counterpart in the reference."""
+    logp, p, on, tok = _row_parts(logits, targets, weights)
+    N, cu = len(logp), np.asarray(cu_seqlens).astype(np.int64)
+    P = len(cu) // 2
+    w = np.ones(N) if weights is None else np.asarray(weights, dtype=np.float64)
+    ref = np.zeros(N) if ref_logp is None else np.asarray(ref_logp, dtype=np.float64)
+    term = np.where(on, w * (logp - np.where(on, ref, 0.0)), 0.0)
+    rewards = beta * np.array([term[cu[s]:cu[s + 1]].sum() for s in range(2 * P)])
+    x = rewards[0::2] - rewards[1::2]
+    e = label_smoothing
+    loss = ((1 - e) * np.logaddexp(0.0, -x) + e * np.logaddexp(0.0, x)) / P
+    sig = np.exp(-np.logaddexp(0.0, -x))
+    gis = np.exp(-np.logaddexp(0.0, x))
+    dx = (e * sig - (1 - e) * gis) / P
+    d = np.zeros(N)
+    for i in range(P):
+        for s, sign in ((2 * i, 1.0), (2 * i + 1, -1.0)):
+            d[cu[s]:cu[s + 1]] = sign * beta * dx[i] * w[cu[s]:cu[s + 1]]
+    d = np.where(on & tok, d, 0.0)
+    return loss, rewards, logp, d, _row_gradient(p, targets, on, tok, d)
+
+
+def clip_coef(grads, max_norm):
+    """(2-norm over all gradients, min(1, max_norm / (norm + 1e-6))), fp64 (the formula
+    of the reference's clip, optim.cu:221-232)."""
+    norm = np.sqrt(sum(float((np.asarray(g, dtype=np.float64) ** 2).sum()) for g in grads))
+    c = max_norm / (norm + 1e-6)
+    return norm, (1.0 if c > 1 else c)
 
 
 def embedding_fwd(indices, weight):
