@@ -503,3 +503,185 @@ def test_offsets_past_32_bits():
     a = nn.preference_loss_forward_backward(z, d["t"], cu, in_place=True)
     b = nn.preference_loss_forward_backward(d["z"], d["t"], cu)
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def large_rows(d, cu, beta, eps, rows=500):
+    """The preference loss in 64 bits on the GPU, some rows of the logits at a time:
+    (loss, rewards, logp, each row's factor)."""
+    z, t = d["z"], d["t"].long()
+    N, V = z.shape
+    on = d["w"] != 0
+    logp = torch.zeros(N, dtype=torch.float64, device="cuda")
+    for a in range(0, N, rows):
+        zi = z[a:a + rows].double()
+        lp = zi.gather(1, t[a:a + rows, None])[:, 0] - torch.logsumexp(zi, 1)
+        logp[a:a + rows] = torch.where(on[a:a + rows], lp, 0.0)
+    term = torch.where(on, d["w"].double() * (logp - d["ref"].double()), 0.0).cpu().numpy()
+    r = beta * np.array([term[a:b].sum() for a, b in zip(cu[:-1], cu[1:])])
+    x, P = r[0::2] - r[1::2], len(cu) // 2
+    loss = ((1 - eps) * np.logaddexp(0, -x) + eps * np.logaddexp(0, x)) / P
+    dx = (eps * np.exp(-np.logaddexp(0, -x)) - (1 - eps) * np.exp(-np.logaddexp(0, x))) / P
+    f = np.zeros(N)
+    for i in range(P):
+        f[cu[2 * i]:cu[2 * i + 1]] = beta * dx[i]
+        f[cu[2 * i + 1]:cu[2 * i + 2]] = -beta * dx[i]
+    return loss, r, logp, torch.from_numpy(f).cuda() * d["w"].double()
+
+
+# logits of over 256 MiB in rows of at least 96 KiB: statistics and gradients in one launch
+LARGE = [(2700, 50257, torch.bfloat16), (1101, 61003, torch.float32), (2111, 65537, torch.float16)]
+LARGE_CU = {
+    "short pairs": lambda N: [0, 3, 3, 3, 3, *range(10, N - 37, 29)],
+    "ragged, rows outside": lambda N: [5, 40, 41, 600, 600, 600, 600, 900, N - 9],
+    "one pair": lambda N: [0, N // 3, N],
+}
+
+
+@pytest.mark.parametrize("shape", LARGE, ids=["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("which", LARGE_CU)
+def test_preference_of_more_logits_than_the_cache(shape, which):
+    from ceo_amd import nn
+
+    N, V, dtype = shape
+    announce(f"preference {N} x {V} {dtype}, {which}")
+    g = torch.Generator(device="cuda").manual_seed(N)
+    z = torch.empty(N, V, dtype=dtype, device="cuda")
+    for a in range(0, N, 256):
+        z[a:a + 256] = torch.randn(min(256, N - a), V, generator=g, device="cuda") * 2.5
+    d = dict(z=z, t=torch.randint(0, V, (N,), generator=g, device="cuda", dtype=torch.int32),
+             w=torch.rand(N, generator=g, device="cuda") + 0.1,
+             ref=torch.randn(N, generator=g, device="cuda") * 0.3 - 13.0)
+    d["w"][torch.rand(N, generator=g, device="cuda") < 0.3] = 0.0
+    z[d["w"] == 0, :64] = float("nan")  # not read
+    cu = LARGE_CU[which](N)
+    cu = cu if len(cu) % 2 else cu[:-1]
+    beta, eps = 0.02, 0.1
+    args = (d["t"], torch.tensor(cu, dtype=torch.int32, device="cuda"), d["ref"], d["w"], beta, eps)
+    got = nn.preference_loss_forward_backward(z, *args)
+    rl, rr, rlp, f = large_rows(d, cu, beta, eps)
+    U64 = rel(V)
+    dl = U * rlp.abs().cpu().numpy() + 64 * U + U64
+    aw = d["w"].cpu().numpy()
+    dr = np.array([beta * (aw * dl)[a:b].sum() for a, b in zip(cu[:-1], cu[1:])])
+    dx = dr[0::2] + dr[1::2]
+    within(got[2], rlp.cpu().numpy(), dl, "logp")
+    within(got[1], rr, dr + U * np.abs(rr) + 1e-30, "rewards")
+    within(got[0], rl, dx / len(rl) + 2 * U * np.abs(rl), "loss")
+    de = np.zeros(N)
+    for i in range(len(rl)):
+        de[cu[2 * i]:cu[2 * i + 2]] = beta * (0.25 * dx[i] / len(rl))
+    de = torch.from_numpy(de).cuda() * d["w"].double() + 4 * U * f.abs()
+    for a in range(0, N, 300):
+        on = f[a:a + 300, None] != 0
+        p = torch.softmax(torch.where(on, z[a:a + 300].double(), 0.0), 1)
+        want = torch.where(on, -f[a:a + 300, None] * p, 0.0)
+        i = torch.arange(len(p), device="cuda")
+        want[i, d["t"][a:a + 300].long()] += f[a:a + 300]
+        p[i, d["t"][a:a + 300].long()] += 1.0
+        tol = (want.abs() * torch.finfo(dtype).eps / 2 + TINY[dtype]
+               + p * (f[a:a + 300, None].abs() * U64 + de[a:a + 300, None]) * 1.01)
+        assert bool(((got[3][a:a + 300].double() - want).abs() <= tol).all())
+    # the same bits again, without the gradient, on a stream of its own, and in place
+    again = nn.preference_loss_forward_backward(z, *args)
+    only = nn.preference_loss_forward_backward(z, *args, need_grad=False)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        other = nn.preference_loss_forward_backward(z, *args)
+    stream.synchronize()
+    place = nn.preference_loss_forward_backward(z, *args, in_place=True)
+    for p in (again, other, place):
+        assert all(torch.equal(a, b) for a, b in zip(got, p))
+    assert all(torch.equal(a, b) for a, b in zip(got[:3], only[:3]))
+
+
+def test_large_preference_offsets_graph_and_bad_rows():
+    """Of more logits than the cache: offsets that fall are those before them, a NaN stays
+    in its pair, targets that are no tokens; and a graph gives the eager bits."""
+    from ceo_amd import nn
+
+    N, V = 2700, 50257
+    announce("large preference: offsets, graph, NaN")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    z = torch.empty(N, V, dtype=torch.bfloat16, device="cuda")
+    z.normal_(0, 2, generator=g)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda", dtype=torch.int32)
+    ref = torch.full((N,), -12.5, device="cuda")
+
+    def call(cu, **kw):
+        return nn.preference_loss_forward_backward(
+            z, t, torch.tensor(cu, dtype=torch.int32, device="cuda"), ref, beta=0.01, **kw)
+    want = call([0, 700, 1500, 1500, 2600])
+    got = call([-9, 700, 1500, 1200, 2600])
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert not want[3][2600:].any() and bool(want[3][:2600].any(1).all())
+    got = call([0, 700, 1500, 1500, 2600, 2600, 1 << 30])  # one more pair: its only row set [2600, N)
+    assert bool(got[3][2600:].any(1).all())
+    none = call([0])
+    assert none[0].shape == (0,) and not none[3].any() and torch.equal(none[2], want[2])
+    keep = t[1000].item()
+    t[1000] = V
+    got = call([0, 700, 1500, 1500, 2600])
+    assert bool(got[0][0].isnan()) and not got[3][1000].any() and bool(got[3][999].isnan().all())
+    assert torch.equal(got[3][1500:], want[3][1500:]) and torch.equal(got[0][1:], want[0][1:])
+    t[1000] = keep
+    cu = torch.tensor([0, 700, 1500, 1500, 2600], dtype=torch.int32, device="cuda")
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        out = nn.preference_loss_forward_backward(z, t, cu, ref, beta=0.01)
+    for k in range(3):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out)), k
+        call([0, 100, 200])
+
+
+def test_small_offsets_that_fall():
+    """Offsets that fall are taken as those before them: pairs never share rows."""
+    from ceo_amd import nn
+
+    x, d, _ = make(61, 12, 300, torch.bfloat16, masked=0.0)
+
+    def call(cu):
+        return nn.preference_loss_forward_backward(
+            d["z"], d["t"], torch.tensor(cu, dtype=torch.int32, device="cuda"),
+            ref_logp=d["ref"], weights=d["w"])
+    a, b = call([0, 8, 10, 9, 7, 6, 12]), call([0, 8, 10, 10, 10, 10, 12])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_more_rows_than_one_grid_dimension(dtype):
+    """Rows past 2^20, which a grid's second dimension holds."""
+    from ceo_amd import nn
+
+    N, V = (1 << 20) + 4099, 5
+    announce(f"{N} rows {dtype}")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    z = torch.randn(N, V, generator=g, device="cuda").to(dtype)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda", dtype=torch.int32)
+    adv = torch.randn(N, generator=g, device="cuda")
+    lp = torch.log_softmax(z.double(), 1)
+    ref = lp.gather(1, t[:, None].long())[:, 0]
+    tol = U * ref.abs() + U * 32 + rel(V)
+    got = nn.token_logprob_forward(z, t)
+    assert bool(((got.double() - ref).abs() <= tol).all())
+    w = torch.ones(N, device="cuda")
+    loss, logp, _, grad = nn.policy_loss_forward_backward(z, t, adv, weights=w)
+    one = torch.nn.functional.one_hot(t.long(), V).double()
+    want = -adv.double()[:, None] * (one - lp.exp())
+    eps = torch.finfo(dtype).eps
+    room = want.abs() * eps / 2 + TINY[dtype] + adv.double().abs()[:, None] * (one + lp.exp()) * (
+        rel(V) + 12 * U)
+    assert bool(((grad.double() - want).abs() <= room).all())
+    assert torch.equal(logp, got)
+    cu = torch.tensor([0, N // 2, N], dtype=torch.int32, device="cuda")
+    _, _, plp, pg = nn.preference_loss_forward_backward(z, t, cu, ref_logp=got, beta=0.5)
+    assert torch.equal(plp, got)
+    want = -0.25 * (one - lp.exp())  # x = 0: half of beta, minus for the chosen
+    want[N // 2:] *= -1
+    room = want.abs() * (eps / 2 + 8 * U) + TINY[dtype] + (one + lp.exp()) * rel(V)
+    assert bool(((pg.double() - want).abs() <= room).all())
