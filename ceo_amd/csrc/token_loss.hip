@@ -62,6 +62,12 @@ struct Vec {
 __device__ __forceinline__ float exp_neg(float d) {
     return __builtin_amdgcn_exp2f(fmaf(d, kLog2e, d * kLog2eLow));
 }
+// the same for a gradient of type T: in 16 bits its own rounding hides the constant's
+template <typename T>
+__device__ __forceinline__ float exp_grad(float d) {
+    if constexpr (sizeof(T) == 4) return exp_neg(d);
+    return __builtin_amdgcn_exp2f(d * kLog2e);
+}
 
 // log s for s > 0, in 64 bits from one v_log_f32 of the mantissa: its error is that
 // of a number in [-1, 0), not that of log2 s
@@ -100,17 +106,21 @@ __device__ __forceinline__ Stat join_waves(Stat a, Stat* sm) {
     return a;
 }
 
-// A row as its whole vectors at 16-byte boundaries and the elements before the first and
-// behind the last of them, one to a thread.  Loads that are not aligned cost a fifth
-// (log-probabilities of 4096 x 50257 in bf16: 100 us against 80), stores, which the cache
-// joins, 3 %: the boundaries are those of the logits, also where the gradient has others.
+// A row as its whole vectors from a boundary on and the elements before the first and
+// behind the last of them, one to a thread.  The boundary is a cache line's, so that no
+// line is two waves' (in fp32 4096 x 50257 327 us against 305 where it is not), in short rows
+// 16 bytes: loads that are not aligned to these cost a fifth (log-probabilities of
+// 4096 x 50257 in bf16: 100 us against 80).  The boundaries are those of the logits, also
+// where the gradient has others: stores, which the cache joins, lose 3 %.
+constexpr int kLineVocab = 4096, kLineThreads = 128;  // its edges: up to 70 elements
+
 template <typename T>
 struct Span {
     static constexpr int N = Vec<T>::N;
     int head, nv, edges;
 
     __device__ __forceinline__ Span(const T* z, int V) {
-        const int h = (int)(-(uintptr_t)z % 16 / sizeof(T));
+        const int h = (int)(-(uintptr_t)z % (V >= kLineVocab ? 128 : 16) / sizeof(T));
         head = h < V ? h : V;
         nv = (V - head) / N;
         edges = V - nv * N;
@@ -188,11 +198,11 @@ struct Row {
             if (c >= p.nv) continue;
             typename Vec<T>::Full y = packed(x[i]);
 #pragma unroll
-            for (int j = 0; j < N; ++j) y[j] = (T)(k * exp_neg((float)y[j] - r));
+            for (int j = 0; j < N; ++j) y[j] = (T)(k * exp_grad<T>((float)y[j] - r));
             Vec<T>::template store<PAST>(g + p.vec(c), y);
         }
         if (threadIdx.x < p.edges)
-            g[p.edge(threadIdx.x)] = (T)(k * exp_neg((float)edge - r));
+            g[p.edge(threadIdx.x)] = (T)(k * exp_grad<T>((float)edge - r));
     }
 };
 
@@ -254,13 +264,13 @@ struct Row<T, 0> {
                 const int c = c0 + u * blockDim.x;
                 if (c >= p.nv) continue;
 #pragma unroll
-                for (int j = 0; j < N; ++j) y[u][j] = (T)(k * exp_neg((float)y[u][j] - r));
+                for (int j = 0; j < N; ++j) y[u][j] = (T)(k * exp_grad<T>((float)y[u][j] - r));
                 Vec<T>::template store<PAST>(g + p.vec(c), y[u]);
             }
         }
         if (threadIdx.x < p.edges) {
             const int c = p.edge(threadIdx.x);
-            g[c] = (T)(k * exp_neg((float)z[c] - r));
+            g[c] = (T)(k * exp_grad<T>((float)z[c] - r));
         }
     }
 };
@@ -279,12 +289,11 @@ __device__ __forceinline__ void target_grad(T* g, const Span<T>& p, int t, float
 
 template <bool PAST, typename T>
 __device__ __forceinline__ void row_zero(T* g, int V) {
-    constexpr int N = Vec<T>::N;
     const typename Vec<T>::Full zero = {};
-    const int nv = V / N;
-    for (int c = threadIdx.x; c < nv; c += blockDim.x) Vec<T>::template store<PAST>(g + (long)c * N, zero);
-    const int c = nv * N + threadIdx.x;
-    if (c < V) g[c] = (T)0.f;
+    const Span<T> p(g, V);
+    for (int c = threadIdx.x; c < p.nv; c += blockDim.x)
+        Vec<T>::template store<PAST>(g + p.vec(c), zero);
+    if ((int)threadIdx.x < p.edges) g[p.edge(threadIdx.x)] = (T)0.f;
 }
 
 // Rows of a grid that has a second dimension where one would not hold them.
@@ -751,13 +760,15 @@ struct Form {
     int nv;
     unsigned threads;
 };
-static Form form_of(size_t vocab, int dtype, int least) {
+static Form form_of(size_t vocab, int dtype, int least, int most) {
     const size_t nv = vocab / (16 / dtype_size(dtype));
     int k = least;
-    while (k <= 16 && nv > (size_t)k * kMaxThreads) k *= 2;
-    if (k > 16) return Form{0, kMaxThreads};
-    const size_t need = nv > 0 ? (nv + k - 1) / k : 1;
-    return Form{k, (unsigned)((need + kWave - 1) / kWave * kWave)};
+    while (k <= most && nv > (size_t)k * kMaxThreads) k *= 2;
+    if (k > most) return Form{0, kMaxThreads};
+    const size_t least_threads = vocab >= kLineVocab ? kLineThreads : kWave;
+    const size_t need = (nv + k - 1) / k;
+    return Form{k, need < least_threads ? (unsigned)least_threads
+                                        : (unsigned)((need + kWave - 1) / kWave * kWave)};
 }
 
 #define TL_PAST(past, PAST, ...)        \
@@ -846,7 +857,7 @@ extern "C" int token_logprob_forward_hip(const void* logits, const int32_t* targ
     if (rc != kSuccess) return rc;
     if (!logp) return kInvalidValue;
     return tl::logprob(logits, targets, weights, logp, nullptr, nullptr, rows, vocab_size, ld,
-                       dtype, tl::form_of(vocab_size, dtype, 8), stream);
+                       dtype, tl::form_of(vocab_size, dtype, 8, 8), stream);
 }
 
 extern "C" int policy_loss_forward_backward_hip(
@@ -869,7 +880,7 @@ extern "C" int policy_loss_forward_backward_hip(
     a.rows = (long)rows, a.V = (int)vocab_size, a.ld = (long)ld, a.ldg = (long)ld_grad;
     a.low = 1.f - clip_low, a.high = 1.f + clip_high, a.kl_coef = kl_coef;
     a.even = 1.f / (float)rows;
-    const tl::Form f = tl::form_of(vocab_size, dtype, 4);
+    const tl::Form f = tl::form_of(vocab_size, dtype, 4, 16);
     TL_TYPED(dtype, T, {
         TL_FORM(f, NV, {
             TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
@@ -943,7 +954,7 @@ extern "C" int preference_loss_forward_backward_hip(
     float2* stat = (float2*)ws;
     float* coef = stat ? (float*)(stat + rows) : nullptr;
     if (rows != 0) {
-        const tl::Form f = draws ? tl::Form{0, threads} : tl::form_of(vocab_size, dtype, 8);
+        const tl::Form f = draws ? tl::Form{0, threads} : tl::form_of(vocab_size, dtype, 8, 8);
         const int rc = tl::logprob(logits, targets, weights, logp, stat, coef, rows, vocab_size,
                                    ld, dtype, f, stream);
         if (rc != kSuccess) return rc;
