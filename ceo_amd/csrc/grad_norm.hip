@@ -7,7 +7,7 @@
 //
 // The tensors' addresses, sizes and types are put into a device table once, when
 // the list is created; a call is then two launches whatever their number.  The
-// elements are dealt out in units of kUnit; a map gives each unit's tensor.  The
+// elements are dealt out in units of 16 KiB; a map gives each unit's tensor.  The
 // first kernel leaves one sum per workgroup, the second adds them, in the same order
 // in every workgroup, so the norm does not depend on scheduling.  Squares and sums are
 // 64 bits: the norm of any finite gradients is right, also where a square leaves
@@ -25,8 +25,8 @@
 namespace efla {
 namespace gn {
 
-constexpr int NT = 256;
-constexpr size_t kUnit = 16384;     // elements
+constexpr int NT = 256, kVecs = 4;
+constexpr size_t kUnit = NT * kVecs * 16;  // bytes
 constexpr unsigned kMaxGrid = 2048;  // workgroups, and sums they leave
 
 struct Entry {
@@ -40,47 +40,65 @@ struct Entry {
 // A list's device memory: entries, then the units' map, then the workgroups' sums.
 struct List {
     int device;
-    size_t count, units;
+    size_t count, units, bytes;
     Entry* entries;
     uint32_t* map;
     double* part;
 };
 
+// A unit, n elements from p on, in a workgroup's registers: 16-byte vectors from a cache
+// line's start on, kVecs to a thread, and the elements before and behind them (70 at
+// most), one to a thread.
 template <typename T>
-struct Vec {
+struct Unit {
     static constexpr int N = 16 / sizeof(T);
     typedef __attribute__((__vector_size__(16))) T Full;
     typedef Full Any __attribute__((aligned(sizeof(T))));
+    int head, nv, edges, edge;
+    Full x[kVecs];
+    T one;
+
+    __device__ __forceinline__ Unit(const T* p, int n) {
+        const int h = (int)(-(uintptr_t)p % 128 / sizeof(T));
+        head = h < n ? h : n;
+        nv = (n - head) / N;
+        edges = n - nv * N;
+        edge = (int)threadIdx.x < head ? threadIdx.x : threadIdx.x + nv * N;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int c = threadIdx.x + i * NT;
+            x[i] = Full{};
+            if (c < nv) x[i] = *reinterpret_cast<const Any*>(p + head + c * N);
+        }
+        one = (T)0.f;
+        if ((int)threadIdx.x < edges) one = p[edge];
+    }
+    __device__ __forceinline__ double square_sum() const {
+        double s = (double)(float)one * (double)(float)one;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) s = fma((double)(float)x[i][j], (double)(float)x[i][j], s);
+        return s;
+    }
+    template <bool PAST>
+    __device__ __forceinline__ void scale(T* q, float f) const {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int c = threadIdx.x + i * NT;
+            if (c >= nv) continue;
+            Full y;
+#pragma unroll
+            for (int j = 0; j < N; ++j) y[j] = (T)((float)x[i][j] * f);
+            Any* to = reinterpret_cast<Any*>(q + head + c * N);
+            if constexpr (PAST)
+                __builtin_nontemporal_store(y, to);
+            else
+                *to = y;
+        }
+        if ((int)threadIdx.x < edges) q[edge] = (T)((float)one * f);
+    }
 };
-
-template <typename T>
-__device__ __forceinline__ double square_sum(const T* p, long n) {
-    constexpr int N = Vec<T>::N;
-    double s = 0.0;
-    const long nv = n / N;
-    for (long c = threadIdx.x; c < nv; c += NT) {
-        const typename Vec<T>::Full x = *reinterpret_cast<const typename Vec<T>::Any*>(p + c * N);
-#pragma unroll
-        for (int i = 0; i < N; ++i) s = fma((double)(float)x[i], (double)(float)x[i], s);
-    }
-    const long c = nv * N + threadIdx.x;
-    if (c < n) s = fma((double)(float)p[c], (double)(float)p[c], s);
-    return s;
-}
-
-template <typename T>
-__device__ __forceinline__ void scale(const T* p, T* q, long n, float f) {
-    constexpr int N = Vec<T>::N;
-    const long nv = n / N;
-    for (long c = threadIdx.x; c < nv; c += NT) {
-        typename Vec<T>::Full x = *reinterpret_cast<const typename Vec<T>::Any*>(p + c * N);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = (T)((float)x[i] * f);
-        *reinterpret_cast<typename Vec<T>::Any*>(q + c * N) = x;
-    }
-    const long c = nv * N + threadIdx.x;
-    if (c < n) q[c] = (T)((float)p[c] * f);
-}
 
 // Every thread gets the workgroup's sum, added in a fixed order.
 __device__ __forceinline__ double block_sum(double s, double* sm) {
@@ -94,6 +112,14 @@ __device__ __forceinline__ double block_sum(double s, double* sm) {
     return s;
 }
 
+// Where unit u starts in its tensor, and its elements.
+template <typename T>
+__device__ __forceinline__ void unit_of(const Entry& e, uint32_t u, size_t* at, int* n) {
+    constexpr size_t kElems = kUnit / sizeof(T);
+    *at = (size_t)(u - e.first) * kElems;
+    *n = (int)(e.numel - *at < kElems ? e.numel - *at : kElems);
+}
+
 __global__ void __launch_bounds__(NT) norm_kernel(const Entry* __restrict__ entries,
                                                   const uint32_t* __restrict__ map,
                                                   uint32_t units, double* __restrict__ part) {
@@ -101,14 +127,18 @@ __global__ void __launch_bounds__(NT) norm_kernel(const Entry* __restrict__ entr
     double s = 0.0;
     for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
         const Entry e = entries[map[u]];
-        const size_t at = (size_t)(u - e.first) * kUnit;
-        const long n = (long)(e.numel - at < kUnit ? e.numel - at : kUnit);
-        if (e.dtype == kDtypeBF16)
-            s += square_sum((const bf16*)e.in + at, n);
-        else if (e.dtype == kDtypeF16)
-            s += square_sum((const f16*)e.in + at, n);
-        else
-            s += square_sum((const float*)e.in + at, n);
+        size_t at;
+        int n;
+        if (e.dtype == kDtypeBF16) {
+            unit_of<bf16>(e, u, &at, &n);
+            s += Unit<bf16>((const bf16*)e.in + at, n).square_sum();
+        } else if (e.dtype == kDtypeF16) {
+            unit_of<f16>(e, u, &at, &n);
+            s += Unit<f16>((const f16*)e.in + at, n).square_sum();
+        } else {
+            unit_of<float>(e, u, &at, &n);
+            s += Unit<float>((const float*)e.in + at, n).square_sum();
+        }
     }
     s = block_sum(s, sm);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -126,6 +156,14 @@ __device__ __forceinline__ float coef_of(double norm, float max_norm) {
     return c > 1.0 ? 1.f : (float)c;  // NaN stays NaN
 }
 
+// The clipping factor; the first workgroup writes the norm.
+__device__ __forceinline__ float factor(const double* __restrict__ part, int parts,
+                                        float max_norm, float* norm, double* sm) {
+    const double v = all_parts(part, parts, sm);
+    if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)v;
+    return coef_of(v, max_norm);
+}
+
 __global__ void __launch_bounds__(NT) final_kernel(const double* __restrict__ part, int parts,
                                                    float max_norm, float* __restrict__ norm,
                                                    float* __restrict__ coef) {
@@ -137,25 +175,42 @@ __global__ void __launch_bounds__(NT) final_kernel(const double* __restrict__ pa
     }
 }
 
+// One unit: its loads are on their way while the first one's factor is added up.
+template <bool PAST, typename T>
+__device__ __forceinline__ void clip_unit(const Entry& e, uint32_t u, bool* known, float* f,
+                                          const double* part, int parts, float max_norm,
+                                          float* norm, double* sm) {
+    size_t at;
+    int n;
+    unit_of<T>(e, u, &at, &n);
+    const Unit<T> x((const T*)e.in + at, n);
+    if (!*known) *f = factor(part, parts, max_norm, norm, sm);
+    *known = true;
+    if (*f == 1.f && e.in == e.out) return;  // nothing changes
+    x.template scale<PAST>((T*)e.out + at, *f);
+}
+
+template <bool PAST>
 __global__ void __launch_bounds__(NT)
 clip_kernel(const Entry* __restrict__ entries, const uint32_t* __restrict__ map, uint32_t units,
             const double* __restrict__ part, int parts, float max_norm,
             float* __restrict__ norm) {
     __shared__ double sm[NT / kWave];
-    const double v = all_parts(part, parts, sm);
-    const float f = coef_of(v, max_norm);
-    if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)v;
-    for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+    bool known = false;
+    float f = 1.f;
+    if (units == 0) factor(part, parts, max_norm, norm, sm);
+    // the last units first: of more gradients than the 256 MB cache holds it has those that
+    // the norm read last
+    for (uint32_t k = blockIdx.x; k < units; k += gridDim.x) {
+        const uint32_t u = units - 1 - k;
         const Entry e = entries[map[u]];
-        if (f == 1.f && e.in == e.out) continue;  // nothing changes
-        const size_t at = (size_t)(u - e.first) * kUnit;
-        const long n = (long)(e.numel - at < kUnit ? e.numel - at : kUnit);
+        if (known && f == 1.f && e.in == e.out) continue;
         if (e.dtype == kDtypeBF16)
-            scale((const bf16*)e.in + at, (bf16*)e.out + at, n, f);
+            clip_unit<PAST, bf16>(e, u, &known, &f, part, parts, max_norm, norm, sm);
         else if (e.dtype == kDtypeF16)
-            scale((const f16*)e.in + at, (f16*)e.out + at, n, f);
+            clip_unit<PAST, f16>(e, u, &known, &f, part, parts, max_norm, norm, sm);
         else
-            scale((const float*)e.in + at, (float*)e.out + at, n, f);
+            clip_unit<PAST, float>(e, u, &known, &f, part, parts, max_norm, norm, sm);
     }
 }
 
@@ -190,7 +245,7 @@ extern "C" int grad_list_create_hip(void** list, const void* const* grads, void*
     *list = nullptr;
     if (count != 0 && (!grads || !numels || !dtypes)) return kInvalidValue;
     if (count > 0x7FFFFFFFull) return kInvalidConfiguration;
-    size_t units = 0;
+    size_t units = 0, total = 0;
     for (size_t i = 0; i < count; ++i) {
         const int d = dtypes[i];
         const size_t size = d == kDtypeF32 ? 4 : d == kDtypeF16 || d == kDtypeBF16 ? 2 : 0;
@@ -200,7 +255,8 @@ extern "C" int grad_list_create_hip(void** list, const void* const* grads, void*
         if (!grads[i] || !out || ((uintptr_t)grads[i] | (uintptr_t)out) % size)
             return kInvalidValue;
         if (numels[i] > (size_t)1 << 46) return kInvalidConfiguration;
-        units += (numels[i] + gn::kUnit - 1) / gn::kUnit;
+        total += numels[i] * size;
+        units += (numels[i] * size + gn::kUnit - 1) / gn::kUnit;
         if (units > 0x7FFFFFFFull) return kInvalidConfiguration;
     }
     int dev = 0;
@@ -222,7 +278,8 @@ extern "C" int grad_list_create_hip(void** list, const void* const* grads, void*
             e[i].numel = numels[i];
             e[i].first = u;
             e[i].dtype = dtypes[i];
-            for (size_t k = 0; k < numels[i]; k += gn::kUnit) map[u++] = (uint32_t)i;
+            const size_t size = dtypes[i] == kDtypeF32 ? 4 : 2;
+            for (size_t k = 0; k < numels[i] * size; k += gn::kUnit) map[u++] = (uint32_t)i;
         }
         rc = (int)hipMemcpy(mem, host, bytes, hipMemcpyHostToDevice);
     }
@@ -235,6 +292,7 @@ extern "C" int grad_list_create_hip(void** list, const void* const* grads, void*
     l->device = dev;
     l->count = count;
     l->units = units;
+    l->bytes = total;
     l->part = (double*)mem;
     l->entries = (gn::Entry*)((uint8_t*)mem + parts);
     l->map = (uint32_t*)(l->entries + count);
@@ -270,7 +328,13 @@ extern "C" int grad_clip_hip(const void* list, float max_norm, float* norm, hipS
     unsigned parts;
     rc = gn::sums(l, &parts, stream);
     if (rc != kSuccess) return rc;
-    EFLA_LAUNCH("grad_clip", gn::clip_kernel, dim3(parts ? parts : 1), dim3(gn::NT), stream,
-                l->entries, l->map, (uint32_t)l->units, l->part, (int)parts, max_norm, norm);
+    const dim3 grid(parts ? parts : 1), block(gn::NT);
+    // gradients and outputs past the 256 MB cache are stored past it
+    if (2 * l->bytes > (size_t)256 << 20)
+        EFLA_LAUNCH("grad_clip", (gn::clip_kernel<true>), grid, block, stream, l->entries, l->map,
+                    (uint32_t)l->units, l->part, (int)parts, max_norm, norm);
+    else
+        EFLA_LAUNCH("grad_clip", (gn::clip_kernel<false>), grid, block, stream, l->entries, l->map,
+                    (uint32_t)l->units, l->part, (int)parts, max_norm, norm);
     return (int)hipPeekAtLastError();
 }

@@ -590,7 +590,7 @@ class GradList:
         self._handle = handle
 
     def __del__(self):
-        if getattr(self, "_handle", None):
+        if getattr(self, "_handle", None) and lib is not None:  # None: the program's end
             lib().grad_list_destroy_hip(self._handle)
             self._handle = None
 
