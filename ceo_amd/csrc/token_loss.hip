@@ -640,7 +640,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PrefArgs a) {
     }
 }
 
-template <typename T>
+template <typename T, bool PAST>
 __global__ void __launch_bounds__(kMaxThreads, 8)
 preference_kernel(const T* logits, T* grad, PrefArgs a) {
     __shared__ Stat sm[kMaxWaves];
@@ -687,7 +687,7 @@ preference_kernel(const T* logits, T* grad, PrefArgs a) {
     const int t = a.targets[row], first = a.first[row];
     const float w = a.weights ? a.weights[row] : 1.f;
     if (w == 0.f) {
-        row_zero<true>(g, a.V);
+        row_zero<PAST>(g, a.V);
         return;
     }
     const T* z = logits + row * a.ld;
@@ -704,13 +704,13 @@ preference_kernel(const T* logits, T* grad, PrefArgs a) {
     }
     __syncthreads();
     if (!tok || first < 0) {
-        row_zero<true>(g, a.V);
+        row_zero<PAST>(g, a.V);
         return;
     }
     const Row<T, 0> x(z, Span<T>(z, a.V));
     const Stat st = sm_stat;
     const float coef = sm_coef;
-    x.template grad<true>(g, st, coef);
+    x.template grad<PAST>(g, st, coef);
     target_grad(g, x.p, t, zt, st, coef);
 }
 
@@ -824,10 +824,14 @@ static int logprob(const void* logits, const int32_t* targets, const float* weig
     return (int)hipPeekAtLastError();
 }
 
-// Whether the preference loss takes the launch that draws rows (see there).
+// Whether the preference loss takes the launch that draws rows (see there): for logits
+// that the cache does not hold, in rows whose work hides the drawing, and for a few short
+// rows, where two launches instead of three count (45 x 32000 in bf16 17.6 us against 21.3;
+// 256 rows 22.7 against 21.5, 45 x 128000 in fp32 33 against 31).
 static bool draws(size_t rows, size_t vocab, int dtype) {
-    const size_t row = vocab * dtype_size(dtype);
-    return row >= (size_t)96 << 10 && rows * row > (size_t)256 << 20;
+    const size_t row = vocab * dtype_size(dtype), all = rows * row;
+    return (row >= (size_t)96 << 10 && all > (size_t)256 << 20) ||
+           (rows <= 128 && all <= (size_t)16 << 20);
 }
 constexpr size_t kInFlight = (size_t)24 << 20;  // logits between a workgroup's two rows
 
@@ -946,8 +950,11 @@ extern "C" int preference_loss_forward_backward_hip(
         if (rc != kSuccess) return rc;
         // the lag is known on the device: as many as it may take
         TL_TYPED(dtype, T, {
-            EFLA_LAUNCH("preference_loss", (tl::preference_kernel<T>), tl::row_grid(2 * rows),
-                        dim3(threads), stream, (const T*)logits, (T*)grad_logits, a);
+            TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
+                EFLA_LAUNCH("preference_loss", (tl::preference_kernel<T, PAST>),
+                            tl::row_grid(2 * rows), dim3(threads), stream, (const T*)logits,
+                            (T*)grad_logits, a);
+            });
         });
         return (int)hipPeekAtLastError();
     }

@@ -502,8 +502,7 @@ def policy_loss_forward_backward(logits: torch.Tensor, targets: torch.Tensor,
         raise ValueError("kl_coef needs ref_logp")
     out = torch.empty(3 if ref_logp is not None else 2, N, dtype=torch.float32,
                       device=logits.device)
-    loss, logp = out[0], out[1]
-    kl = out[2] if ref_logp is not None else None
+    loss, logp, kl = out.unbind(0) if ref_logp is not None else (*out.unbind(0), None)
     g, ldg = _loss_grad(logits, need_grad, in_place, ld)
     rc = lib().policy_loss_forward_backward_hip(
         _p(logits), _p(targets), _p(advantages), _p(old_logp), _p(ref_logp), _p(weights),
@@ -532,9 +531,8 @@ def preference_loss_forward_backward(logits: torch.Tensor, targets: torch.Tensor
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() % 2 == 0:
         raise ValueError("cu_seqlens must hold 2 pairs + 1 offsets")
     P = cu_seqlens.numel() // 2
-    loss = torch.empty(P, dtype=torch.float32, device=dev)
-    rewards = torch.empty(2 * P, dtype=torch.float32, device=dev)
-    logp = torch.empty(N, dtype=torch.float32, device=dev)
+    out = torch.empty(3 * P + N, dtype=torch.float32, device=dev)
+    loss, rewards, logp = out.split((P, 2 * P, N))
     g, ldg = _loss_grad(logits, need_grad, in_place, ld)
     ws, wsb = None, 0
     if need_grad and N:
