@@ -115,6 +115,7 @@ class EflaLM:
         for i in range(cfg.n_layers):
             self._groups[i] = (first[i], first[i + 1])
         self._upd_stream = None
+        self._grad_list = None
 
     # -- parameter views ------------------------------------------------------
     def _view(self, buf: torch.Tensor, name: str) -> torch.Tensor:
@@ -144,13 +145,10 @@ class EflaLM:
         return self._ws
 
     # -- forward --------------------------------------------------------------
-    def forward(self, tokens: torch.Tensor, targets: torch.Tensor, train: bool = True):
-        """tokens, targets: (B, T) int32.  Returns (mean loss tensor, saved).
-
-        With ``train`` (the step's forward) the cross-entropy also writes
-        dL/dlogits over the logits in place, and ``saved`` holds what
-        backward() needs.  With ``train=False`` (evaluation) the logits are
-        kept (``saved["logits"]``) and no activation or gradient is stored."""
+    def logits(self, tokens: torch.Tensor, train: bool = True):
+        """tokens: (B, T) int32.  Returns (logits (B * T, vocab) bf16, saved).  With
+        ``train``, ``saved`` holds what backward() needs but for its ``dlogits``, which a
+        loss puts there."""
         cfg = self.cfg
         B, T = tokens.shape
         N, D, H, dh = B * T, cfg.d_model, cfg.n_heads, cfg.head_dim
@@ -183,7 +181,19 @@ class EflaLM:
             x = x2
         af, mf, rf = nn.layernorm_forward(x, self.w("lnf.w"), self.w("lnf.b"), cfg.ln_eps,
                                           save_stats=True)
-        logits = nn.gemm_forward(af, self.w("head"))
+        if train:
+            saved.update(x=x, af=af, mf=mf, rf=rf)
+        return nn.gemm_forward(af, self.w("head")), saved
+
+    def forward(self, tokens: torch.Tensor, targets: torch.Tensor, train: bool = True):
+        """tokens, targets: (B, T) int32.  Returns (mean loss tensor, saved).
+
+        With ``train`` (the step's forward) the cross-entropy also writes
+        dL/dlogits over the logits in place, and ``saved`` holds what
+        backward() needs.  With ``train=False`` (evaluation) the logits are
+        kept (``saved["logits"]``) and no activation or gradient is stored."""
+        cfg = self.cfg
+        logits, saved = self.logits(tokens, train)
         tflat = targets.reshape(-1)
         if not train:
             loss_rows = nn.cross_entropy_forward(logits, tflat, cfg.label_smoothing)
@@ -194,7 +204,7 @@ class EflaLM:
         loss_rows, dlogits = nn.cross_entropy_forward_backward(logits, tflat,
                                                                cfg.label_smoothing,
                                                                in_place=True)
-        saved.update(x=x, af=af, mf=mf, rf=rf, dlogits=dlogits, targets=tflat)
+        saved.update(dlogits=dlogits, targets=tflat)
         return loss_rows.sum(), saved
 
     # -- backward -------------------------------------------------------------
@@ -282,13 +292,21 @@ class EflaLM:
         upd("embed")
 
     # -- update ---------------------------------------------------------------
-    def update(self) -> None:
-        """One AdamW step over every parameter (fp32 master, bf16 copy refreshed)."""
+    def update(self, max_norm=None):
+        """One AdamW step over every parameter (fp32 master, bf16 copy refreshed).  With
+        ``max_norm`` on the gradients clipped to that norm (the factor goes to the step,
+        nothing is written for it); returns their norm before, a device value."""
         cfg = self.cfg
+        norm = coef = None
+        if max_norm is not None:
+            if self._grad_list is None:
+                self._grad_list = nn.GradList([self.grads])
+            norm, coef = nn.grad_norm(self._grad_list, max_norm)
         self.step_count += 1
         nn.adamw_step_master(self.master, self.grads, self.exp_avg, self.exp_avg_sq, cfg.lr,
                              cfg.beta1, cfg.beta2, cfg.adam_eps, cfg.weight_decay,
-                             self.step_count, param_bf16=self.weights)
+                             self.step_count, param_bf16=self.weights, grad_scale=coef)
+        return norm
 
     def train_step(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         """forwardStep, backwardStep, updateStep; returns the loss (device scalar).
