@@ -39,6 +39,13 @@ __device__ __forceinline__ f16 from_f<f16>(float x) { return (f16)x; }
 __device__ __forceinline__ int lane_id() { return threadIdx.x & (kWave - 1); }
 __device__ __forceinline__ int wave_id() { return threadIdx.x / kWave; }
 
+// Item k of n taken from the last to the first in eights, each in its own order: workgroups
+// go to the 8 XCDs in turn, so an item that an earlier launch gave to workgroup i, and this
+// one to k, is the same XCD's (and L2's).  May be n or more.
+__device__ __forceinline__ long backwards(long k, long n) {
+    return (((n + 7) >> 3) - 1 - (k >> 3)) * 8 + (k & 7);
+}
+
 // ---------------------------------------------------------------------------
 // MFMA traits per operand type
 // ---------------------------------------------------------------------------

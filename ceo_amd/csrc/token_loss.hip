@@ -23,7 +23,11 @@
 //
 // One workgroup has a row.  Where the gradient needs nothing but the row (the policy
 // loss), the row stays in its registers between the statistics and the gradient, so
-// each logit moves once in and once out of memory.
+// each logit moves once in and once out of memory, which is what bounds it: 16384 x 32000
+// in bf16 take 342 to 360 us, 5.8 to 6.1 TB/s (a large copy: 5.15).  A row of over 128 KiB
+// leaves no room for a second one on its compute unit, so its loads wait for its
+// stores (2048 x 128003 in fp16 192 to 209 us, 4.5 to 4.9 TB/s).  A few rows are bound by
+// their own latency, 8 us for 64 x 32000, and the host's 13.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -108,10 +112,11 @@ __device__ __forceinline__ Stat join_waves(Stat a, Stat* sm) {
 
 // A row as its whole vectors from a boundary on and the elements before the first and
 // behind the last of them, one to a thread.  The boundary is a cache line's, so that no
-// line is two waves' (in fp32 4096 x 50257 327 us against 305 where it is not), in short rows
-// 16 bytes: loads that are not aligned to these cost a fifth (log-probabilities of
-// 4096 x 50257 in bf16: 100 us against 80).  The boundaries are those of the logits, also
-// where the gradient has others: stores, which the cache joins, lose 3 %.
+// line is two waves' (policy loss of 4096 x 50257 in fp32 305 us, 329 from 16-byte
+// boundaries), in short rows 16 bytes: loads that are not aligned to these cost a fifth
+// (log-probabilities of 4096 x 50257 in bf16: 100 us against 80).  The boundaries are those
+// of the logits, also where the gradient has others, whose stores cost less (151 us where
+// they agree, 164 where not).
 constexpr int kLineVocab = 4096, kLineThreads = 128;  // its edges: up to 70 elements
 
 template <typename T>
@@ -513,9 +518,9 @@ grad_kernel(const T* logits, T* grad, const int32_t* __restrict__ targets,
             const float* __restrict__ weights, const float2* __restrict__ stat,
             const float* __restrict__ coef, long rows, int V, long ld, long ldg) {
     // the last rows first: of more logits than the 256 MB cache holds it has those that the
-    // statistics read last
-    const long row = rows - 1 - block_row();
-    if (row < 0) return;
+    // statistics read last (8191 x 32000 in bf16 200 us in all, 230 from the first on)
+    const long row = backwards(block_row(), rows);
+    if (row < 0 || row >= rows) return;
     T* g = grad + row * ldg;
     const int t = targets[row];
     if ((weights && weights[row] == 0.f) || t < 0 || t >= V) {
@@ -538,10 +543,10 @@ grad_kernel(const T* logits, T* grad, const int32_t* __restrict__ targets,
 // The rows are drawn from a counter, so that a workgroup waits only for what has been
 // drawn before (a gradient for its pair's sums, a pair's last row for the pair's other
 // rows), by workgroups that run already and do their statistics first: every wait ends
-// whatever else the GPU does.  32 pairs of 4100 x 50257 in all: fp32 343 us against 441
-// in three launches, bf16 187 against 211; 8 pairs of 2048 x 128000 in bf16 207 against 232.
+// whatever else the GPU does.  32 pairs of 4100 x 50257 in all: fp32 331 us against 398
+// in three launches, bf16 184 against 206; 8 pairs of 2048 x 128000 in bf16 205 against 213.
 // Drawing takes 13 ns, one workgroup after another, so that shorter rows are faster in
-// three launches: 8 pairs of 8191 x 32000 in bf16 201 us against 224.
+// three launches: 8 pairs of 8191 x 32000 in bf16 201 us against 223.
 struct PairInfo {
     int pair, mid, end;  // of the pair that starts at this row
     uint32_t coef;       // d loss / d (sum of the chosen rows' w logp): a message
@@ -751,11 +756,12 @@ static int check(const void* logits, const int32_t* targets, const void* grad, s
         }                                \
     } while (0)
 
-// The form for rows of this length: vectors per thread (0: streamed) and threads.  As
-// few vectors as `least` and 1024 threads allow: a policy step of 16384 x 32000 in bf16
-// takes 368 us with 4 and 1024 threads (388 with 8 and 512, 389 with 16 and 256), one of
-// 20000 x 1000 22 us with 4 (28, 44); log-probabilities, which write nothing, take
-// 105 us with 8 and 127 with 4 for the former's logits, 40 % of the rows without weight.
+// The form for rows of this length: vectors per thread (0: streamed) and threads, from
+// `least` vectors to `most`, as few as 1024 threads allow.  The policy loss of 16384 x
+// 32000 in bf16 takes 360 us with 4 vectors (378 with 8, 370 with 16), that of 20000 x
+// 1000 21 us (28, 44).  Log-probabilities, which write nothing, take 109 us with 8 and 131
+// with 4 for the former's logits, 40 % of the rows without weight; 2048 x 128003 take 90 us
+// streamed and 108 with 16.
 struct Form {
     int nv;
     unsigned threads;
@@ -806,7 +812,9 @@ static dim3 row_grid(size_t rows) {
 }
 
 // Whether logits and gradient are more than the 256 MB cache: then the gradient is stored
-// past it (16384 x 32000 in bf16 351 us, 359 through it); else what reads it next finds it.
+// past it (policy loss of 16384 x 32000 in bf16 360 us, 369 through it; preference loss of
+// 8191 x 32000, whose second read the cache serves, 202 and 249); else what reads the
+// gradient next finds it there.
 static bool past_cache(size_t rows, size_t vocab, int dtype) {
     return 2 * rows * vocab * dtype_size(dtype) > ((size_t)256 << 20);
 }
@@ -826,8 +834,8 @@ static int logprob(const void* logits, const int32_t* targets, const float* weig
 
 // Whether the preference loss takes the launch that draws rows (see there): for logits
 // that the cache does not hold, in rows whose work hides the drawing, and for a few short
-// rows, where two launches instead of three count (45 x 32000 in bf16 17.6 us against 21.3;
-// 256 rows 22.7 against 21.5, 45 x 128000 in fp32 33 against 31).
+// rows, where two launches instead of three count (45 x 32000 in bf16 18.0 us against 21.4;
+// 256 rows 22.7 against 21.3, 45 x 128000 in fp32 33 against 31).
 static bool draws(size_t rows, size_t vocab, int dtype) {
     const size_t row = vocab * dtype_size(dtype), all = rows * row;
     return (row >= (size_t)96 << 10 && all > (size_t)256 << 20) ||
@@ -976,7 +984,7 @@ extern "C" int preference_loss_forward_backward_hip(
     if (grad_logits && rows != 0) {
         TL_TYPED(dtype, T, {
             TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
-                EFLA_LAUNCH("preference_grad", (tl::grad_kernel<T, PAST>), tl::row_grid(rows),
+                EFLA_LAUNCH("preference_grad", (tl::grad_kernel<T, PAST>), tl::row_grid((rows + 7) & ~(size_t)7),
                             dim3(threads), stream, (const T*)logits, (T*)grad_logits, targets,
                             weights, stat, coef, (long)rows, (int)vocab_size, (long)ld,
                             (long)ld_grad);

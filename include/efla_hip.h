@@ -497,7 +497,7 @@ int adamw_step_master_scaled_hip(float* param, const void* grad, const float* gr
 /* Makes a list for the current device.  Clipping writes to outs[i], which may be
  * grads[i] (outs NULL: all in place); an output that overlaps any other gradient
  * or output is undefined.  A gradient of no element may be NULL.  NULL arguments,
- * an unknown dtype or a misaligned pointer -> 1; more than 2^45 elements in all
+ * an unknown dtype or a misaligned pointer -> 1; more than 2^45 bytes in all
  * -> 9.  Waits for its copy to the device: not for use under stream capture. */
 int grad_list_create_hip(void** list, const void* const* grads, void* const* outs,
                          const size_t* numels, const int* dtypes, size_t count);
@@ -639,9 +639,9 @@ size_t preference_loss_workspace_size(size_t rows);
  * gives means instead of sums).  Sums are 64 bits, in a fixed order.  Sequences may
  * be empty; offsets are clamped to the rows and to their predecessors; rows outside
  * of every sequence have gradient 0.  A NaN in one row makes its pair's loss, rewards
- * and gradient NaN.  workspace NULL: the stream's cached one (only a call with
- * grad_logits needs any).  beta not positive and finite, eps outside [0, 1), or a
- * workspace that is too small -> 1. */
+ * and gradient NaN.  The workspace (any contents, one call at a time) may be NULL: the
+ * stream's cached one; only a call with grad_logits needs any.  beta not positive and
+ * finite, eps outside [0, 1), or a workspace that is too small -> 1; rows past 2^30 -> 9. */
 int preference_loss_forward_backward_hip(
     const void* logits, const int32_t* targets, const float* ref_logp, const float* weights,
     const int32_t* cu_seqlens, float* loss, float* rewards, float* logp, void* grad_logits,
