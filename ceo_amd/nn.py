@@ -433,28 +433,33 @@ def cross_entropy_backward(grad_loss: torch.Tensor, logits: torch.Tensor, target
 # losses on rewards and preferences
 # ---------------------------------------------------------------------------
 def _loss_rows(logits, targets, **rows):
-    """(rows, vocab, row stride, dtype code) of 2-D logits whose rows are contiguous,
-    after checking the per-row operands given by name (None: absent)."""
+    """(rows, vocab, row stride, dtype code, device) of 2-D logits whose rows are
+    contiguous, after checking the per-row operands given by name (None: absent)."""
     _require(logits, "logits", contiguous=False)
-    if logits.dtype not in DTYPE_CODES:
+    dt = DTYPE_CODES.get(logits.dtype)
+    if dt is None:
         raise ValueError(f"unsupported dtype {logits.dtype}")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be 2-D with contiguous rows")
-    N, V = logits.shape
+    N, V = shape = logits.shape
     # a single row's stride says nothing
     ld = logits.stride(0) if N > 1 else max(V, 1)
     if ld < V:
         raise ValueError("logits rows overlap")
     dev = logits.device
     _require(targets, "targets", torch.int32, dev)
-    if targets.shape != (N,):
+    one = shape[:1]
+    if targets.shape != one:
         raise ValueError("targets must hold one token per row of logits")
     for name, t in rows.items():
-        if t is not None:
-            _require(t, name, torch.float32, dev)
-            if t.shape != (N,):
-                raise ValueError(f"{name} must hold one value per row of logits")
-    return N, V, ld, DTYPE_CODES[logits.dtype]
+        # a small call spends more on these checks than on the GPU: in one expression, what
+        # is wrong said only where something is
+        if t is None or (isinstance(t, torch.Tensor) and t.dtype is torch.float32
+                         and t.shape == one and t.device == dev and t.is_contiguous()):
+            continue
+        _require(t, name, torch.float32, dev)
+        raise ValueError(f"{name} must hold one value per row of logits")
+    return N, V, ld, dt, dev
 
 
 def _loss_grad(logits, need_grad, in_place, ld):
@@ -465,7 +470,8 @@ def _loss_grad(logits, need_grad, in_place, ld):
         return None, 0
     if in_place:
         return logits, ld
-    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
+    g = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    return g, logits.shape[1]
 
 
 def token_logprob_forward(logits: torch.Tensor, targets: torch.Tensor,
@@ -473,8 +479,8 @@ def token_logprob_forward(logits: torch.Tensor, targets: torch.Tensor,
     """log softmax(logits)[i, targets[i]], fp32 (rows,), for (rows, vocab) logits in
     bf16, fp16 or fp32 (a row stride is fine).  A row whose weight (fp32 (rows,),
     None: all count) is 0 is not read and gives 0."""
-    N, V, ld, dt = _loss_rows(logits, targets, weights=weights)
-    logp = torch.empty(N, dtype=torch.float32, device=logits.device)
+    N, V, ld, dt, dev = _loss_rows(logits, targets, weights=weights)
+    logp = torch.empty(N, dtype=torch.float32, device=dev)
     rc = lib().token_logprob_forward_hip(_p(logits), _p(targets), _p(weights), _p(logp), N, V, ld,
                                          dt, _stream(logits))
     check(rc, "token_logprob_forward_hip")
@@ -494,14 +500,13 @@ def policy_loss_forward_backward(logits: torch.Tensor, targets: torch.Tensor,
     Without ``old_logp`` the sampling policy is this one (r = 1, with its gradient);
     without ``ref_logp`` there is no kl; without ``weights`` every row has 1 / rows.
     Rows of weight 0 are not read.  With ``in_place`` the gradient overwrites the logits."""
-    N, V, ld, dt = _loss_rows(logits, targets, advantages=advantages, old_logp=old_logp,
+    N, V, ld, dt, dev = _loss_rows(logits, targets, advantages=advantages, old_logp=old_logp,
                               ref_logp=ref_logp, weights=weights)
     if advantages is None:
         raise TypeError("advantages must be a tensor")
     if ref_logp is None and kl_coef != 0:
         raise ValueError("kl_coef needs ref_logp")
-    out = torch.empty(3 if ref_logp is not None else 2, N, dtype=torch.float32,
-                      device=logits.device)
+    out = torch.empty(3 if ref_logp is not None else 2, N, dtype=torch.float32, device=dev)
     loss, logp, kl = out.unbind(0) if ref_logp is not None else (*out.unbind(0), None)
     g, ldg = _loss_grad(logits, need_grad, in_place, ld)
     rc = lib().policy_loss_forward_backward_hip(
@@ -525,8 +530,7 @@ def preference_loss_forward_backward(logits: torch.Tensor, targets: torch.Tensor
     ``loss = (-(1 - e) log sigmoid(x) - e log sigmoid(-x)) / pairs``, e the label smoothing.
     Rows of weight 0 (prompts, padding) are not read; without ``weights`` all count.
     With ``in_place`` the gradient overwrites the logits."""
-    N, V, ld, dt = _loss_rows(logits, targets, ref_logp=ref_logp, weights=weights)
-    dev = logits.device
+    N, V, ld, dt, dev = _loss_rows(logits, targets, ref_logp=ref_logp, weights=weights)
     _require(cu_seqlens, "cu_seqlens", torch.int32, dev)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() % 2 == 0:
         raise ValueError("cu_seqlens must hold 2 pairs + 1 offsets")
