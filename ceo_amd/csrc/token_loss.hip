@@ -434,17 +434,29 @@ struct PairSum {
         __shared__ double sm[2][NT / kWave];
         if (threadIdx.x < NT) {
             sum[0] = sum[1] = 0.0;
-            for (int i = a0 + (int)threadIdx.x; i < a2; i += NT) {
-                const float w = weights ? weights[i] : 1.f;
-                if (w == 0.f) continue;
-                const float lp = told ? __builtin_bit_cast(
-                                            float, hear(reinterpret_cast<uint32_t*>(logp) + i, kAbsent))
-                                      : logp[i];
-                const double d = (double)w * ((double)lp - (ref ? (double)ref[i] : 0.0));
-                if (i < a1)
-                    sum[0] += d;
-                else
-                    sum[1] += d;
+            constexpr int U = 4;  // rows whose loads are on their way together
+            for (int i0 = a0 + (int)threadIdx.x; i0 < a2; i0 += U * NT) {
+                float w[U], lp[U], rf[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + u * NT;
+                    w[u] = lp[u] = rf[u] = 0.f;
+                    if (i >= a2) continue;
+                    w[u] = weights ? weights[i] : 1.f;
+                    if (ref) rf[u] = ref[i];
+                    lp[u] = told ? __builtin_bit_cast(
+                                       float, hear(reinterpret_cast<uint32_t*>(logp) + i, kAbsent))
+                                 : logp[i];
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const double d =
+                        w[u] != 0.f ? (double)w[u] * ((double)lp[u] - (double)rf[u]) : 0.0;
+                    if (i0 + u * NT < a1)
+                        sum[0] += d;
+                    else
+                        sum[1] += d;
+                }
             }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {

@@ -559,7 +559,8 @@ class GradList:
     It keeps the tensors (contiguous, bf16, fp16 or fp32, on one device) and the device
     table of their addresses; what they hold is read at each call.  Clipping writes into
     ``outs`` (shaped and typed like the gradients), or in place without.  One call at a
-    time may use a list: two streams need two."""
+    time may use a list: two streams need two.  Making one copies to the device and freeing
+    one waits for it: for a graph, make it before the capture and keep it."""
 
     def __init__(self, grads, outs=None):
         self.grads = list(grads)
