@@ -950,7 +950,7 @@ extern "C" int preference_loss_forward_backward_hip(
     }
     const float inv_pairs = pairs ? 1.f / (float)pairs : 0.f;
     const unsigned threads = tl::stream_threads(vocab_size, dtype);
-    const bool draws = tl::draws(rows, vocab_size, dtype);
+    const bool draws = rows != 0 && tl::draws(rows, vocab_size, dtype);
     if (draws && grad_logits) {
         tl::PrefArgs a;
         a.targets = targets, a.cu = cu_seqlens, a.ref = ref_logp, a.weights = weights;

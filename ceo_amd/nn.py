@@ -618,7 +618,8 @@ def grad_norm(grads, max_norm: float = float("inf")):
 def clip_grad_norm(grads, max_norm: float) -> torch.Tensor:
     """Scales the gradients of a ``GradList`` (or tensors, in place) by
     ``min(1, max_norm / (norm + 1e-6))``; returns their norm (before), an fp32 device
-    value.  A list's ``outs`` receive the scaled gradients where it has them."""
+    value.  A list's ``outs`` receive the scaled gradients where it has them.  A list made
+    for one call costs a copy to the device and a wait for it."""
     gl = _grad_list(grads)
     norm = torch.empty((), dtype=torch.float32, device=gl.device)
     rc = lib().grad_clip_hip(gl._handle, float(max_norm), _p(norm), _stream(norm))

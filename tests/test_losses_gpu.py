@@ -685,3 +685,73 @@ def test_more_rows_than_one_grid_dimension(dtype):
     want[N // 2:] *= -1
     room = want.abs() * (eps / 2 + 8 * U) + TINY[dtype] + (one + lp.exp()) * rel(V)
     assert bool(((pg.double() - want).abs() <= room).all())
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 4101), (torch.float16, 8197),
+                                     (torch.float32, 4099), (torch.bfloat16, 33)], ids=str)
+def test_every_alignment(oracle, dtype, V):
+    """Rows that start at each multiple of the type's size within a cache line, logits and
+    gradient at different ones; in place the same bits."""
+    from ceo_amd import nn
+
+    N = 130
+    announce(f"every alignment {dtype} V={V}")
+    x, d, store = make(V, N, V, dtype, pad=2, skew=1)  # the gradient is packed
+    check_policy(x, d, dtype, V)
+    check_preference(x, d, [0, 40, 65, 65, N], dtype, V)
+    cu = torch.tensor([0, 40, 65, 65, N], dtype=torch.int32, device="cuda")
+    for f in (lambda ip: nn.preference_loss_forward_backward(d["z"], d["t"], cu, d["ref"], d["w"],
+                                                             in_place=ip),
+              lambda ip: nn.policy_loss_forward_backward(d["z"], d["t"], d["adv"], d["old"],
+                                                         d["ref"], d["w"], in_place=ip)):
+        kept = store.clone()
+        want = f(False)
+        got = f(True)
+        assert all(torch.equal(p, q) for p, q in zip(want[:2], got[:2]))
+        assert torch.equal(want[3], got[3])
+        outside = torch.ones_like(store, dtype=torch.bool)
+        outside[1:1 + N * (V + 2)].view(N, V + 2)[:, :V] = False
+        assert bool(store[outside].isnan().all())
+        store.copy_(kept)
+
+
+def test_no_rows_with_a_gradient_pointer():
+    """Pairs without rows through the C ABI, a gradient and a workspace given all the same."""
+    from ceo_amd import _lib
+
+    cu = torch.zeros(5, dtype=torch.int32, device="cuda")
+    loss, rew = torch.full((2,), 7.0, device="cuda"), torch.full((4,), 7.0, device="cuda")
+    buf = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    rc = _lib.lib().preference_loss_forward_backward_hip(
+        None, None, None, None, cu.data_ptr(), loss.data_ptr(), rew.data_ptr(), None,
+        buf.data_ptr(), 2, 0, 100, 100, 100, 0.1, 0.0, 14, buf.data_ptr(), 4096, st)
+    assert rc == 0
+    assert np.allclose(loss.cpu().numpy(), np.log(2) / 2, rtol=2 * U) and not rew.any()
+    assert not buf[2048:].any()
+
+
+def test_large_preferences_on_two_streams():
+    """Two of the launches whose workgroups wait for each other, at once: each waits only
+    for its own."""
+    from ceo_amd import nn
+
+    N, V = 2800, 50257
+    announce("large preference losses on two streams")
+    cu = torch.tensor([0, 90, 200, 900, 1000, 1300, 2000, 2400, N], dtype=torch.int32,
+                      device="cuda")
+    t = torch.arange(N, device="cuda", dtype=torch.int32)
+    zs = [torch.empty(N, V, dtype=torch.bfloat16, device="cuda").normal_() for _ in range(2)]
+    want = [nn.preference_loss_forward_backward(z, t, cu, beta=0.01) for z in zs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in zs]
+    got = [[], []]
+    for _ in range(3):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(nn.preference_loss_forward_backward(zs[k], t, cu, beta=0.01))
+    for st in streams:
+        st.synchronize()
+    for w, g in zip(want, got):
+        for r in g:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
