@@ -534,6 +534,8 @@ LARGE_CU = {
     "short pairs": lambda N: [0, 3, 3, 3, 3, *range(10, N - 37, 29)],
     "ragged, rows outside": lambda N: [5, 40, 41, 600, 600, 600, 600, 900, N - 9],
     "one pair": lambda N: [0, N // 3, N],
+    # more than a workgroup's threads, one row to a sequence, some without
+    "many pairs": lambda N: [*range(0, N - 99), *[N - 99] * 5, *range(N - 99, N - 2, 3)],
 }
 
 
