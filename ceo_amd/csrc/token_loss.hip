@@ -844,14 +844,21 @@ static int logprob(const void* logits, const int32_t* targets, const float* weig
     return (int)hipPeekAtLastError();
 }
 
-// Whether the preference loss takes the launch that draws rows (see there): for logits
-// that the cache does not hold, in rows whose work hides the drawing, and for a few short
-// rows, where two launches instead of three count (45 x 32000 in bf16 18.0 us against 21.4;
-// 256 rows 22.7 against 21.3, 45 x 128000 in fp32 33 against 31).
-static bool draws(size_t rows, size_t vocab, int dtype) {
-    const size_t row = vocab * dtype_size(dtype), all = rows * row;
-    return (row >= (size_t)96 << 10 && all > (size_t)256 << 20) ||
-           (rows <= 128 && all <= (size_t)16 << 20);
+// Logits that the cache does not hold, in rows whose work hides the drawing: their
+// preference loss streams them.
+static bool streams(size_t rows, size_t vocab, int dtype) {
+    const size_t row = vocab * dtype_size(dtype);
+    return row >= (size_t)96 << 10 && rows * row > (size_t)256 << 20;
+}
+// Whether the preference loss takes the launch that draws rows (see there): for such logits
+// of pairs that the cache holds (8000 x 50257 in bf16, 4 pairs: 345 us against 347, 2 pairs
+// 380 against 350), and for a few short rows, where two launches instead of three count
+// (45 x 32000 in bf16 18.0 us against 21.4; 256 rows 22.7 against 21.3, 45 x 128000 in
+// fp32 33 against 31).
+static bool draws(size_t rows, size_t pairs, size_t vocab, int dtype) {
+    const size_t all = rows * vocab * dtype_size(dtype);
+    return streams(rows, vocab, dtype) ? pairs != 0 && all / pairs <= (size_t)192 << 20
+                                       : rows <= 128 && all <= (size_t)16 << 20;
 }
 constexpr size_t kInFlight = (size_t)24 << 20;  // logits between a workgroup's two rows
 
@@ -950,7 +957,7 @@ extern "C" int preference_loss_forward_backward_hip(
     }
     const float inv_pairs = pairs ? 1.f / (float)pairs : 0.f;
     const unsigned threads = tl::stream_threads(vocab_size, dtype);
-    const bool draws = rows != 0 && tl::draws(rows, vocab_size, dtype);
+    const bool draws = rows != 0 && tl::draws(rows, pairs, vocab_size, dtype);
     if (draws && grad_logits) {
         tl::PrefArgs a;
         a.targets = targets, a.cu = cu_seqlens, a.ref = ref_logp, a.weights = weights;
@@ -981,7 +988,10 @@ extern "C" int preference_loss_forward_backward_hip(
     float2* stat = (float2*)ws;
     float* coef = stat ? (float*)(stat + rows) : nullptr;
     if (rows != 0) {
-        const tl::Form f = draws ? tl::Form{0, threads} : tl::form_of(vocab_size, dtype, 8, 8);
+        // the same sums as where rows are drawn, so that these do not depend on the gradient
+        const tl::Form f = draws || tl::streams(rows, vocab_size, dtype)
+                               ? tl::Form{0, threads}
+                               : tl::form_of(vocab_size, dtype, 8, 8);
         const int rc = tl::logprob(logits, targets, weights, logp, stat, coef, rows, vocab_size,
                                    ld, dtype, f, stream);
         if (rc != kSuccess) return rc;
