@@ -58,10 +58,13 @@ struct ProfScope {
     }
 };
 
-#define EFLA_LAUNCH(name, kernel, grid, block, stream, ...)                         \
+#define EFLA_LAUNCH(name, kernel, grid, block, stream, ...) \
+    EFLA_LAUNCH_LDS(name, kernel, grid, block, 0, stream, __VA_ARGS__)
+// with `lds` bytes of dynamic LDS
+#define EFLA_LAUNCH_LDS(name, kernel, grid, block, lds, stream, ...)                \
     do {                                                                             \
         ::efla::ProfScope _efla_ps(name, stream);                                    \
-        hipLaunchKernelGGL(kernel, grid, block, 0, stream, __VA_ARGS__);             \
+        hipLaunchKernelGGL(kernel, grid, block, lds, stream, __VA_ARGS__);           \
     } while (0)
 
 #define EFLA_CHECK(expr)                      \

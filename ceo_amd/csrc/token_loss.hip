@@ -860,6 +860,12 @@ static bool draws(size_t rows, size_t pairs, size_t vocab, int dtype) {
     return streams(rows, vocab, dtype) ? pairs != 0 && all / pairs <= (size_t)192 << 20
                                        : rows <= 128 && all <= (size_t)16 << 20;
 }
+// LDS that nobody uses: over half of a compute unit's, so that it has one workgroup, where the
+// rows in flight would else be as much as the cache (32 pairs of 2048 x 128000 in fp32 456 us,
+// 520 with two; in bf16 229 with either).
+static unsigned draw_lds(size_t vocab, int dtype) {
+    return vocab * dtype_size(dtype) > (size_t)256 << 10 ? 84 << 10 : 0;
+}
 constexpr size_t kInFlight = (size_t)24 << 20;  // logits between a workgroup's two rows
 
 // The preference loss's scratch, of either kind.
@@ -978,9 +984,10 @@ extern "C" int preference_loss_forward_backward_hip(
         // the lag is known on the device: as many as it may take
         TL_TYPED(dtype, T, {
             TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
-                EFLA_LAUNCH("preference_loss", (tl::preference_kernel<T, PAST>),
-                            tl::row_grid(2 * rows), dim3(threads), stream, (const T*)logits,
-                            (T*)grad_logits, a);
+                EFLA_LAUNCH_LDS("preference_loss", (tl::preference_kernel<T, PAST>),
+                                tl::row_grid(2 * rows), dim3(threads),
+                                tl::draw_lds(vocab_size, dtype), stream, (const T*)logits,
+                                (T*)grad_logits, a);
             });
         });
         return (int)hipPeekAtLastError();

@@ -529,17 +529,18 @@ def large_rows(d, cu, beta, eps, rows=500):
 
 
 # logits of over 256 MiB in rows of at least 96 KiB: statistics and gradients in one launch
-LARGE = [(2700, 50257, torch.bfloat16), (1101, 61003, torch.float32), (2111, 65537, torch.float16)]
+LARGE = [(2700, 50257, torch.bfloat16), (1101, 61003, torch.float32), (2111, 65537, torch.float16),
+         (700, 100001, torch.float32)]
 LARGE_CU = {
     "short pairs": lambda N: [0, 3, 3, 3, 3, *range(10, N - 37, 29)],
-    "ragged, rows outside": lambda N: [5, 40, 41, 600, 600, 600, 600, 900, N - 9],
+    "ragged, rows outside": lambda N: [5, 40, 41, 500, 500, 500, 500, 650, N - 9],
     "one pair": lambda N: [0, N // 3, N],
     # more than a workgroup's threads, one row to a sequence, some without
     "many pairs": lambda N: [*range(0, N - 99), *[N - 99] * 5, *range(N - 99, N - 2, 3)],
 }
 
 
-@pytest.mark.parametrize("shape", LARGE, ids=["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("shape", LARGE, ids=["bf16", "fp32", "fp16", "fp32 long"])
 @pytest.mark.parametrize("which", LARGE_CU)
 def test_preference_of_more_logits_than_the_cache(shape, which):
     from ceo_amd import nn
