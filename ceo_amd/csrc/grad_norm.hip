@@ -14,8 +14,8 @@
 // fp32's range.  A NaN or an infinity anywhere gives norm NaN or inf, and the
 // gradients what the formula says (coef NaN or 0).
 //
-// Two reads and one write bound it: 368 million bf16 gradients take 375 us, 2.2 GB at
-// 5.9 TB/s (a large copy: 5.15; what the 256 MB cache keeps from the first read to the
+// Two reads and one write bound it: 368 million bf16 gradients take 351 us, 2.2 GB at
+// 6.3 TB/s (a large copy: 5.15; what the 256 MB cache keeps from the first read to the
 // second does not come from memory again).  14.5 million take 17 us, a small model's 23
 // gradients 7, and the host's two launches 9.
 #include <hip/hip_runtime.h>
@@ -53,8 +53,8 @@ struct List {
 
 // A unit, n elements from p on, in a workgroup's registers: 16-byte vectors from a cache
 // line's start on, kVecs to a thread, and the elements before and behind them (70 at
-// most), one to a thread.
-template <typename T>
+// most), one to a thread.  ONCE: nothing reads them again soon.
+template <typename T, bool ONCE>
 struct Unit {
     static constexpr int N = 16 / sizeof(T);
     typedef __attribute__((__vector_size__(16))) T Full;
@@ -73,7 +73,12 @@ struct Unit {
         for (int i = 0; i < kVecs; ++i) {
             const int c = threadIdx.x + i * NT;
             x[i] = Full{};
-            if (c < nv) x[i] = *reinterpret_cast<const Any*>(p + head + c * N);
+            if (c >= nv) continue;
+            const Any* from = reinterpret_cast<const Any*>(p + head + c * N);
+            if constexpr (ONCE)
+                x[i] = __builtin_nontemporal_load(from);
+            else
+                x[i] = *from;
         }
         one = (T)0.f;
         if ((int)threadIdx.x < edges) one = p[edge];
@@ -136,13 +141,13 @@ __global__ void __launch_bounds__(NT) norm_kernel(const Entry* __restrict__ entr
         int n;
         if (e.dtype == kDtypeBF16) {
             unit_of<bf16>(e, u, &at, &n);
-            s += Unit<bf16>((const bf16*)e.in + at, n).square_sum();
+            s += Unit<bf16, false>((const bf16*)e.in + at, n).square_sum();
         } else if (e.dtype == kDtypeF16) {
             unit_of<f16>(e, u, &at, &n);
-            s += Unit<f16>((const f16*)e.in + at, n).square_sum();
+            s += Unit<f16, false>((const f16*)e.in + at, n).square_sum();
         } else {
             unit_of<float>(e, u, &at, &n);
-            s += Unit<float>((const float*)e.in + at, n).square_sum();
+            s += Unit<float, false>((const float*)e.in + at, n).square_sum();
         }
     }
     s = block_sum(s, sm);
@@ -188,7 +193,7 @@ __device__ __forceinline__ void clip_unit(const Entry& e, uint32_t u, bool* know
     size_t at;
     int n;
     unit_of<T>(e, u, &at, &n);
-    const Unit<T> x((const T*)e.in + at, n);
+    const Unit<T, PAST> x((const T*)e.in + at, n);
     if (!*known) *f = factor(part, parts, max_norm, norm, sm);
     *known = true;
     if (*f == 1.f && e.in == e.out) return;  // nothing changes
@@ -205,7 +210,7 @@ clip_kernel(const Entry* __restrict__ entries, const uint32_t* __restrict__ map,
     float f = 1.f;
     if (units == 0) factor(part, parts, max_norm, norm, sm);
     // the last units first: of more gradients than the 256 MB cache holds it has those that
-    // the norm read last (368 million in bf16 380 us in all, 393 from the first on)
+    // the norm read last (368 million in bf16 380 us, 393 from the first on, all through the cache)
     for (uint32_t k = blockIdx.x; k < ((units + 7) & ~7u); k += gridDim.x) {
         const uint32_t u = (uint32_t)backwards(k, units);
         if (u >= units) continue;
@@ -335,8 +340,10 @@ extern "C" int grad_clip_hip(const void* list, float max_norm, float* norm, hipS
     rc = gn::sums(l, &parts, stream);
     if (rc != kSuccess) return rc;
     const dim3 grid(parts ? (parts + 7) / 8 * 8 : 1), block(gn::NT);
-    // outputs that the 256 MB cache does not hold are stored past it (380 us, 412 through it)
-    if (2 * l->bytes > (size_t)256 << 20)
+    // Where gradients and outputs are over half of the 256 MB cache, this pass leaves the cache
+    // to the gradients that the norm has read: it reads and writes past it (368 million in
+    // bf16 351 us, 412 through it; 23 million 43.6 and 53.6).
+    if (2 * l->bytes > (size_t)128 << 20)
         EFLA_LAUNCH("grad_clip", (gn::clip_kernel<true>), grid, block, stream, l->entries, l->map,
                     (uint32_t)l->units, l->part, (int)parts, max_norm, norm);
     else

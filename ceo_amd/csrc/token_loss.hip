@@ -49,7 +49,10 @@ struct Vec {
     static constexpr int N = 16 / sizeof(T);
     typedef __attribute__((__vector_size__(16))) T Full;
     typedef Full Any __attribute__((aligned(sizeof(T))));
+    // ONCE: nothing reads it again soon
+    template <bool ONCE>
     static __device__ __forceinline__ Full load(const T* p) {
+        if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const Any*>(p));
         return *reinterpret_cast<const Any*>(p);
     }
     template <bool PAST>
@@ -142,7 +145,7 @@ struct Span {
 
 // Rows of at most blockDim.x * NV vectors stay in registers: thread i holds vectors i,
 // i + blockDim.x, ... and one of the edges.
-template <typename T, int NV>
+template <typename T, int NV, bool ONCE>
 struct Row {
     static constexpr int N = Vec<T>::N;
     Span<T> p;
@@ -164,7 +167,7 @@ struct Row {
             const int c = threadIdx.x + i * blockDim.x;
 #pragma unroll
             for (int j = 0; j < N; ++j) x[i][j] = (T)-INFINITY;
-            if (c < p.nv) x[i] = Vec<T>::load(z + p.vec(c));
+            if (c < p.nv) x[i] = Vec<T>::template load<ONCE>(z + p.vec(c));
         }
         edge = (T)-INFINITY;
         if (threadIdx.x < p.edges) edge = z[p.edge(threadIdx.x)];
@@ -211,9 +214,10 @@ struct Row {
     }
 };
 
-// Longer rows stream: read once for the statistics and again for the gradient.
-template <typename T>
-struct Row<T, 0> {
+// Longer rows stream: read once for the statistics and again for the gradient (ONCE: if
+// for the former alone).
+template <typename T, bool ONCE>
+struct Row<T, 0, ONCE> {
     static constexpr int N = Vec<T>::N, U = 4;
     const T* z;
     Span<T> p;
@@ -229,7 +233,7 @@ struct Row<T, 0> {
                 const int c = c0 + u * blockDim.x;
 #pragma unroll
                 for (int j = 0; j < N; ++j) x[u][j] = (T)-INFINITY;
-                if (c < p.nv) x[u] = Vec<T>::load(z + p.vec(c));
+                if (c < p.nv) x[u] = Vec<T>::template load<ONCE>(z + p.vec(c));
             }
             float m = a.m;
 #pragma unroll
@@ -262,7 +266,7 @@ struct Row<T, 0> {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int c = c0 + u * blockDim.x;
-                if (c < p.nv) y[u] = Vec<T>::load(z + p.vec(c));
+                if (c < p.nv) y[u] = Vec<T>::template load<PAST>(z + p.vec(c));
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -306,7 +310,7 @@ __device__ __forceinline__ long block_row() {
     return blockIdx.x + (long)blockIdx.y * gridDim.x;
 }
 
-template <typename T, int NV>
+template <typename T, int NV, bool ONCE>
 __global__ void __launch_bounds__(kMaxThreads, NV > 8 ? 4 : 8)
 logprob_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets,
                const float* __restrict__ weights, float* __restrict__ logp, float2* stat,
@@ -322,7 +326,7 @@ logprob_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets
     }
     const T* z = logits + row * ld;
     const int t = targets[row];
-    const Row<T, NV> x(z, Span<T>(z, V));
+    const Row<T, NV, ONCE> x(z, Span<T>(z, V));
     const float zt = t >= 0 && t < V ? (float)z[t] : NAN;
     const Stat a = x.stat(sm);
     if (threadIdx.x == 0) {
@@ -361,7 +365,7 @@ policy_kernel(const T* logits, T* grad, PolicyArgs a) {
     const T* z = logits + row * a.ld;
     const int t = a.targets[row];
     const bool tok = t >= 0 && t < a.V;
-    const Row<T, NV> x(z, Span<T>(z, a.V));
+    const Row<T, NV, (PAST && NV > 0)> x(z, Span<T>(z, a.V));
     const float zt = tok ? (float)z[t] : 0.f;  // read before the gradient may overwrite it
     const float adv = a.adv[row];
     const float old = a.old ? a.old[row] : 0.f, ref = a.ref ? a.ref[row] : 0.f;
@@ -542,7 +546,7 @@ grad_kernel(const T* logits, T* grad, const int32_t* __restrict__ targets,
     const T* z = logits + row * ld;
     const Stat a{stat[row].x, stat[row].y};
     const float zt = (float)z[t];  // in place its own thread overwrites it, later
-    const Row<T, 0> x(z, Span<T>(z, V));
+    const Row<T, 0, false> x(z, Span<T>(z, V));
     x.template grad<PAST>(g, a, coef[row]);
     target_grad(g, x.p, t, zt, a, coef[row]);
 }
@@ -675,7 +679,7 @@ preference_kernel(const T* logits, T* grad, PrefArgs a) {
         if (!a.weights || a.weights[row] != 0.f) {
             const T* z = logits + row * a.ld;
             const int t = a.targets[row];
-            const Row<T, 0> x(z, Span<T>(z, a.V));
+            const Row<T, 0, false> x(z, Span<T>(z, a.V));
             const float zt = t >= 0 && t < a.V ? (float)z[t] : NAN;
             const Stat st = x.stat(sm);
             lp = (float)logp_of(st, zt);
@@ -724,7 +728,7 @@ preference_kernel(const T* logits, T* grad, PrefArgs a) {
         row_zero<PAST>(g, a.V);
         return;
     }
-    const Row<T, 0> x(z, Span<T>(z, a.V));
+    const Row<T, 0, false> x(z, Span<T>(z, a.V));
     const Stat st = sm_stat;
     const float coef = sm_coef;
     x.template grad<PAST>(g, st, coef);
@@ -773,7 +777,7 @@ static int check(const void* logits, const int32_t* targets, const void* grad, s
 // 32000 in bf16 takes 360 us with 4 vectors (378 with 8, 370 with 16), that of 20000 x
 // 1000 21 us (28, 44).  Log-probabilities, which write nothing, take 109 us with 8 and 131
 // with 4 for the former's logits, 40 % of the rows without weight; 2048 x 128003 take 90 us
-// streamed and 108 with 16.
+// streamed and 108 with 16 (all through the cache).
 struct Form {
     int nv;
     unsigned threads;
@@ -825,20 +829,24 @@ static dim3 row_grid(size_t rows) {
 
 // Whether logits and gradient are more than the 256 MB cache: then the gradient is stored
 // past it (policy loss of 16384 x 32000 in bf16 360 us, 369 through it; preference loss of
-// 8191 x 32000, whose second read the cache serves, 202 and 249); else what reads the
-// gradient next finds it there.
+// 8191 x 32000, whose second read the cache serves, 202 and 249), and what is read for the
+// last time read past it (log-probabilities of 16384 x 32000 98 us against 105, of 4096 x
+// 50257 in fp32 120 against 130; preference losses 1 to 4 %); else what comes next finds
+// them there.
 static bool past_cache(size_t rows, size_t vocab, int dtype) {
     return 2 * rows * vocab * dtype_size(dtype) > ((size_t)256 << 20);
 }
 
 static int logprob(const void* logits, const int32_t* targets, const float* weights, float* logp,
                    float2* stat, float* coef, size_t rows, size_t vocab, size_t ld, int dtype,
-                   Form f, hipStream_t st) {
+                   Form f, bool once, hipStream_t st) {
     TL_TYPED(dtype, T, {
         TL_FORM(f, NV, {
-            EFLA_LAUNCH("token_logprob", (logprob_kernel<T, NV>), row_grid(rows),
-                        dim3(f.threads), st, (const T*)logits, targets, weights, logp, stat, coef,
-                        (long)rows, (int)vocab, (long)ld);
+            TL_PAST(once, ONCE, {
+                EFLA_LAUNCH("token_logprob", (logprob_kernel<T, NV, ONCE>), row_grid(rows),
+                            dim3(f.threads), st, (const T*)logits, targets, weights, logp, stat,
+                            coef, (long)rows, (int)vocab, (long)ld);
+            });
         });
     });
     return (int)hipPeekAtLastError();
@@ -894,7 +902,8 @@ extern "C" int token_logprob_forward_hip(const void* logits, const int32_t* targ
     if (rc != kSuccess) return rc;
     if (!logp) return kInvalidValue;
     return tl::logprob(logits, targets, weights, logp, nullptr, nullptr, rows, vocab_size, ld,
-                       dtype, tl::form_of(vocab_size, dtype, 8, 8), stream);
+                       dtype, tl::form_of(vocab_size, dtype, 8, 8),
+                       tl::past_cache(rows, vocab_size, dtype), stream);
 }
 
 extern "C" int policy_loss_forward_backward_hip(
@@ -1000,7 +1009,7 @@ extern "C" int preference_loss_forward_backward_hip(
                                ? tl::Form{0, threads}
                                : tl::form_of(vocab_size, dtype, 8, 8);
         const int rc = tl::logprob(logits, targets, weights, logp, stat, coef, rows, vocab_size,
-                                   ld, dtype, f, stream);
+                                   ld, dtype, f, false, stream);
         if (rc != kSuccess) return rc;
     }
     if (pairs != 0) {
