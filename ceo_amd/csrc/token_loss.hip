@@ -559,10 +559,10 @@ grad_kernel(const T* logits, T* grad, const int32_t* __restrict__ targets,
 // The rows are drawn from a counter, so that a workgroup waits only for what has been
 // drawn before (a gradient for its pair's sums, a pair's last row for the pair's other
 // rows), by workgroups that run already and do their statistics first: every wait ends
-// whatever else the GPU does.  32 pairs of 4100 x 50257 in all: fp32 331 us against 398
-// in three launches, bf16 184 against 206; 8 pairs of 2048 x 128000 in bf16 205 against 213.
+// whatever else the GPU does.  32 pairs of 4100 x 50257 in all: fp32 323 us against 384
+// in three launches, bf16 178 against 195; 8 pairs of 2048 x 128000 in bf16 187 against 204.
 // Drawing takes 13 ns, one workgroup after another, so that shorter rows are faster in
-// three launches: 8 pairs of 8191 x 32000 in bf16 201 us against 223.
+// three launches: 8 pairs of 8191 x 32000 in bf16 195 us against 207.
 struct PairInfo {
     int pair, mid, end;  // of the pair that starts at this row
     uint32_t coef;       // d loss / d (sum of the chosen rows' w logp): a message
@@ -859,8 +859,8 @@ static bool streams(size_t rows, size_t vocab, int dtype) {
     return row >= (size_t)96 << 10 && rows * row > (size_t)256 << 20;
 }
 // Whether the preference loss takes the launch that draws rows (see there): for such logits
-// of pairs that the cache holds (8000 x 50257 in bf16, 4 pairs: 345 us against 347, 2 pairs
-// 380 against 350), and for a few short rows, where two launches instead of three count
+// of pairs that the cache holds (8000 x 50257 in bf16, 4 pairs: 303 us against 340, 2 pairs
+// 344 against 345, one 382 against 350), and for a few short rows, where two launches instead of three count
 // (45 x 32000 in bf16 18.0 us against 21.4; 256 rows 22.7 against 21.3, 45 x 128000 in
 // fp32 33 against 31).
 static bool draws(size_t rows, size_t pairs, size_t vocab, int dtype) {
@@ -869,12 +869,12 @@ static bool draws(size_t rows, size_t pairs, size_t vocab, int dtype) {
                                        : rows <= 128 && all <= (size_t)16 << 20;
 }
 // LDS that nobody uses: over half of a compute unit's, so that it has one workgroup, where the
-// rows in flight would else be as much as the cache (32 pairs of 2048 x 128000 in fp32 456 us,
-// 520 with two; in bf16 229 with either).
+// rows in flight would else be as much as the cache (32 pairs of 2048 x 128000 in fp32 411 us,
+// 432 with two; in bf16 187 with either, of 4100 x 50257 219 with one and 179 with two).
 static unsigned draw_lds(size_t vocab, int dtype) {
     return vocab * dtype_size(dtype) > (size_t)256 << 10 ? 84 << 10 : 0;
 }
-constexpr size_t kInFlight = (size_t)24 << 20;  // logits between a workgroup's two rows
+constexpr size_t kInFlight = (size_t)64 << 20;  // logits between a workgroup's two rows
 
 // The preference loss's scratch, of either kind.
 static size_t preference_scratch(size_t rows) {
