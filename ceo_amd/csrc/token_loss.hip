@@ -772,25 +772,41 @@ static int check(const void* logits, const int32_t* targets, const void* grad, s
         }                                \
     } while (0)
 
-// The form for rows of this length: vectors per thread (0: streamed) and threads, from
-// `least` vectors to `most`, as few as 1024 threads allow.  The policy loss of 16384 x
-// 32000 in bf16 takes 360 us with 4 vectors (378 with 8, 370 with 16), that of 20000 x
-// 1000 21 us (28, 44).  Log-probabilities, which write nothing, take 109 us with 8 and 131
-// with 4 for the former's logits, 40 % of the rows without weight; 2048 x 128003 take 90 us
-// streamed and 108 with 16 (all through the cache).
+// The form for rows of this length: vectors per thread (0: streamed) and threads.
 struct Form {
     int nv;
     unsigned threads;
 };
-static Form form_of(size_t vocab, int dtype, int least, int most) {
-    const size_t nv = vocab / (16 / dtype_size(dtype));
-    int k = least;
-    while (k <= most && nv > (size_t)k * kMaxThreads) k *= 2;
-    if (k > most) return Form{0, kMaxThreads};
-    const size_t least_threads = vocab >= kLineVocab ? kLineThreads : kWave;
+static Form form_with(size_t vocab, size_t nv, int k) {
+    const size_t least = vocab >= kLineVocab ? kLineThreads : kWave;
     const size_t need = (nv + k - 1) / k;
-    return Form{k, need < least_threads ? (unsigned)least_threads
-                                        : (unsigned)((need + kWave - 1) / kWave * kWave)};
+    return Form{k, need < least ? (unsigned)least : (unsigned)((need + kWave - 1) / kWave * kWave)};
+}
+// The policy loss: waves that fill whole rounds of a compute unit's four SIMDs, so the number
+// of vectors, 4 to 8 (to 16 where 8 do not hold the row), that leaves the fewest places of
+// such rounds empty, the smaller where two do.  In bf16, us with 4 to 8 vectors: 16384 x
+// 32000 354, 385, 357, 359, 359; x 28000 341, 310, 314, 309, 308; x 17000 197, 187, 186,
+// 187, 188; x 1000 18.7, 20.6, 21.8, 23.3, 23.7; 8192 x 36000 211 with 5, 201 with 6, 204,
+// 206; 4096 x 50257 147 with 7, 151 with 8; 2048 x 100000 161 with 13, 176 with 16.
+static Form policy_form(size_t vocab, int dtype) {
+    const size_t nv = vocab / (16 / dtype_size(dtype));
+    if (nv > 16 * kMaxThreads) return Form{0, kMaxThreads};
+    int best = 0;
+    size_t places = 0;
+    for (int k = 4; k <= (nv <= 8 * kMaxThreads ? 8 : 16); ++k) {
+        const size_t need = (nv + k - 1) / k, round = (need + 4 * kWave - 1) / (4 * kWave);
+        if (need > kMaxThreads || (best && k * round >= places)) continue;
+        best = k;
+        places = k * round;
+    }
+    return form_with(vocab, nv, best);
+}
+// Log-probabilities, which write nothing: 16384 x 32000 in bf16, 40 % of the rows without
+// weight, take 109 us with 8 vectors and 131 with 4; 2048 x 128003 90 us streamed and 108
+// with 16 (all through the cache).
+static Form logprob_form(size_t vocab, int dtype) {
+    const size_t nv = vocab / (16 / dtype_size(dtype));
+    return nv <= 8 * kMaxThreads ? form_with(vocab, nv, 8) : Form{0, kMaxThreads};
 }
 
 #define TL_PAST(past, PAST, ...)        \
@@ -804,22 +820,34 @@ static Form form_of(size_t vocab, int dtype, int least, int most) {
         }                               \
     } while (0)
 
-#define TL_FORM(form, NV, ...)      \
-    do {                            \
-        if ((form).nv == 4) {       \
-            constexpr int NV = 4;   \
-            __VA_ARGS__             \
-        } else if ((form).nv == 8) { \
-            constexpr int NV = 8;   \
-            __VA_ARGS__             \
-        } else if ((form).nv == 16) { \
-            constexpr int NV = 16;  \
-            __VA_ARGS__             \
-        } else {                    \
-            constexpr int NV = 0;   \
-            __VA_ARGS__             \
-        }                           \
-    } while (0)
+#define TL_CASE(k, NV, ...)      \
+    case k: {                    \
+        constexpr int NV = k;    \
+        __VA_ARGS__              \
+        break;                   \
+    }
+#define TL_POLICY_FORM(form, NV, ...)     \
+    switch ((form).nv) {                  \
+        TL_CASE(4, NV, __VA_ARGS__)       \
+        TL_CASE(5, NV, __VA_ARGS__)       \
+        TL_CASE(6, NV, __VA_ARGS__)       \
+        TL_CASE(7, NV, __VA_ARGS__)       \
+        TL_CASE(8, NV, __VA_ARGS__)       \
+        TL_CASE(9, NV, __VA_ARGS__)       \
+        TL_CASE(10, NV, __VA_ARGS__)      \
+        TL_CASE(11, NV, __VA_ARGS__)      \
+        TL_CASE(12, NV, __VA_ARGS__)      \
+        TL_CASE(13, NV, __VA_ARGS__)      \
+        TL_CASE(14, NV, __VA_ARGS__)      \
+        TL_CASE(15, NV, __VA_ARGS__)      \
+        TL_CASE(16, NV, __VA_ARGS__)      \
+        TL_CASE(0, NV, __VA_ARGS__)       \
+    }
+#define TL_LOGPROB_FORM(form, NV, ...)    \
+    switch ((form).nv) {                  \
+        TL_CASE(8, NV, __VA_ARGS__)       \
+        TL_CASE(0, NV, __VA_ARGS__)       \
+    }
 
 // A workgroup each; a grid's dimension times its threads stays below 2^32.
 static dim3 row_grid(size_t rows) {
@@ -841,7 +869,7 @@ static int logprob(const void* logits, const int32_t* targets, const float* weig
                    float2* stat, float* coef, size_t rows, size_t vocab, size_t ld, int dtype,
                    Form f, bool once, hipStream_t st) {
     TL_TYPED(dtype, T, {
-        TL_FORM(f, NV, {
+        TL_LOGPROB_FORM(f, NV, {
             TL_PAST(once, ONCE, {
                 EFLA_LAUNCH("token_logprob", (logprob_kernel<T, NV, ONCE>), row_grid(rows),
                             dim3(f.threads), st, (const T*)logits, targets, weights, logp, stat,
@@ -902,7 +930,7 @@ extern "C" int token_logprob_forward_hip(const void* logits, const int32_t* targ
     if (rc != kSuccess) return rc;
     if (!logp) return kInvalidValue;
     return tl::logprob(logits, targets, weights, logp, nullptr, nullptr, rows, vocab_size, ld,
-                       dtype, tl::form_of(vocab_size, dtype, 8, 8),
+                       dtype, tl::logprob_form(vocab_size, dtype),
                        tl::past_cache(rows, vocab_size, dtype), stream);
 }
 
@@ -926,9 +954,9 @@ extern "C" int policy_loss_forward_backward_hip(
     a.rows = (long)rows, a.V = (int)vocab_size, a.ld = (long)ld, a.ldg = (long)ld_grad;
     a.low = 1.f - clip_low, a.high = 1.f + clip_high, a.kl_coef = kl_coef;
     a.even = 1.f / (float)rows;
-    const tl::Form f = tl::form_of(vocab_size, dtype, 4, 16);
+    const tl::Form f = tl::policy_form(vocab_size, dtype);
     TL_TYPED(dtype, T, {
-        TL_FORM(f, NV, {
+        TL_POLICY_FORM(f, NV, {
             TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
                 EFLA_LAUNCH("policy_loss", (tl::policy_kernel<T, NV, PAST>), tl::row_grid(rows),
                             dim3(f.threads), stream, (const T*)logits, (T*)grad_logits, a);
@@ -1007,7 +1035,7 @@ extern "C" int preference_loss_forward_backward_hip(
         // the same sums as where rows are drawn, so that these do not depend on the gradient
         const tl::Form f = draws || tl::streams(rows, vocab_size, dtype)
                                ? tl::Form{0, threads}
-                               : tl::form_of(vocab_size, dtype, 8, 8);
+                               : tl::logprob_form(vocab_size, dtype);
         const int rc = tl::logprob(logits, targets, weights, logp, stat, coef, rows, vocab_size,
                                    ld, dtype, f, false, stream);
         if (rc != kSuccess) return rc;

@@ -758,3 +758,13 @@ def test_large_preferences_on_two_streams():
     for w, g in zip(want, got):
         for r in g:
             assert all(torch.equal(a, b) for a, b in zip(w, r))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [20483, 24571, 37001, 45003, 53249, 81001, 95003, 114699])
+def test_policy_rows_of_every_form(oracle, V, dtype):
+    """Row lengths for each number of vectors that a thread holds."""
+    announce(f"policy forms V={V} {dtype}")
+    x, d, _ = make(V, 3, V, dtype, pad=3, skew=5, masked=0.0)
+    check_policy(x, d, dtype, V)
+    check_policy(x, d, dtype, V, in_place=True)
