@@ -801,12 +801,23 @@ static Form policy_form(size_t vocab, int dtype) {
     }
     return form_with(vocab, nv, best);
 }
-// Log-probabilities, which write nothing: 16384 x 32000 in bf16, 40 % of the rows without
-// weight, take 109 us with 8 vectors and 131 with 4; 2048 x 128003 90 us streamed and 108
-// with 16 (all through the cache).
+// Log-probabilities, which write nothing, take workgroups as small as 8 vectors make them
+// (bf16, us with 4 to 8: 16384 x 28000 168, 161, 168, 142, 138; x 9000 56, 51, 47, 50, 54),
+// in rows of a few waves the number that leaves the fewest places empty (x 5000 32, 30, 31,
+// 33, 35; x 1000 11.0, 12.2, 13.4, 15.1, 16.6).  Where that would be over 640 threads the row
+// is streamed by 512 (4096 x 50257 67, 81 in registers; x 40000 58 and 57), and by 1024
+// where the policy loss streams too (2048 x 128003 82 with either): both then sum a row in
+// the same order.
 static Form logprob_form(size_t vocab, int dtype) {
     const size_t nv = vocab / (16 / dtype_size(dtype));
-    return nv <= 8 * kMaxThreads ? form_with(vocab, nv, 8) : Form{0, kMaxThreads};
+    if (nv > 8 * 640) return Form{0, nv > 16 * kMaxThreads ? unsigned(kMaxThreads) : 512u};
+    Form best = form_with(vocab, nv, 8);
+    if (nv > 8 * 256) return best;
+    for (int k = 7; k >= 4; --k) {
+        const Form f = form_with(vocab, nv, k);
+        if (f.nv * f.threads < best.nv * best.threads) best = f;
+    }
+    return best;
 }
 
 #define TL_PAST(past, PAST, ...)        \
@@ -845,6 +856,10 @@ static Form logprob_form(size_t vocab, int dtype) {
     }
 #define TL_LOGPROB_FORM(form, NV, ...)    \
     switch ((form).nv) {                  \
+        TL_CASE(4, NV, __VA_ARGS__)       \
+        TL_CASE(5, NV, __VA_ARGS__)       \
+        TL_CASE(6, NV, __VA_ARGS__)       \
+        TL_CASE(7, NV, __VA_ARGS__)       \
         TL_CASE(8, NV, __VA_ARGS__)       \
         TL_CASE(0, NV, __VA_ARGS__)       \
     }
