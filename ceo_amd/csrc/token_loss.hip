@@ -902,13 +902,14 @@ static bool streams(size_t rows, size_t vocab, int dtype) {
     return row >= (size_t)96 << 10 && rows * row > (size_t)256 << 20;
 }
 // Whether the preference loss takes the launch that draws rows (see there): for such logits
-// of pairs that the cache holds (8000 x 50257 in bf16, 4 pairs: 303 us against 340, 2 pairs
-// 344 against 345, one 382 against 350), and for a few short rows, where two launches instead of three count
-// (45 x 32000 in bf16 18.0 us against 21.4; 256 rows 22.7 against 21.3, 45 x 128000 in
-// fp32 33 against 31).
+// of pairs that the cache holds (8000 x 50257 in bf16, 30 % of the rows without weight: 4
+// pairs 302 us against 340, 3 pairs 320 against 341, 2 pairs 344 against 345, one 382 against
+// 352; all with weight: 409 against 425, 411 and 425, 420 and 428), and for a few short rows,
+// where two launches instead of three count (45 x 32000 in bf16 18.0 us against 21.4; 256
+// rows 22.7 against 21.3, 45 x 128000 in fp32 33 against 31).
 static bool draws(size_t rows, size_t pairs, size_t vocab, int dtype) {
     const size_t all = rows * vocab * dtype_size(dtype);
-    return streams(rows, vocab, dtype) ? pairs != 0 && all / pairs <= (size_t)192 << 20
+    return streams(rows, vocab, dtype) ? pairs != 0 && all / pairs <= (size_t)256 << 20
                                        : rows <= 128 && all <= (size_t)16 << 20;
 }
 // LDS that nobody uses: over half of a compute unit's, so that it has one workgroup, where the
