@@ -373,10 +373,11 @@ policy_kernel(const T* logits, T* grad, PolicyArgs a) {
     // the first wave turns the statistics into the row's outputs and its coefficient
     if (wave_id() == 0) {
         const double lp = logp_of(st, zt);
-        const float r = a.old ? expf((float)(lp - (double)old)) : 1.f;
-        const float rc = fminf(fmaxf(r, a.low), a.high);
-        float l = -fminf(r * adv, rc * adv);
-        float d = (adv >= 0.f ? r <= a.high : r >= a.low) ? -adv * r : 0.f;
+        // fminf and fmaxf drop a NaN, which has to reach the loss and the coefficient
+        const float r = a.old ? expf((float)(lp - (double)old)) : lp == lp ? 1.f : NAN;
+        const float u = r * adv, c = fminf(fmaxf(r, a.low), a.high) * adv;
+        float l = -(c < u ? c : u);
+        float d = (adv >= 0.f ? r > a.high : r < a.low) ? 0.f : -adv * r;
         float kl = 0.f;
         if (a.ref) {
             const float y = (float)((double)ref - lp);

@@ -665,10 +665,11 @@ def policy_loss(logits, targets, advantages, old_logp=None, ref_logp=None, weigh
     w = np.full(N, 1.0 / N) if weights is None else np.asarray(weights, dtype=np.float64)
     a = np.asarray(advantages, dtype=np.float64)
     with np.errstate(invalid="ignore", over="ignore"):
-        r = np.ones(N) if old_logp is None else np.exp(logp - np.asarray(old_logp, np.float64))
+        r = (np.where(np.isnan(logp), np.nan, 1.0) if old_logp is None
+             else np.exp(logp - np.asarray(old_logp, np.float64)))
         low, high = 1.0 - clip_low, 1.0 + clip_high
         loss = -np.minimum(r * a, np.clip(r, low, high) * a)
-        d = np.where(np.where(a >= 0, r <= high, r >= low), -a * r, 0.0)
+        d = np.where(np.where(a >= 0, r > high, r < low), 0.0, -a * r)
         kl = np.zeros(N)
         if ref_logp is not None:
             x = np.asarray(ref_logp, np.float64) - logp

@@ -322,6 +322,44 @@ def test_masked_rows_and_special_logits(oracle, V, dtype):
     within(grad[sel], rg, grad_tol(rg, rd, de, xs, dtype, V), "grad of masked logits")
 
 
+@pytest.mark.parametrize("old", [True, False], ids=["old", "itself"])
+@pytest.mark.parametrize("V", [70, 5000, 140000])
+def test_nan_reaches_the_policy_loss(oracle, V, old):
+    """Without a KL term to carry it: a row with NaN, +inf or nothing but -inf, and a NaN
+    or infinite statistic of the sampling policy."""
+    announce(f"nan in the policy loss V={V} old={old}")
+    from ceo_amd import nn
+
+    N = 10
+    x, d, _ = make(V, N, V, torch.bfloat16, masked=0.0)
+    x["w"][:] = 1.0
+    x["adv"][:] = [1, -1, 2, -2, 1, -1, 0, 0.5, -0.5, 1]
+    z = x["z"]
+    z[1, V // 3] = np.nan
+    z[2, V - 1] = np.inf
+    z[3] = -np.inf
+    z[4, 0] = np.nan
+    x["old"][5] = np.nan
+    x["old"][6] = -np.inf
+    x["adv"][8] = np.nan
+    d["z"].copy_(torch.from_numpy(z))
+    for k in ("w", "old", "adv"):
+        d[k].copy_(torch.from_numpy(x[k]))
+    rl, rlp, _, _, rg = oracle.policy_loss(z, x["t"], x["adv"], x["old"] if old else None, None,
+                                           x["w"])
+    bad = [1, 2, 3, 4, 8] + ([5, 6] if old else [])
+    assert sorted(np.flatnonzero(np.isnan(rl))) == sorted(bad)
+    for need in (True, False):
+        loss, logp, _, grad = nn.policy_loss_forward_backward(
+            d["z"], d["t"], d["adv"], d["old"] if old else None, None, d["w"], need_grad=need)
+        assert np.array_equal(np.isnan(loss.cpu().numpy()), np.isnan(rl))
+        assert np.array_equal(np.isnan(logp.cpu().numpy()), np.isnan(rlp))
+    grad = nn.policy_loss_forward_backward(d["z"], d["t"], d["adv"], d["old"] if old else None,
+                                           None, d["w"])[3]
+    assert np.array_equal(grad.isnan().all(1).cpu().numpy(), np.isnan(rg).all(1))
+    assert np.array_equal(grad.isnan().any(1).cpu().numpy(), np.isnan(rg).any(1))
+
+
 def test_everything_masked():
     from ceo_amd import nn
 
