@@ -491,7 +491,8 @@ struct PairLoss {
         const double minus = lg + fmax(x, 0.0);  // -log sig(-x)
         const double sig = x >= 0 ? 1.0 / (1.0 + u) : u / (1.0 + u);
         const double gis = x >= 0 ? u / (1.0 + u) : 1.0 / (1.0 + u);  // sig(-x)
-        loss = ((1.0 - eps) * plus + eps * minus) * inv_pairs;
+        // without smoothing the other side's term is not there, also where it is infinite
+        loss = ((1.0 - eps) * plus + (eps != 0.0 ? eps * minus : 0.0)) * inv_pairs;
         dx = (eps * sig - (1.0 - eps) * gis) * inv_pairs;
     }
 };

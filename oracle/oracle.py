@@ -696,7 +696,10 @@ def preference_loss(logits, targets, cu_seqlens, ref_logp=None, weights=None, be
     rewards = beta * np.array([term[cu[s]:cu[s + 1]].sum() for s in range(2 * P)])
     x = rewards[0::2] - rewards[1::2]
     e = label_smoothing
-    loss = ((1 - e) * np.logaddexp(0.0, -x) + e * np.logaddexp(0.0, x)) / P
+    loss = np.logaddexp(0.0, -x)
+    if e != 0:
+        loss = (1 - e) * loss + e * np.logaddexp(0.0, x)
+    loss = loss / P
     sig = np.exp(-np.logaddexp(0.0, -x))
     gis = np.exp(-np.logaddexp(0.0, x))
     dx = (e * sig - (1 - e) * gis) / P

@@ -360,6 +360,42 @@ def test_nan_reaches_the_policy_loss(oracle, V, old):
     assert np.array_equal(grad.isnan().any(1).cpu().numpy(), np.isnan(rg).any(1))
 
 
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+@pytest.mark.parametrize("N", [24, 400])
+def test_preference_of_impossible_tokens(oracle, N, smoothing):
+    """A target at -inf in the chosen, the rejected or both sequences: an infinite margin
+    costs nothing on its right side, where no smoothing asks for the other."""
+    announce(f"impossible tokens N={N} smoothing={smoothing}")
+    from ceo_amd import nn
+
+    V, P = 70, 4
+    x, d, _ = make(N, N, V, torch.float32, masked=0.0)
+    x["w"][:] = 1.0
+    cu = np.linspace(0, N, 2 * P + 1).astype(np.int32)
+    z = x["z"]
+    for s in (0, 3, 4, 5):  # chosen, rejected, both; the last pair as it is
+        z[cu[s], x["t"][cu[s]]] = -np.inf
+    d["z"].copy_(torch.from_numpy(z))
+    d["w"].copy_(torch.from_numpy(x["w"]))
+    with np.errstate(invalid="ignore"):
+        rl, rr, _, rd, rg = oracle.preference_loss(z, x["t"], cu, x["ref"], x["w"],
+                                                   label_smoothing=smoothing)
+    assert rl[0] == np.inf and np.isnan(rl[2]) and np.isfinite(rl[3])
+    assert rl[1] == (0.0 if smoothing == 0 else np.inf)
+    for need in (True, False):
+        loss, rewards, _, grad = nn.preference_loss_forward_backward(
+            d["z"], d["t"], torch.from_numpy(cu).cuda(), d["ref"], d["w"],
+            label_smoothing=smoothing, need_grad=need)
+        assert np.array_equal(loss[:3].cpu().numpy(), rl[:3].astype(np.float32), equal_nan=True)
+        assert np.array_equal(np.isinf(rewards.cpu().numpy()), np.isinf(rr))
+        if need:
+            g = grad[:cu[4]].cpu().numpy().astype(np.float64)
+            # an infinite margin's factor is exact, the softmax as good as its sum
+            assert (np.abs(g - rg[:cu[4]]) <= np.abs(rd[:cu[4], None]) * (rel(V) + 64 * U)).all()
+            assert bool(grad[cu[4]:cu[6]].isnan().any(1).all())
+            assert bool(grad[cu[6]:].isfinite().all())
+
+
 def test_everything_masked():
     from ceo_amd import nn
 
