@@ -478,6 +478,21 @@ struct PairSum {
             for (int k = 1; k < NT / kWave; ++k) sum[q] += sm[q][k];
         }
     }
+
+    // by one wave, a row at most to each lane: the same sums as the workgroup's
+    __device__ __forceinline__ PairSum(const float* logp, const float* ref, const float* weights,
+                                       int a0, int a1, int a2) {
+        const int i = a0 + lane_id();
+        const float w = i >= a2 ? 0.f : weights ? weights[i] : 1.f;
+        const float lp = i < a2 ? logp[i] : 0.f, rf = ref && i < a2 ? ref[i] : 0.f;
+        const double d = w != 0.f ? (double)w * ((double)lp - (double)rf) : 0.0;
+        sum[0] = 0.0 + (i < a1 ? d : 0.0);
+        sum[1] = 0.0 + (i < a1 ? 0.0 : d);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) sum[q] += __shfl_xor(sum[q], off);
+    }
 };
 
 // loss and d loss / dx of a pair whose rewards differ by x
@@ -497,36 +512,76 @@ struct PairLoss {
     }
 };
 
-// One pair of sequences: their sums, the pair's loss, and each row's coefficient.  An
-// offset is taken as at least all before it and at most the rows.
+// The pairs' sums and losses, and each row's coefficient.  A pair to a workgroup, or, of MANY
+// pairs, `each` of them, as many at a time as it has waves: each wave one of up to 64 rows,
+// the workgroup the longer ones.  An offset is taken as at least all before it, which the
+// workgroup looks through for its first pair, and at most the rows.
+template <bool MANY>
 __global__ void __launch_bounds__(NT)
 pair_kernel(const int32_t* __restrict__ cu, float* logp,
             const float* __restrict__ ref, const float* __restrict__ weights, int rows,
-            float beta, float eps, float inv_pairs, float* __restrict__ loss,
-            float* __restrict__ rewards, float* __restrict__ coef) {
-    __shared__ int sm_low[NT / kWave];
-    const long pair = blockIdx.x;
-    int at[3], low = 0;
-    for (long i = threadIdx.x; i < 2 * pair; i += NT) low = max(low, cu[i]);
+            int pairs, int each, float beta, float eps, float inv_pairs,
+            float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ coef) {
+    constexpr int kWaves = NT / kWave;
+    __shared__ int sm_low[kWaves];
+    const long begin = (long)blockIdx.x * each;
+    const long end = begin + each < pairs ? begin + each : pairs;
+    int low = 0;
+    constexpr int U = 16;  // loads on their way together
+    for (long i0 = threadIdx.x; i0 < 2 * begin; i0 += U * NT) {
+        int v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = i0 + u * NT < 2 * begin ? cu[i0 + u * NT] : 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) low = max(low, v[u]);
+    }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) low = max(low, __shfl_xor(low, off));
     if (lane_id() == 0) sm_low[wave_id()] = low;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NT / kWave; ++k) low = max(low, sm_low[k]);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) at[i] = low = min(max(low, cu[2 * pair + i]), rows);
-    const PairSum d(logp, ref, weights, at[0], at[1], at[2], false);
-    const PairLoss l((double)beta * (d.sum[0] - d.sum[1]), eps, inv_pairs);
-    if (threadIdx.x == 0) {
-        loss[pair] = (float)l.loss;
-        rewards[2 * pair] = (float)((double)beta * d.sum[0]);
-        rewards[2 * pair + 1] = (float)((double)beta * d.sum[1]);
-    }
-    if (coef) {
+    for (int k = 0; k < kWaves; ++k) low = max(low, sm_low[k]);
+    const auto finish = [&](long pair, const int* at, const PairSum& d, int tid, int threads) {
+        const PairLoss l((double)beta * (d.sum[0] - d.sum[1]), eps, inv_pairs);
+        if (tid == 0) {
+            loss[pair] = (float)l.loss;
+            rewards[2 * pair] = (float)((double)beta * d.sum[0]);
+            rewards[2 * pair + 1] = (float)((double)beta * d.sum[1]);
+        }
+        if (!coef) return;
         const float c = (float)((double)beta * l.dx);
-        for (int i = at[0] + threadIdx.x; i < at[2]; i += NT)
+        for (int i = at[0] + tid; i < at[2]; i += threads)
             coef[i] = (i < at[1] ? c : -c) * (weights ? weights[i] : 1.f);
+    };
+    if constexpr (!MANY) {
+        int at[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) at[i] = low = min(max(low, cu[2 * begin + i]), rows);
+        finish(begin, at, PairSum(logp, ref, weights, at[0], at[1], at[2], false), threadIdx.x,
+               NT);
+        return;
+    }
+    for (long p0 = begin; p0 < end; p0 += kWaves) {
+        int at[kWaves][3], own[3] = {0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < kWaves; ++q)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                if (p0 + q < end) low = min(max(low, cu[2 * (p0 + q) + i]), rows);
+                at[q][i] = low;
+                if (q == wave_id()) own[i] = low;
+            }
+        if (p0 + wave_id() < end && own[2] - own[0] <= kWave)
+            finish(p0 + wave_id(), own, PairSum(logp, ref, weights, own[0], own[1], own[2]),
+                   lane_id(), kWave);
+#pragma unroll
+        for (int q = 0; q < kWaves; ++q) {
+            if (at[q][2] - at[q][0] <= kWave) continue;
+            __syncthreads();  // the last such pair's sums have been read
+            finish(p0 + q, at[q],
+                   PairSum(logp, ref, weights, at[q][0], at[q][1], at[q][2], false), threadIdx.x,
+                   NT);
+        }
     }
 }
 
@@ -822,13 +877,13 @@ static Form logprob_form(size_t vocab, int dtype) {
     return best;
 }
 
-#define TL_PAST(past, PAST, ...)        \
+#define TL_IF(cond, NAME, ...)          \
     do {                                \
-        if (past) {                     \
-            constexpr bool PAST = true; \
+        if (cond) {                     \
+            constexpr bool NAME = true; \
             __VA_ARGS__                 \
         } else {                        \
-            constexpr bool PAST = false; \
+            constexpr bool NAME = false; \
             __VA_ARGS__                 \
         }                               \
     } while (0)
@@ -887,7 +942,7 @@ static int logprob(const void* logits, const int32_t* targets, const float* weig
                    Form f, bool once, hipStream_t st) {
     TL_TYPED(dtype, T, {
         TL_LOGPROB_FORM(f, NV, {
-            TL_PAST(once, ONCE, {
+            TL_IF(once, ONCE, {
                 EFLA_LAUNCH("token_logprob", (logprob_kernel<T, NV, ONCE>), row_grid(rows),
                             dim3(f.threads), st, (const T*)logits, targets, weights, logp, stat,
                             coef, (long)rows, (int)vocab, (long)ld);
@@ -921,6 +976,12 @@ static unsigned draw_lds(size_t vocab, int dtype) {
     return vocab * dtype_size(dtype) > (size_t)256 << 10 ? 84 << 10 : 0;
 }
 constexpr size_t kInFlight = (size_t)64 << 20;  // logits between a workgroup's two rows
+
+// Workgroups of the pairs' launch: as many at most as run at once with room to spare, since
+// each looks through the offsets before its own (131072 rows of 200 in bf16, 65536 pairs: 243
+// us with 1024 workgroups, 264 with 512, 252 with 2048, 1140 with one to a pair; 16384 x 1000,
+// 8192 pairs: 40.8, 43.0, 43.2, 61.8).
+constexpr size_t kPairGroups = 1024;
 
 // The preference loss's scratch, of either kind.
 static size_t preference_scratch(size_t rows) {
@@ -975,7 +1036,7 @@ extern "C" int policy_loss_forward_backward_hip(
     const tl::Form f = tl::policy_form(vocab_size, dtype);
     TL_TYPED(dtype, T, {
         TL_POLICY_FORM(f, NV, {
-            TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
+            TL_IF(tl::past_cache(rows, vocab_size, dtype), PAST, {
                 EFLA_LAUNCH("policy_loss", (tl::policy_kernel<T, NV, PAST>), tl::row_grid(rows),
                             dim3(f.threads), stream, (const T*)logits, (T*)grad_logits, a);
             });
@@ -1038,7 +1099,7 @@ extern "C" int preference_loss_forward_backward_hip(
         if (rc != kSuccess) return rc;
         // the lag is known on the device: as many as it may take
         TL_TYPED(dtype, T, {
-            TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
+            TL_IF(tl::past_cache(rows, vocab_size, dtype), PAST, {
                 EFLA_LAUNCH_LDS("preference_loss", (tl::preference_kernel<T, PAST>),
                                 tl::row_grid(2 * rows), dim3(threads),
                                 tl::draw_lds(vocab_size, dtype), stream, (const T*)logits,
@@ -1059,15 +1120,19 @@ extern "C" int preference_loss_forward_backward_hip(
         if (rc != kSuccess) return rc;
     }
     if (pairs != 0) {
-        EFLA_LAUNCH("preference_pairs", tl::pair_kernel, dim3((unsigned)pairs), dim3(tl::NT),
-                    stream, cu_seqlens, logp, ref_logp, weights, (int)rows, beta,
-                    label_smoothing, inv_pairs, loss, rewards, coef);
+        const size_t each = (pairs + tl::kPairGroups - 1) / tl::kPairGroups;
+        TL_IF(each > 1, MANY, {
+            EFLA_LAUNCH("preference_pairs", tl::pair_kernel<MANY>,
+                        dim3((unsigned)((pairs + each - 1) / each)), dim3(tl::NT), stream,
+                        cu_seqlens, logp, ref_logp, weights, (int)rows, (int)pairs, (int)each,
+                        beta, label_smoothing, inv_pairs, loss, rewards, coef);
+        });
         const int rc = (int)hipPeekAtLastError();
         if (rc != kSuccess) return rc;
     }
     if (grad_logits && rows != 0) {
         TL_TYPED(dtype, T, {
-            TL_PAST(tl::past_cache(rows, vocab_size, dtype), PAST, {
+            TL_IF(tl::past_cache(rows, vocab_size, dtype), PAST, {
                 EFLA_LAUNCH("preference_grad", (tl::grad_kernel<T, PAST>), tl::row_grid((rows + 7) & ~(size_t)7),
                             dim3(threads), stream, (const T*)logits, (T*)grad_logits, targets,
                             weights, stat, coef, (long)rows, (int)vocab_size, (long)ld,

@@ -180,6 +180,34 @@ def test_many_rows(oracle, N, V, dtype):
     check_preference(x, d, [0, *cut.tolist(), N], dtype, V)
 
 
+@pytest.mark.parametrize("pairs,longest", [(1024, 3), (1025, 3), (2500, 2), (6001, 1)])
+def test_preference_of_many_pairs(oracle, pairs, longest):
+    """More pairs than workgroups: empty sequences, short ones, some of over a wave's 64 rows
+    next to each other, some of exactly 64 and 65; offsets behind their predecessors."""
+    from ceo_amd import nn
+
+    announce(f"preference of {pairs} pairs")
+    rng = np.random.default_rng(pairs)
+    lengths = rng.integers(0, longest + 1, 2 * pairs)
+    for at in (0, 40, 41, 42, pairs // 2, pairs - 1):
+        lengths[2 * at:2 * at + 2] = rng.integers(20, 300, 2)
+    lengths[20:24] = [64, 0, 30, 35]
+    cu = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    N, V = int(cu[-1]), 37
+    x, d, _ = make(pairs, N, V, torch.bfloat16)
+    check_preference(x, d, cu.tolist(), torch.bfloat16, V)
+    # the same offsets after clamping
+    odd = cu.copy()
+    back = np.flatnonzero(np.diff(cu) == 0) + 1
+    odd[back] -= rng.integers(0, 50, len(back)).astype(np.int32)
+    odd[-1] = N + 5
+    f = lambda c, need: nn.preference_loss_forward_backward(  # noqa: E731
+        d["z"], d["t"], torch.from_numpy(c).cuda(), d["ref"], d["w"], need_grad=need)
+    want, got, only = f(cu, True), f(odd, True), f(odd, False)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    assert all(torch.equal(p, q) for p, q in zip(want[:3], only[:3]))
+
+
 @pytest.mark.parametrize("lengths", [[0, 5, 3, 0], [1, 1], [0, 0, 0, 8], [2, 1, 0, 0, 3, 2]])
 def test_preference_short_and_empty_sequences(oracle, lengths):
     announce(f"preference lengths {lengths}")
