@@ -550,8 +550,10 @@ pair_kernel(const int32_t* __restrict__ cu, float* logp,
         }
         if (!coef) return;
         const float c = (float)((double)beta * l.dx);
-        for (int i = at[0] + tid; i < at[2]; i += threads)
-            coef[i] = (i < at[1] ? c : -c) * (weights ? weights[i] : 1.f);
+        for (int i = at[0] + tid; i < at[2]; i += threads) {
+            const float w = weights ? weights[i] : 1.f;
+            coef[i] = w != 0.f ? (i < at[1] ? c : -c) * w : 0.f;  // 0 also of a NaN
+        }
     };
     if constexpr (!MANY) {
         int at[3];
@@ -588,15 +590,18 @@ pair_kernel(const int32_t* __restrict__ cu, float* logp,
 template <typename T, bool PAST>
 __global__ void __launch_bounds__(kMaxThreads)
 grad_kernel(const T* logits, T* grad, const int32_t* __restrict__ targets,
-            const float* __restrict__ weights, const float2* __restrict__ stat,
-            const float* __restrict__ coef, long rows, int V, long ld, long ldg) {
+            const float2* __restrict__ stat, const float* __restrict__ coef, long rows, int V,
+            long ld, long ldg) {
     // the last rows first: of more logits than the 256 MB cache holds it has those that the
     // statistics read last (8191 x 32000 in bf16 200 us in all, 230 from the first on)
     const long row = backwards(block_row(), rows);
     if (row < 0 || row >= rows) return;
     T* g = grad + row * ldg;
     const int t = targets[row];
-    if ((weights && weights[row] == 0.f) || t < 0 || t >= V) {
+    const float c = coef[row];
+    // 0: a row without weight or outside of every sequence, whose logits may be anything (one
+    // that counts has NaN here where its statistics are), or a pair without a gradient
+    if (c == 0.f || t < 0 || t >= V) {
         row_zero<PAST>(g, V);
         return;
     }
@@ -604,8 +609,8 @@ grad_kernel(const T* logits, T* grad, const int32_t* __restrict__ targets,
     const Stat a{stat[row].x, stat[row].y};
     const float zt = (float)z[t];  // in place its own thread overwrites it, later
     const Row<T, 0, false> x(z, Span<T>(z, V));
-    x.template grad<PAST>(g, a, coef[row]);
-    target_grad(g, x.p, t, zt, a, coef[row]);
+    x.template grad<PAST>(g, a, c);
+    target_grad(g, x.p, t, zt, a, c);
 }
 
 // The preference loss of more logits than the 256 MB cache holds, in one launch.  Each
@@ -1135,8 +1140,7 @@ extern "C" int preference_loss_forward_backward_hip(
             TL_IF(tl::past_cache(rows, vocab_size, dtype), PAST, {
                 EFLA_LAUNCH("preference_grad", (tl::grad_kernel<T, PAST>), tl::row_grid((rows + 7) & ~(size_t)7),
                             dim3(threads), stream, (const T*)logits, (T*)grad_logits, targets,
-                            weights, stat, coef, (long)rows, (int)vocab_size, (long)ld,
-                            (long)ld_grad);
+                            stat, coef, (long)rows, (int)vocab_size, (long)ld, (long)ld_grad);
             });
         });
     }

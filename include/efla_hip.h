@@ -638,8 +638,8 @@ size_t preference_loss_workspace_size(size_t rows);
  * and d sum(loss) / d logits.  ref_logp NULL: 0; weights NULL: 1 each (1 / length
  * gives means instead of sums).  Sums are 64 bits, in a fixed order.  Sequences may
  * be empty; offsets are clamped to the rows and to their predecessors; rows outside
- * of every sequence have gradient 0.  A NaN in one row makes its pair's loss, rewards
- * and gradient NaN.  The workspace (any contents, one call at a time) may be NULL: the
+ * of every sequence have gradient 0 whatever their logits are (their log-probability is
+ * given).  A NaN in one row makes its pair's loss, rewards and gradient NaN.  The workspace (any contents, one call at a time) may be NULL: the
  * stream's cached one; only a call with grad_logits needs any.  beta not positive and
  * finite, eps outside [0, 1), or a workspace that is too small -> 1; rows past 2^30 -> 9. */
 int preference_loss_forward_backward_hip(

@@ -704,9 +704,13 @@ def preference_loss(logits, targets, cu_seqlens, ref_logp=None, weights=None, be
     gis = np.exp(-np.logaddexp(0.0, x))
     dx = (e * sig - (1 - e) * gis) / P
     d = np.zeros(N)
+    inside = np.zeros(N, bool)
     for i in range(P):
+        inside[cu[2 * i]:cu[2 * i + 2]] = True
         for s, sign in ((2 * i, 1.0), (2 * i + 1, -1.0)):
             d[cu[s]:cu[s + 1]] = sign * beta * dx[i] * w[cu[s]:cu[s + 1]]
+    # rows outside of every sequence have no gradient, whatever their logits are
+    on = on & inside
     d = np.where(on & tok, d, 0.0)
     return loss, rewards, logp, d, _row_gradient(p, targets, on, tok, d)
 

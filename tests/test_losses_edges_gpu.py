@@ -1,0 +1,91 @@
+"""Rows at the edges of the losses on rewards and preferences: rows outside of every
+sequence, and beside a NaN."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import announce
+
+pytestmark = pytest.mark.gpu
+
+
+# the launch that draws rows and the three launches, for a few rows, for more, for pairs in
+# groups and for logits of over 256 MiB in short and in long rows
+OUTSIDE = {
+    "few rows, one launch": (100, 70, torch.bfloat16, [3, 20, 50, 70, 90]),
+    "three launches": (300, 70, torch.bfloat16, [5, 100, 290]),
+    "rows in registers": (200, 20000, torch.float16, [1, 60, 120, 121, 180]),
+    "pairs in groups": (5000, 64, torch.float32, [*range(7, 4994, 2)]),
+    "short rows past the cache": (4400, 32000, torch.bfloat16, [9, 1000, 2000, 3000, 4391]),
+    "long rows past the cache, one launch": (2700, 50257, torch.bfloat16,
+                                             [9, 700, 1500, 2000, 2600]),
+    "long rows past the cache, one pair": (2700, 50257, torch.bfloat16, [9, 1300, 2692]),
+}
+
+
+@pytest.mark.parametrize("weighted", [False, True], ids=["all count", "weights"])
+@pytest.mark.parametrize("which", OUTSIDE)
+def test_rows_outside_of_every_sequence(which, weighted):
+    """Before the first offset and behind the last the gradient is 0 whatever the logits
+    are, NaN, +inf and nothing but -inf among them; the pairs' bits are those that they
+    have beside ordinary rows."""
+    from ceo_amd import nn
+
+    N, V, dtype, cu = OUTSIDE[which]
+    cu = cu if len(cu) % 2 else cu[:-1]
+    announce(f"rows outside of every sequence: {which}, weights {weighted}")
+    g = torch.Generator(device="cuda").manual_seed(N)
+    z = torch.empty(N, V, dtype=dtype, device="cuda").normal_(0, 2, generator=g)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda", dtype=torch.int32)
+    ref = torch.full((N,), -float(np.log(V)) - 2.0, device="cuda")
+    w = torch.rand(N, generator=g, device="cuda") + 0.5 if weighted else None
+    offsets = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    out = torch.ones(N, dtype=torch.bool, device="cuda")
+    out[cu[0]:cu[-1]] = False
+    rows = out.nonzero()[:, 0]
+
+    def call(logits, **kw):
+        return nn.preference_loss_forward_backward(logits, t, offsets, ref, w, beta=0.01, **kw)
+    want = call(z)
+    assert not want[3][out].any() and bool(want[3][~out].any(1).all())
+    # each side has all four kinds of rows, or as many as it has rows
+    z[rows[0::4], V // 2] = float("nan")
+    z[rows[1::4], V - 1] = float("inf")
+    z[rows[2::4]] = float("-inf")
+    got = call(z)
+    assert all(torch.equal(p, q) for p, q in zip(want[:2], got[:2]))
+    assert torch.equal(want[2][~out], got[2][~out])
+    bad = torch.cat([rows[0::4], rows[1::4], rows[2::4]])
+    assert bool(got[2][bad].isnan().all())
+    assert not got[3][out].any()  # a NaN counts as any
+    assert torch.equal(want[3], got[3])
+    place = z.clone()
+    again = call(place, in_place=True)
+    assert again[3] is place and torch.equal(want[3], place)
+
+
+@pytest.mark.parametrize("which", OUTSIDE)
+def test_rows_without_weight_in_a_pair_that_is_nan(which):
+    """One row of the first pair is NaN: the pair's other rows that count are, those without
+    weight have gradient 0, and the other pairs keep their bits."""
+    from ceo_amd import nn
+
+    N, V, dtype, cu = OUTSIDE[which]
+    cu = cu if len(cu) % 2 else cu[:-1]
+    announce(f"a pair that is NaN: {which}")
+    g = torch.Generator(device="cuda").manual_seed(N + 1)
+    z = torch.empty(N, V, dtype=dtype, device="cuda").normal_(0, 2, generator=g)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda", dtype=torch.int32)
+    w = torch.ones(N, device="cuda")
+    w[cu[0] + 1:cu[2]:2] = 0.0
+    offsets = torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+    def call():
+        return nn.preference_loss_forward_backward(z, t, offsets, None, w, beta=0.001)
+    want = call()
+    z[cu[0], 0] = float("nan")
+    got = call()
+    assert bool(got[0][0].isnan()) and torch.equal(got[0][1:], want[0][1:])
+    pair = got[3][cu[0]:cu[2]]
+    assert bool(pair[0::2].isnan().all()) and not pair[1::2].any()
+    assert torch.equal(got[3][cu[2]:], want[3][cu[2]:])

@@ -125,3 +125,17 @@ def test_clip_coef_against_torch(oracle, max_norm):
     assert abs(n.item() - norm) <= 1e-12 * norm
     for p, b in zip(ps, before):
         assert np.allclose(p.grad.numpy(), c * b, rtol=1e-12)
+
+
+def test_rows_outside_of_every_sequence(oracle):
+    """Their gradient is 0 and the pair's what it is alone, whatever their logits are."""
+    x = _inputs(4, 12, 6)
+    x["w"][:] = 1.0
+    cu = [2, 5, 9]
+    alone = oracle.preference_loss(x["z"][2:9], x["t"][2:9], [0, 3, 7], x["ref"][2:9])
+    x["z"][0], x["z"][1, 3], x["z"][9, 0], x["z"][10] = np.nan, np.inf, np.nan, -np.inf
+    for w in (None, x["w"]):
+        loss, r, _, d, g = oracle.preference_loss(x["z"], x["t"], cu, x["ref"], w)
+        assert np.array_equal(loss, alone[0]) and np.array_equal(r, alone[1])
+        assert not d[[0, 1, 9, 10, 11]].any() and not g[[0, 1, 9, 10, 11]].any()
+        assert np.array_equal(g[2:9], alone[4])
