@@ -377,7 +377,8 @@ policy_kernel(const T* logits, T* grad, PolicyArgs a) {
         const float r = a.old ? expf((float)(lp - (double)old)) : lp == lp ? 1.f : NAN;
         const float u = r * adv, c = fminf(fmaxf(r, a.low), a.high) * adv;
         float l = -(c < u ? c : u);
-        float d = (adv >= 0.f ? r > a.high : r < a.low) ? 0.f : -adv * r;
+        // an advantage that is NaN is on neither side
+        float d = (adv >= 0.f && r > a.high) || (adv < 0.f && r < a.low) ? 0.f : -adv * r;
         float kl = 0.f;
         if (a.ref) {
             const float y = (float)((double)ref - lp);

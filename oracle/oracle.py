@@ -669,7 +669,7 @@ def policy_loss(logits, targets, advantages, old_logp=None, ref_logp=None, weigh
              else np.exp(logp - np.asarray(old_logp, np.float64)))
         low, high = 1.0 - clip_low, 1.0 + clip_high
         loss = -np.minimum(r * a, np.clip(r, low, high) * a)
-        d = np.where(np.where(a >= 0, r > high, r < low), 0.0, -a * r)
+        d = np.where(((a >= 0) & (r > high)) | ((a < 0) & (r < low)), 0.0, -a * r)
         kl = np.zeros(N)
         if ref_logp is not None:
             x = np.asarray(ref_logp, np.float64) - logp

@@ -1,10 +1,11 @@
 """Rows at the edges of the losses on rewards and preferences: rows outside of every
-sequence, and beside a NaN."""
+sequence, and beside a NaN, advantages that are NaN."""
 import numpy as np
 import pytest
 import torch
 
 from helpers import announce
+from test_losses_gpu import POLICY, make
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,34 @@ def test_rows_without_weight_in_a_pair_that_is_nan(which):
     pair = got[3][cu[0]:cu[2]]
     assert bool(pair[0::2].isnan().all()) and not pair[1::2].any()
     assert torch.equal(got[3][cu[2]:], want[3][cu[2]:])
+
+
+@pytest.mark.parametrize("kl_coef", [0.0, 0.05])
+@pytest.mark.parametrize("V", [70, 5000, 140000])
+def test_nan_advantages_reach_loss_and_gradient(oracle, V, kl_coef):
+    """Whichever side of the clipping the ratio is on: below it, inside, above it."""
+    announce(f"NaN advantages V={V} kl_coef={kl_coef}")
+    from ceo_amd import nn
+
+    N = 6
+    x, d, _ = make(V + 3, N, V, torch.bfloat16, masked=0.0)
+    x["w"][:] = 1.0
+    lp = oracle.token_logprob(x["z"], x["t"])
+    x["old"] = (lp + np.array([1.0, 1.0, 0.0, 0.0, -1.0, -1.0])).astype(np.float32)
+    x["adv"][0::2] = np.nan
+    x["adv"][1::2] = [-1.5, 1.5, 1.5]  # clipped, free and clipped
+    for k in ("w", "old", "adv"):
+        d[k].copy_(torch.from_numpy(x[k]))
+    a = {**POLICY, "kl_coef": kl_coef}
+    rl, _, _, rd, rg = oracle.policy_loss(x["z"], x["t"], x["adv"], x["old"], x["ref"], x["w"],
+                                          **a)
+    assert np.isnan(rl[0::2]).all() and np.isnan(rd[0::2]).all() and np.isnan(rg[0::2]).all()
+    if kl_coef == 0:
+        assert rd[1] == 0 and rd[3] != 0 and rd[5] == 0
+    loss, logp, kl, grad = nn.policy_loss_forward_backward(
+        d["z"], d["t"], d["adv"], d["old"], d["ref"], d["w"], **a)
+    assert bool(loss[0::2].isnan().all()) and bool(grad[0::2].isnan().all())
+    assert bool(loss[1::2].isfinite().all()) and bool(grad[1::2].isfinite().all())
+    assert bool(logp.isfinite().all()) and bool(kl.isfinite().all())
+    if kl_coef == 0:
+        assert not grad[1].any() and bool(grad[3].any()) and not grad[5].any()

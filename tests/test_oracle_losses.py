@@ -139,3 +139,14 @@ def test_rows_outside_of_every_sequence(oracle):
         assert np.array_equal(loss, alone[0]) and np.array_equal(r, alone[1])
         assert not d[[0, 1, 9, 10, 11]].any() and not g[[0, 1, 9, 10, 11]].any()
         assert np.array_equal(g[2:9], alone[4])
+
+
+def test_nan_advantages(oracle):
+    """Loss and gradient are NaN whichever side of the clipping the ratio is on."""
+    x = _inputs(7, 3, 9)
+    lp = oracle.token_logprob(x["z"], x["t"])
+    for kc in (0.0, 0.1):
+        loss, _, _, d, g = oracle.policy_loss(x["z"], x["t"], np.full(3, np.nan),
+                                              lp + np.array([1.0, 0.0, -1.0]), x["ref"],
+                                              np.ones(3), kl_coef=kc)
+        assert np.isnan(loss).all() and np.isnan(d).all() and np.isnan(g).all()
