@@ -383,7 +383,7 @@ policy_kernel(const T* logits, T* grad, PolicyArgs a) {
         if (a.ref) {
             const float y = (float)((double)ref - lp);
             const float em = expm1f(y);
-            kl = em - y;
+            kl = em == INFINITY ? INFINITY : em - y;  // also where y is infinite
             if (a.kl_coef != 0.f) {
                 l += a.kl_coef * kl;
                 d -= a.kl_coef * em;

@@ -615,10 +615,12 @@ int token_logprob_forward_hip(const void* logits, const int32_t* targets, const 
  * and d sum(loss) / d logits from one read of the logits (two where a row is more than
  * a workgroup's registers hold).  old_logp NULL: the policy itself (r = 1, with
  * the gradient of r).  At a border of the clipping the gradient is the unclipped
- * side's.  An advantage or old_logp that is NaN gives a loss and a gradient that are.  weights NULL: 1 / rows each, so that sum(loss) is the mean.  loss, logp and
- * kl (may be NULL; else it needs ref_logp) are fp32 (rows).  clip_low outside
- * [0, 1], clip_high or kl_coef negative, NaN, or kl_coef infinite or without
- * ref_logp -> 1. */
+ * side's.  An advantage or old_logp that is NaN gives a loss and a gradient that are.
+ * A target that cannot occur (logit -inf) where ref_logp is finite has kl +inf, and with
+ * kl_coef a loss of +inf and a gradient that is not finite.  weights NULL: 1 / rows
+ * each, so that sum(loss) is the mean.  loss, logp and kl (may be NULL; else it needs
+ * ref_logp) are fp32 (rows).  clip_low outside [0, 1], clip_high or kl_coef negative,
+ * NaN, or kl_coef infinite or without ref_logp -> 1. */
 int policy_loss_forward_backward_hip(const void* logits, const int32_t* targets,
                                      const float* advantages, const float* old_logp,
                                      const float* ref_logp, const float* weights, float* loss,

@@ -651,7 +651,8 @@ def _row_gradient(p, targets, on, tok, dlogp):
     """dlogp_i ([j = t_i] - softmax_ij); zero rows without weight or target."""
     rows = np.flatnonzero(on & tok)
     g = np.zeros_like(p)
-    g[rows] = -dlogp[rows, None] * p[rows]
+    with np.errstate(invalid="ignore"):
+        g[rows] = -dlogp[rows, None] * p[rows]
     g[rows, np.asarray(targets).astype(np.int64)[rows]] += dlogp[rows]
     return g
 
@@ -673,7 +674,7 @@ def policy_loss(logits, targets, advantages, old_logp=None, ref_logp=None, weigh
         kl = np.zeros(N)
         if ref_logp is not None:
             x = np.asarray(ref_logp, np.float64) - logp
-            kl = np.expm1(x) - x
+            kl = np.where(x == np.inf, np.inf, np.expm1(x) - x)
             if kl_coef != 0:
                 loss, d = loss + kl_coef * kl, d - kl_coef * np.expm1(x)
         loss, d = w * loss, w * d

@@ -1,11 +1,11 @@
 """Rows at the edges of the losses on rewards and preferences: rows outside of every
-sequence, and beside a NaN, advantages that are NaN."""
+sequence, and beside a NaN, advantages that are NaN, tokens that cannot occur."""
 import numpy as np
 import pytest
 import torch
 
 from helpers import announce
-from test_losses_gpu import POLICY, make
+from test_losses_gpu import POLICY, U, make
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +121,44 @@ def test_nan_advantages_reach_loss_and_gradient(oracle, V, kl_coef):
     assert bool(logp.isfinite().all()) and bool(kl.isfinite().all())
     if kl_coef == 0:
         assert not grad[1].any() and bool(grad[3].any()) and not grad[5].any()
+
+
+@pytest.mark.parametrize("V", [70, 5000, 140000])
+def test_kl_of_tokens_that_cannot_occur(oracle, V):
+    """A target at -inf that the reference model gives a chance: the KL estimate e^x - 1 - x
+    is +inf, and so is a loss that it enters; without its factor the loss is the policy's own."""
+    announce(f"KL of impossible tokens V={V}")
+    from ceo_amd import nn
+
+    N = 6
+    x, d, _ = make(V + 4, N, V, torch.float32, masked=0.0)
+    x["w"][:] = 0.5
+    x["adv"][:] = [1.0, -1.0, 0.5, 2.0, -2.0, 1.0]
+    bad = [0, 1, 4]
+    x["z"][bad, x["t"][bad]] = -np.inf
+    x["ref"][4] = np.float32(3e38)  # the largest there is, still finite
+    x["ref"][5] = np.float32(-3e38)  # and its opposite: kl is large, not infinite
+    d["z"].copy_(torch.from_numpy(x["z"]))
+    for k in ("w", "adv", "ref"):
+        d[k].copy_(torch.from_numpy(x[k]))
+    for kl_coef in (0.0, 0.05):
+        a = {**POLICY, "kl_coef": kl_coef}
+        rl, rlp, rkl, _, rg = oracle.policy_loss(x["z"], x["t"], x["adv"], x["old"], x["ref"],
+                                                 x["w"], **a)
+        assert (rlp[bad] == -np.inf).all() and (rkl[bad] == np.inf).all()
+        for need in (True, False):
+            loss, logp, kl, grad = nn.policy_loss_forward_backward(
+                d["z"], d["t"], d["adv"], d["old"], d["ref"], d["w"], need_grad=need, **a)
+            assert bool((logp[bad] == -np.inf).all()) and bool((kl[bad] == np.inf).all())
+            assert bool(kl[[2, 3, 5]].isfinite().all())
+            loss = loss.cpu().numpy()
+            if kl_coef:
+                assert (rl[bad] == np.inf).all() and (loss[bad] == np.inf).all()
+                assert np.isfinite(loss[[2, 3, 5]]).all()
+            else:
+                # r = 0: nothing to gain, and (1 - clip_low) |A| where A is negative; each
+                # within the roundings of the border and of two products
+                assert np.isfinite(rl[bad]).all()
+                assert (np.abs(loss[bad] - rl[bad]) <= 4 * U * np.abs(rl[bad])).all()
+                if need:
+                    assert not rg[bad].any() and not grad[bad].any()

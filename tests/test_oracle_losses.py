@@ -150,3 +150,15 @@ def test_nan_advantages(oracle):
                                               lp + np.array([1.0, 0.0, -1.0]), x["ref"],
                                               np.ones(3), kl_coef=kc)
         assert np.isnan(loss).all() and np.isnan(d).all() and np.isnan(g).all()
+
+
+def test_kl_of_tokens_that_cannot_occur(oracle):
+    """e^x - 1 - x for x = +inf is +inf, and for x = -inf too."""
+    z = np.array([[0.0, -np.inf, 1.0], [0.0, 2.0, 1.0]])
+    t = np.array([1, 0], np.int32)
+    ref = np.array([-2.0, -np.inf])
+    for kc in (0.0, 0.1):
+        loss, lp, kl, _, _ = oracle.policy_loss(z, t, np.ones(2), np.full(2, -2.0), ref, np.ones(2),
+                                                kl_coef=kc)
+        assert lp[0] == -np.inf and (kl == np.inf).all()
+        assert (loss == np.inf).all() if kc else np.isfinite(loss).all()
