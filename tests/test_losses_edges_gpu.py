@@ -1,5 +1,6 @@
 """Rows at the edges of the losses on rewards and preferences: rows outside of every
-sequence, and beside a NaN, advantages that are NaN, tokens that cannot occur."""
+sequence, and beside a NaN, advantages that are NaN, tokens that cannot occur, policies
+that are nearly the reference."""
 import numpy as np
 import pytest
 import torch
@@ -162,3 +163,36 @@ def test_kl_of_tokens_that_cannot_occur(oracle, V):
                 assert (np.abs(loss[bad] - rl[bad]) <= 4 * U * np.abs(rl[bad])).all()
                 if need:
                     assert not rg[bad].any() and not grad[bad].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("V", [1, 70, 5000, 140000])
+def test_kl_of_a_policy_near_its_reference(V, dtype):
+    """Only the target's logit is finite, so that logp is 0 and x = ref - logp the given
+    reference's: e^x - 1 - x, about x^2 / 2, has to keep its digits.
+
+    Tolerance: below 1/2 a sum of terms x^2 x^k / (k + 2)!, each at most a third of the one
+    before: roundings of x^2, the product and the last additions, under 8 in all; above it
+    e^x - 1, within two roundings of at most 4.4 times the result, and the difference's, under 10."""
+    announce(f"KL near the reference V={V} {dtype}")
+    from ceo_amd import nn
+
+    mags = [1e-12, 1e-9, 1e-7, 3e-7, 1e-6, 1e-5, 1e-4, 1e-3, 1e-2, 0.1, 0.3, 0.499, 0.501, 0.7, 1.0,
+            3.0, 10.0]
+    y = np.array([s * m for m in mags for s in (1, -1)] + [0.0, -40.0], dtype=np.float32)
+    N = len(y)
+    t = torch.from_numpy((np.arange(N) * 7919 % V).astype(np.int32)).cuda()
+    z = torch.full((N, V), float("-inf"), dtype=dtype, device="cuda")
+    z[torch.arange(N, device="cuda"), t.long()] = 0.5
+    x = y.astype(np.float64)
+    # the series to x^11 / 11!, 1e-13 of the sum at 0.3, and the formula beyond
+    series, term = np.zeros(N), x * x / 2
+    for k in range(3, 13):
+        series, term = series + term, term * x / k
+    want = np.where(np.abs(x) < 0.3, series, np.expm1(x) - x)
+    _, logp, kl, _ = nn.policy_loss_forward_backward(
+        z, t, torch.ones(N, device="cuda"), ref_logp=torch.from_numpy(y).cuda())
+    assert not logp.any()
+    off = np.abs(kl.double().cpu().numpy() - want)
+    print(f"  worst {np.max(off[x != 0] / want[x != 0]) / U:.2f} roundings", flush=True)
+    assert (off <= 16 * U * want).all()
