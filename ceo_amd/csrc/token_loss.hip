@@ -1086,6 +1086,8 @@ extern "C" int preference_loss_forward_backward_hip(
             tl::check(logits, targets, grad_logits, rows, vocab_size, ld, ld_grad, dtype);
         if (rc != kSuccess) return rc;
         if (!logp) return kInvalidValue;
+    } else if (tl::dtype_size(dtype) == 0) {
+        return kInvalidValue;
     }
     if (!(beta > 0.f && beta < INFINITY) || !(label_smoothing >= 0.f && label_smoothing < 1.f))
         return kInvalidValue;

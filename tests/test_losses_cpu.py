@@ -90,6 +90,11 @@ def test_preference_refusals(L):
     assert L.preference_loss_workspace_size(BIG) == 0
 
 
+def test_preference_without_rows_refuses_an_unknown_type(L):
+    for dt in (1, 3, 99, -1):
+        assert _preference(L, z=NULL, t=NULL, lp=NULL, g=NULL, rows=0, dt=dt) == 1
+
+
 def test_grad_list_refusals(L):
     h = ctypes.c_void_p()
     ptrs = (ctypes.c_void_p * 2)(64, 128)
