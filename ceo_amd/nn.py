@@ -592,6 +592,9 @@ class GradList:
         check(rc, "grad_list_create_hip")
         self._handle = handle
 
+    def __reduce__(self):  # a copy has a table of its own
+        return type(self), (self.grads, self.outs)
+
     def __del__(self):
         if getattr(self, "_handle", None) and lib is not None:  # None: the program's end
             lib().grad_list_destroy_hip(self._handle)

@@ -1,6 +1,8 @@
 """Refusals of the policy and preference losses and of gradient lists, without a
 GPU: they come before any HIP call, with the library's codes (0 success, 1 invalid
 value, 9 invalid configuration)."""
+import contextlib
+import copy
 import ctypes
 
 import pytest
@@ -115,6 +117,39 @@ def test_grad_list_refusals(L):
     assert L.grad_list_destroy_hip(NULL) == 0
     assert L.grad_norm_hip(NULL, 1.0, P, P, NULL) == 1
     assert L.grad_clip_hip(NULL, 1.0, P, NULL) == 1
+
+
+def test_copies_of_a_grad_list_have_their_own_table(monkeypatch):
+    """A copy (of a model that keeps a list, say) makes and frees a table of its own; a deep
+    copy holds the copied gradients.  The library is a stand-in that counts."""
+    made, freed = [], []
+
+    class Counts:
+        def grad_list_create_hip(self, handle, ptrs, *rest):
+            made.append(64 * (len(made) + 1))
+            handle._obj.value = made[-1]
+            return 0
+
+        def grad_list_destroy_hip(self, handle):
+            freed.append(handle.value)
+            return 0
+
+    counts = Counts()
+    monkeypatch.setattr(nn, "lib", lambda: counts)
+    monkeypatch.setattr(nn, "_require", lambda *a, **k: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    flat = torch.ones(6)
+    lists = [nn.GradList([flat], [flat])]
+    try:
+        lists.append(copy.copy(lists[0]))
+        assert lists[1].grads[0] is flat and lists[1].outs[0] is flat
+        deep = copy.deepcopy({"flat": flat, "list": lists[0]})
+        lists.append(deep["list"])
+        assert deep["list"].grads[0] is deep["flat"] is deep["list"].outs[0] is not flat
+    finally:
+        for gl in lists:
+            gl.__del__()
+    assert len(made) == 3 and sorted(freed) == made
 
 
 def test_adamw_scaled_refusals(L):

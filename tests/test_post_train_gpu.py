@@ -108,3 +108,20 @@ def test_steps_train():
     m = post_train.train_preference(_model(4, scale=1.0), steps=15)
     print("  margins", [f"{x:.2f}" for x in m], flush=True)
     assert abs(m[0]) <= 1e-2 and m[-1] >= 0.5
+
+
+def test_a_copy_of_a_model_clips_its_own_gradients():
+    """copy.deepcopy between two clipped updates: the copy's norm is of its own gradients."""
+    import copy
+
+    announce("post-training: a model's copy")
+    model = _model(3)
+    model.grads.zero_()
+    model.grads[:1024] = 1.0 / 32  # norm 1
+    assert abs(model.update(max_norm=0.5).item() - 1.0) <= 2.0 ** -23
+    other = copy.deepcopy(model)
+    assert torch.equal(other.master, model.master) and other.grads is not model.grads
+    other.grads.mul_(2.0)
+    assert abs(other.update(max_norm=0.5).item() - 2.0) <= 2.0 ** -22
+    del model
+    assert abs(other.update(max_norm=0.5).item() - 2.0) <= 2.0 ** -22
