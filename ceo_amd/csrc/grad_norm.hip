@@ -342,7 +342,8 @@ extern "C" int grad_clip_hip(const void* list, float max_norm, float* norm, hipS
     const dim3 grid(parts ? (parts + 7) / 8 * 8 : 1), block(gn::NT);
     // Where gradients and outputs are over half of the 256 MB cache, this pass leaves the cache
     // to the gradients that the norm has read: it reads and writes past it (368 million in
-    // bf16 351 us, 412 through it; 23 million 43.6 and 53.6).
+    // bf16 351 us, 412 through it; 23 million 43.6 and 53.6).  In place they are counted twice
+    // too; lists of 64 to 128 MiB clipped in place have not been measured.
     if (2 * l->bytes > (size_t)128 << 20)
         EFLA_LAUNCH("grad_clip", (gn::clip_kernel<true>), grid, block, stream, l->entries, l->map,
                     (uint32_t)l->units, l->part, (int)parts, max_norm, norm);

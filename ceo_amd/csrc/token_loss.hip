@@ -27,7 +27,7 @@
 // in bf16 take 342 to 360 us, 5.8 to 6.1 TB/s (a large copy: 5.15).  A row of over 128 KiB
 // leaves no room for a second one on its compute unit, so its loads wait for its
 // stores (2048 x 128003 in fp16 192 to 209 us, 4.5 to 4.9 TB/s).  A few rows are bound by
-// their own latency, 8 us for 64 x 32000, and the host's 13.
+// their own latency, 8 us for 64 x 32000, and the host's 12 to 13.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -957,7 +957,8 @@ static dim3 row_grid(size_t rows) {
 // 8191 x 32000, whose second read the cache serves, 202 and 249), and what is read for the
 // last time read past it (log-probabilities of 16384 x 32000 98 us against 105, of 4096 x
 // 50257 in fp32 120 against 130; preference losses 1 to 4 %); else what comes next finds
-// them there.
+// them there.  The gradient is counted beside the logits also where it overwrites them or
+// there is none; between 128 and 256 MiB of logits those calls have not been measured.
 static bool past_cache(size_t rows, size_t vocab, int dtype) {
     return 2 * rows * vocab * dtype_size(dtype) > ((size_t)256 << 20);
 }
@@ -978,7 +979,10 @@ static int logprob(const void* logits, const int32_t* targets, const float* weig
 }
 
 // Logits that the cache does not hold, in rows whose work hides the drawing: their
-// preference loss streams them.
+// preference loss streams them.  420 MB in 16 pairs, us drawn and in three launches: rows of
+// 55 KiB (28000 in bf16) 232 and 201, 78 KiB 209 and 203, 94 KiB 199 and 205, 98 KiB 198 and
+// 206, 125 KiB 190 and 205; in fp32, of half as many logits, 62 KiB 195 and 198, 94 KiB 188
+// and 203, 109 KiB 185 and 205.
 static bool streams(size_t rows, size_t vocab, int dtype) {
     const size_t row = vocab * dtype_size(dtype);
     return row >= (size_t)96 << 10 && rows * row > (size_t)256 << 20;

@@ -295,7 +295,9 @@ class EflaLM:
     def update(self, max_norm=None):
         """One AdamW step over every parameter (fp32 master, bf16 copy refreshed).  With
         ``max_norm`` on the gradients clipped to that norm (the factor goes to the step,
-        nothing is written for it); returns their norm before, a device value."""
+        nothing is written for it); returns their norm before, a device value.  The norm
+        needs every gradient, so ``train_step``, which updates group by group beside the
+        backward, takes none: a clipped step is forward, backward, update(max_norm)."""
         cfg = self.cfg
         norm = coef = None
         if max_norm is not None:
