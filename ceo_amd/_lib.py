@@ -134,6 +134,17 @@ _SIGS = {
     "preference_loss_workspace_size": (sz, [sz]),
     "preference_loss_forward_backward_hip": (i32, [vp] * 9 + [sz] * 5 + [f32] * 2 +
                                              [i32, vp, sz, vp]),
+    # generating text
+    "beam_select_workspace_size": (sz, [sz, sz, sz, sz]),
+    "beam_select_hip": (i32, [vp] * 7 + [sz] * 5 + [i32, i32, i32, vp, sz, vp]),
+    "state_list_create_hip": (i32, [ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(vp),
+                                    ctypes.POINTER(sz), sz, sz, sz]),
+    "state_list_destroy_hip": (i32, [vp]),
+    "state_reorder_hip": (i32, [vp, vp, vp]),
+    "int8_weight_size": (sz, [sz, sz]),
+    "int8_weight_pack_hip": (i32, [vp, sz, vp, sz, sz, i32, vp]),
+    "linear_int8_workspace_size": (sz, [sz, sz]),
+    "linear_int8_hip": (i32, [vp, sz, vp, vp, vp, sz, vp, sz, sz, sz, sz, i32, i32, vp, sz, vp]),
     # sequence packing (host)
     "efla_pack_sequences": (i32, [vp, vp, sz, sz, vp, vp, vp, vp, ctypes.POINTER(sz),
                                   ctypes.POINTER(sz)]),

@@ -1,0 +1,479 @@
+// Beam search's selection for gfx950: of all continuations of a text's beams, the best.
+//
+//   value(k, v) = score_k + z_kv - log sum_v exp z_kv      (beam k, token v, logits z)
+//
+// and of a text's beams * vocabulary values the `select` largest, ties to the lowest
+// k * vocabulary + v.  A finished beam offers the end token at its own score and nothing
+// else.  A beam whose score is not finite, or whose logits have no finite sum of
+// exponentials (a NaN, +inf, -inf everywhere), offers nothing: its values are -inf.
+//
+// The logits are read once and nothing of their size is written.  Two launches:
+//
+// slice_kernel: a workgroup takes a slice of one row, 1 to 4 16-byte vectors a thread, in
+// registers.  Maximum and sum of exponentials are each thread's own first (no barrier
+// stands between load and exponentials), then joined.  For the best n of the slice each
+// wave finds the n-th largest of its 64 lanes' maxima, bit by bit with one ballot a
+// bit: n logits of the slice are no less, so that is a bound, and the largest of the waves'
+// bounds leaves a few tens of a slice's thousands.  Those go to LDS and are ranked by
+// counting how many are better (value, then token: no two are equal, so the order in
+// which they arrive does not matter).  Where more pass the bound than LDS has places
+// (many equal logits) the best are taken out one by one.
+//
+// join_kernel: a workgroup per text joins the slices' sums (64 bits), and does the same
+// with the slices' best, whose values it forms in 64 bits.  -inf is never a candidate:
+// where fewer than `select` finite values exist, the rest are the lowest pairs (k, v)
+// that are not among them, which is what the order above gives.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include "../../include/efla_hip.h"
+#include "common.hpp"
+#include "internal.hpp"
+
+namespace efla {
+namespace bs {
+
+constexpr int NT = 256, NWV = NT / kWave;
+constexpr int kMaxSelect = 64, kMaxBeams = 64;
+constexpr int kPlaces = 1024;  // candidates that LDS holds
+
+// What is left of a slice: one of its best logits; none: token -1.
+struct Cand {
+    float z;
+    int token;
+};
+
+// Whole numbers in the order of the floats that they stand for.
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t b = __float_as_uint(f);
+    return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ uint64_t ordered(double f) {
+    const uint64_t b = (uint64_t)__double_as_longlong(f);
+    return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+// A bound that at least n of the wave's 64 keys reach: their n-th largest with its bits
+// below LOW cleared.  n <= 64.
+template <int LOW>
+__device__ __forceinline__ uint32_t wave_bound(uint32_t key, int n) {
+    uint32_t got = 0;
+#pragma unroll
+    for (int b = 31; b >= LOW; --b) {
+        const uint32_t t = got | (1u << b);
+        if (__popcll(__ballot(key >= t)) >= n) got = t;
+    }
+    return got;
+}
+
+__device__ __forceinline__ float exp_diff(float d) {  // e^d
+    return __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+}
+
+// A row's vectors start at cache lines: element i of the row is at i + shift, shift its
+// first element's place in its line, and slice s holds [s L, (s + 1) L) of that.
+template <typename T, int VPT>
+__global__ void __launch_bounds__(NT)
+slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
+             const float* __restrict__ scores, const uint8_t* __restrict__ finished,
+             float2* __restrict__ stats, Cand* __restrict__ cands) {
+    constexpr int N = 16 / sizeof(T), L = NT * VPT * N;
+    typedef __attribute__((__vector_size__(16))) T Vec;
+    __shared__ uint64_t place[kPlaces];
+    __shared__ float wm[NWV], ws[NWV];
+    __shared__ uint32_t wb[NWV];
+    __shared__ uint64_t best[NWV];
+    __shared__ int count;
+    const long row = blockIdx.y;
+    // a beam that offers no continuation is not read
+    if ((finished && finished[row]) || !(fabsf(scores[row]) < INFINITY)) return;
+    const T* p = logits + row * ld;
+    const int shift = (int)((uintptr_t)p % 128 / sizeof(T));
+    const long v0 = (long)blockIdx.x * L - shift;  // the slice's first token
+    if (threadIdx.x == 0) count = 0;
+
+    Vec x[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const long v = v0 + (long)(threadIdx.x + i * NT) * N;
+        if (v >= 0 && v + N <= V) {
+            x[i] = *reinterpret_cast<const Vec*>(p + v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                x[i][j] = v + j >= 0 && v + j < V ? p[v + j] : (T)-INFINITY;
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = fmaxf(m, to_f(x[i][j]));
+    m += 0.f;  // -0 is 0
+    // a thread without a logit above -inf: 0, or NaN from a NaN
+    const float m0 = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) s += exp_diff(to_f(x[i][j]) - m0);
+    const uint32_t bound = wave_bound<sizeof(T) == 2 && !__is_same(T, f16) ? 16 : 12>(ordered(m), n);
+    float M = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    const float M0 = M == -INFINITY ? 0.f : M;
+    s *= exp_diff(m0 - M0 < 0.f ? m0 - M0 : 0.f);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (lane_id() == 0) {
+        wm[wave_id()] = M;
+        ws[wave_id()] = s;
+        wb[wave_id()] = bound;
+    }
+    __syncthreads();
+    uint32_t least = wb[0];
+#pragma unroll
+    for (int k = 1; k < NWV; ++k) least = max(least, wb[k]);
+    const long slot = row * gridDim.x + blockIdx.x;
+    if (threadIdx.x == 0) {
+        float W = wm[0];
+#pragma unroll
+        for (int k = 1; k < NWV; ++k) W = fmaxf(W, wm[k]);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < NWV; ++k)
+            sum += wm[k] == -INFINITY ? ws[k] : ws[k] * exp_diff(wm[k] - W);
+        stats[slot] = make_float2(W, sum);
+    }
+    // key: the logit, then the lower token
+    auto key_of = [&](int i, int j) {
+        const float z = to_f(x[i][j]) + 0.f;
+        const uint32_t v = (uint32_t)(v0 + (long)(threadIdx.x + i * NT) * N + j);
+        return z > -INFINITY ? (uint64_t)ordered(z) << 32 | (uint32_t)~v : 0ull;
+    };
+    if (m > -INFINITY && ordered(m) >= least) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint64_t key = key_of(i, j);
+                if (key == 0 || (uint32_t)(key >> 32) < least) continue;
+                const int at = atomicAdd(&count, 1);
+                if (at < kPlaces) place[at] = key;
+            }
+    }
+    __syncthreads();
+    const int c = count;
+    Cand* out = cands + slot * n;
+    auto write = [&](int rank, uint64_t key) {
+        out[rank] = Cand{unordered((uint32_t)(key >> 32)), (int)~(uint32_t)key};
+    };
+    if (c <= kPlaces) {
+        for (int i = threadIdx.x; i < c; i += NT) {
+            const uint64_t mine = place[i];
+            int rank = 0;
+            for (int k = 0; k < c; ++k) rank += place[k] > mine;
+            if (rank < n) write(rank, mine);
+        }
+        for (int i = c + threadIdx.x; i < n; i += NT) out[i] = Cand{0.f, -1};
+        return;
+    }
+    // too many: the best, then the best below it, n times (c > n: there are as many)
+    uint64_t last = ~0ull;
+    for (int r = 0; r < n; ++r) {
+        uint64_t top = 0;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint64_t key = key_of(i, j);
+                if (key < last && key > top) top = key;
+            }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t other = __shfl_xor(top, o);
+            if (other > top) top = other;
+        }
+        __syncthreads();  // `best` has been read
+        if (lane_id() == 0) best[wave_id()] = top;
+        __syncthreads();
+        last = best[0];
+#pragma unroll
+        for (int k = 1; k < NWV; ++k)
+            if (best[k] > last) last = best[k];
+        if (threadIdx.x == 0) write(r, last);
+    }
+}
+
+// A candidate of the join: its value and its place in the order of ties.
+struct Best {
+    double value;
+    int beam, token;
+};
+__device__ __forceinline__ bool better(const Best& a, const Best& b) {
+    if (a.value != b.value) return a.value > b.value;
+    if (a.beam != b.beam) return a.beam < b.beam;
+    return a.token < b.token;
+}
+
+__global__ void __launch_bounds__(NT)
+join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, int slices,
+            const float* __restrict__ scores, const uint8_t* __restrict__ finished, int V,
+            int beams, int n, int end_token, int keep_slots, float* __restrict__ out_scores,
+            int* __restrict__ out_parents, int* __restrict__ out_tokens,
+            uint8_t* __restrict__ out_finished) {
+    __shared__ double offset[kMaxBeams];  // score - log sum exp; -inf: offers nothing
+    __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
+    __shared__ Best place[kPlaces];
+    __shared__ Best res[kMaxSelect];
+    __shared__ Best wbest[NWV];
+    __shared__ uint32_t wb[NWV];
+    __shared__ int count;
+    const long text = blockIdx.x, row0 = text * beams;
+    if (threadIdx.x == 0) count = 0;
+    for (int k = wave_id(); k < beams; k += NWV) {
+        const float score = scores[row0 + k];
+        const bool fin = finished && finished[row0 + k], ok = fabsf(score) < INFINITY;
+        double lse = 0.0;
+        if (ok && !fin) {
+            const float2* st = stats + (row0 + k) * slices;
+            float M = -INFINITY;
+            for (int i = lane_id(); i < slices; i += kWave) M = fmaxf(M, st[i].x);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+            double s = 0.0;
+            for (int i = lane_id(); i < slices; i += kWave) {
+                const float2 a = st[i];
+                // a slice without a logit above -inf: 0, or NaN from a NaN
+                s += a.x == -INFINITY ? (double)a.y : (double)a.y * exp((double)a.x - (double)M);
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+            lse = (double)M + log(s);
+        }
+        if (lane_id() == 0) {
+            const bool live = ok && fabs(lse) < (double)INFINITY;
+            state[k] = !live ? 2 : fin ? 1 : 0;
+            offset[k] = live ? (double)score - lse : -(double)INFINITY;
+        }
+    }
+    __syncthreads();
+    const int per = slices * n, total = beams * per;
+    // entry e, or a value of -inf; a finished beam has one
+    auto entry = [&](int e) {
+        const int k = e / per, i = e - k * per;
+        Best b{-(double)INFINITY, k, 0};
+        if (state[k] == 0) {
+            const Cand c = cands[(row0 + k) * per + i];
+            if (c.token >= 0) b = Best{(double)c.z + offset[k], k, c.token};
+        } else if (state[k] == 1 && i == 0) {
+            b = Best{offset[k], k, end_token};
+        }
+        return b;
+    };
+    uint64_t top = 0;
+    for (int e = threadIdx.x; e < total; e += NT) {
+        const Best b = entry(e);
+        if (b.value > -(double)INFINITY) {
+            const uint64_t o = ordered(b.value + 0.0);
+            if (o > top) top = o;
+        }
+    }
+    const uint32_t bound = wave_bound<4>((uint32_t)(top >> 32), n);
+    if (lane_id() == 0) wb[wave_id()] = bound;
+    __syncthreads();
+    uint32_t least = wb[0];
+#pragma unroll
+    for (int k = 1; k < NWV; ++k) least = max(least, wb[k]);
+    for (int e = threadIdx.x; e < total; e += NT) {
+        const Best b = entry(e);
+        if (!(b.value > -(double)INFINITY) || (uint32_t)(ordered(b.value + 0.0) >> 32) < least)
+            continue;
+        const int at = atomicAdd(&count, 1);
+        if (at < kPlaces) place[at] = b;
+    }
+    __syncthreads();
+    const int c = count;
+    if (c <= kPlaces) {
+        for (int i = threadIdx.x; i < c; i += NT) {
+            const Best mine = place[i];
+            int rank = 0;
+            for (int k = 0; k < c; ++k) rank += better(place[k], mine);
+            if (rank < n) res[rank] = mine;
+        }
+    } else {
+        // too many (equal values): the best, then the best behind it, n times
+        Best last{(double)INFINITY, -1, -1};
+        for (int r = 0; r < n; ++r) {
+            Best mine{-(double)INFINITY, beams, 0};
+            for (int e = threadIdx.x; e < total; e += NT) {
+                const Best b = entry(e);
+                if (b.value > -(double)INFINITY && better(last, b) && better(b, mine)) mine = b;
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                const Best other{__shfl_xor(mine.value, o), __shfl_xor(mine.beam, o),
+                                 __shfl_xor(mine.token, o)};
+                if (better(other, mine)) mine = other;
+            }
+            __syncthreads();  // `wbest` has been read
+            if (lane_id() == 0) wbest[wave_id()] = mine;
+            __syncthreads();
+            last = wbest[0];
+#pragma unroll
+            for (int k = 1; k < NWV; ++k)
+                if (better(wbest[k], last)) last = wbest[k];
+            if (threadIdx.x == 0) res[r] = last;
+        }
+    }
+    __syncthreads();
+    // fewer finite values than asked for: the lowest pairs that are not among them
+    if (threadIdx.x == 0 && c < n) {
+        int beam = 0, token = 0;
+        for (int r = c; r < n;) {
+            bool taken = false;
+            for (int k = 0; k < c; ++k) taken |= res[k].beam == beam && res[k].token == token;
+            if (!taken) res[r++] = Best{-(double)INFINITY, beam, token};
+            if (++token == V) token = 0, ++beam;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= n) return;
+    const int r = threadIdx.x;
+    const Best b = res[r];
+    int to = r;
+    if (keep_slots) {
+        // the first child of a beam takes that beam's slot, the others the free ones in order
+        uint64_t used = 0;
+        int rest = 0;
+        bool first = true;
+        for (int k = 0; k < n; ++k) {
+            const uint64_t bit = 1ull << res[k].beam;
+            if (k < r && (used & bit)) ++rest;
+            if (k == r) first = !(used & bit);
+            used |= bit;
+        }
+        to = b.beam;
+        if (!first) {
+            uint64_t open = ~used;
+            for (int k = 0; k < rest; ++k) open &= open - 1;
+            to = __ffsll((unsigned long long)open) - 1;
+        }
+    }
+    const long at = text * n + to;
+    out_scores[at] = (float)b.value;
+    out_parents[at] = b.beam;
+    out_tokens[at] = b.token;
+    if (out_finished)
+        out_finished[at] = (finished && finished[row0 + b.beam]) || b.token == end_token;
+}
+
+static size_t dtype_size(int d) {
+    return d == kDtypeF32 ? 4 : d == kDtypeF16 || d == kDtypeBF16 ? 2 : 0;
+}
+
+// Vectors a thread: as many as leave the chip four workgroups for each of its compute units.
+static int vectors(size_t rows, size_t vocab, size_t size) {
+    const size_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    for (int v = 4; v > 1; v /= 2)
+        if (rows * ((vocab * size + NT * 16 * v - 1) / (NT * 16 * v)) >= 4 * cus) return v;
+    return 1;
+}
+// Slices of a row of whatever alignment.
+static size_t slices_of(size_t vocab, size_t size, int vpt, bool lines) {
+    const size_t l = (size_t)NT * vpt * 16 / size, shift = lines ? 0 : 128 / size - 1;
+    return (vocab + shift + l - 1) / l;
+}
+
+static size_t scratch(size_t batch, size_t beams, size_t vocab, size_t n) {
+    // whatever the type and the alignment: 4-byte logits, one vector a thread
+    const size_t slices = slices_of(vocab, 4, 1, false);
+    return batch * beams * slices * (sizeof(float2) + n * sizeof(Cand));
+}
+
+template <typename T>
+static void launch(const void* logits, const float* scores, const uint8_t* finished,
+                   const uint8_t* ws, size_t rows, size_t beams, size_t vocab, size_t ld, size_t n,
+                   int vpt, size_t slices, hipStream_t st) {
+    float2* stats = (float2*)ws;
+    Cand* cands = (Cand*)(stats + rows * slices);
+    const T* z = (const T*)logits;
+    for (size_t r0 = 0; r0 < rows; r0 += 32768) {
+        const dim3 grid((unsigned)slices, (unsigned)(rows - r0 < 32768 ? rows - r0 : 32768));
+        const size_t s0 = r0 * slices;
+#define BS_SLICE(VPT)                                                                          \
+    EFLA_LAUNCH("beam_slice", (slice_kernel<T, VPT>), grid, dim3(NT), st, z + r0 * ld, (long)ld, \
+                (int)vocab, (int)beams, (int)n, scores + r0, finished ? finished + r0 : nullptr, \
+                stats + s0, cands + s0 * n)
+        if (vpt == 1) BS_SLICE(1);
+        else if (vpt == 2) BS_SLICE(2);
+        else BS_SLICE(4);
+#undef BS_SLICE
+    }
+}
+
+}  // namespace bs
+}  // namespace efla
+
+using namespace efla;
+
+extern "C" size_t beam_select_workspace_size(size_t batch, size_t beams, size_t vocab_size,
+                                             size_t select) {
+    if (beams > bs::kMaxBeams || select > bs::kMaxSelect || vocab_size > 0x3FFFFFFFull ||
+        batch > (1ull << 31) / (beams ? beams : 1))
+        return 0;
+    return bs::scratch(batch, beams, vocab_size, select);
+}
+
+extern "C" int beam_select_hip(const void* logits, const float* scores, const uint8_t* finished,
+                               float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                               uint8_t* out_finished, size_t batch, size_t beams,
+                               size_t vocab_size, size_t ld, size_t select, int32_t end_token,
+                               int keep_slots, int dtype, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream) {
+    const size_t size = bs::dtype_size(dtype);
+    if (size == 0 || beams == 0 || beams > bs::kMaxBeams || select == 0 ||
+        select > bs::kMaxSelect || vocab_size == 0 || ld < vocab_size)
+        return kInvalidValue;
+    if ((keep_slots && select != beams) || beams * vocab_size < select) return kInvalidValue;
+    if ((finished || out_finished) && (end_token < 0 || (size_t)end_token >= vocab_size))
+        return kInvalidValue;
+    if (batch == 0) return kSuccess;
+    if (!logits || !scores || !out_scores || !out_parents || !out_tokens) return kInvalidValue;
+    if ((uintptr_t)logits % size) return kInvalidValue;
+    size_t rows, elems;
+    if (vocab_size > 0x3FFFFFFFull || !mul_ok(batch, beams, &rows) || rows > 0x7FFFFFFFull ||
+        !mul_ok(rows, ld, size, &elems) || elems > (1ull << 62))
+        return kInvalidConfiguration;
+    const size_t need = bs::scratch(batch, beams, vocab_size, select);
+    void* ws = workspace;
+    WsLease lease;
+    if (!ws) {
+        const int rc = workspace_acquire(need, stream, &ws, lease);
+        if (rc != kSuccess) return rc;
+    } else if (workspace_bytes < need || (uintptr_t)ws % 8) {
+        return kInvalidValue;
+    }
+    const int vpt = bs::vectors(rows, vocab_size, size);
+    const bool lines = (uintptr_t)logits % 128 == 0 && ld * size % 128 == 0;
+    const size_t slices = bs::slices_of(vocab_size, size, vpt, lines);
+    if (dtype == kDtypeBF16)
+        bs::launch<bf16>(logits, scores, finished, (const uint8_t*)ws, rows, beams, vocab_size, ld,
+                         select, vpt, slices, stream);
+    else if (dtype == kDtypeF16)
+        bs::launch<f16>(logits, scores, finished, (const uint8_t*)ws, rows, beams, vocab_size, ld,
+                        select, vpt, slices, stream);
+    else
+        bs::launch<float>(logits, scores, finished, (const uint8_t*)ws, rows, beams, vocab_size, ld,
+                          select, vpt, slices, stream);
+    EFLA_CHECK(hipPeekAtLastError());
+    const float2* stats = (const float2*)ws;
+    EFLA_LAUNCH("beam_join", bs::join_kernel, dim3((unsigned)batch), dim3(bs::NT), stream, stats,
+                (const bs::Cand*)(stats + rows * slices), (int)slices, scores, finished,
+                (int)vocab_size, (int)beams, (int)select, (int)end_token, keep_slots, out_scores,
+                out_parents, out_tokens, out_finished);
+    return (int)hipPeekAtLastError();
+}

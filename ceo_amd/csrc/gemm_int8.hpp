@@ -1,0 +1,447 @@
+// Products in 8-bit integers with a scale for each token and channel, for gfx950
+// (included by gemm_int8.hip).
+//
+//   sx_m = max_k |x_mk| / 127, qx_mk = x_mk / sx_m to the nearest whole number (ties to even)
+//   sw_n, qw_kn the same over the columns of the weight, once, when it is packed
+//   y_mn = act((sum_k qx_mk qw_kn) sx_m sw_n + bias_n) + residual_mn, rounded once
+//
+// The sums are whole and exact (k <= 131072: below 2^31), so nothing depends on how they
+// are split.  A packed weight is one row of whole 128-byte lines per channel, zero
+// behind k, after the scales; quantised tokens are rows of the same length.
+#pragma once
+#include "common.hpp"
+#include "gemm_fast.hpp"
+
+namespace efla {
+namespace i8 {
+
+typedef __attribute__((__vector_size__(4 * sizeof(int)))) int int4v;
+typedef __attribute__((__vector_size__(16 * sizeof(int)))) int int16v;
+
+constexpr long kLine = 128;
+inline __host__ __device__ long up_to(long x, long m) { return (x + m - 1) / m * m; }
+
+// --- quantising -----------------------------------------------------------------
+// A row's (column's) scale from its largest magnitude.  NaN where that is not finite: the
+// row's products are NaN then.
+__device__ __forceinline__ float scale_of(float amax) {
+    return amax < INFINITY ? amax / 127.f : NAN;
+}
+
+// x / scale to the nearest whole number, ties to even, as an exact quotient would round.
+// x times the reciprocal is off by a few units in the last place, so the whole number
+// can miss by one next to a half; x - r scale, which one fused operation gives
+// without rounding (x and scale have 24 bits, r 7, and the difference is below scale),
+// says on which side of the half x lies.
+struct Quantizer {
+    float scale, inv, half;
+    bool zero, tiny;
+    __device__ __forceinline__ explicit Quantizer(float s)
+        : scale(s), inv(1.f / s), half(0.5f * s), zero(!(s > 0.f)), tiny(s < 0x1p-100f) {}
+    __device__ __forceinline__ int operator()(float x) const {
+        if (zero) return 0;  // a row of zeros, or one that is NaN
+        if (tiny)            // the reciprocal or the half may leave the normal range
+            return (int)fminf(fmaxf(rintf(x / scale), -127.f), 127.f);
+        float r = rintf(x * inv);
+        const float d = fmaf(-r, scale, x), t = fabsf(d);
+        const bool odd = (int)r & 1;
+        if (t > half || (t == half && odd)) r += copysignf(1.f, d);
+        return (int)r;
+    }
+};
+
+// The larger magnitude, NaN if either is: magnitudes are compared as whole numbers, in
+// which NaN is above infinity.
+__device__ __forceinline__ float amax2(float a, float x) {
+    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(x) & 0x7FFFFFFFu));
+}
+__device__ __forceinline__ float wave_amax(float m) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = amax2(m, __shfl_xor(m, o));
+    return m;
+}
+
+// 8 elements from p on, those past cnt zero
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, long cnt, float (&v)[8]) {
+    const auto x = gf::Piece<8, T>::load(p, cnt);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
+}
+
+__device__ __forceinline__ uint2 pack8(const Quantizer& q, const float (&v)[8]) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e / 4] |= ((uint32_t)q(v[e]) & 0xFFu) << (8 * (e & 3));
+    return make_uint2(w[0], w[1]);
+}
+
+// One wave quantises a row: q gets kp bytes (zero behind k).  Rows of up to 64 * 8 * HOLD
+// elements stay in registers between the maximum and the quotients, longer ones are read
+// again.  Returns the scale.
+template <typename T, int HOLD>
+__device__ __forceinline__ float quantize_row(const T* x, long k, long kp, uint8_t* q) {
+    const int l = lane_id();
+    float v[HOLD][8];
+    float m = 0.f;
+    for (long c0 = 0; c0 < kp; c0 += 512 * HOLD) {
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i) {
+            const long c = c0 + 8 * (l + 64 * i);
+            if (c < k) {
+                load8<T>(x + c, k - c, v[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = amax2(m, v[i][e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+            }
+        }
+    }
+    const float s = scale_of(wave_amax(m));
+    const Quantizer qz(s);
+    if (kp <= 512 * HOLD) {
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i) {
+            const long c = 8 * (l + 64 * i);
+            if (c < kp) *reinterpret_cast<uint2*>(q + c) = pack8(qz, v[i]);
+        }
+    } else {
+        for (long c = 8 * l; c < kp; c += 512) {
+            float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (c < k) load8<T>(x + c, k - c, y);
+            *reinterpret_cast<uint2*>(q + c) = pack8(qz, y);
+        }
+    }
+    return s;
+}
+
+// Four rows to a workgroup, a wave each.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ldx,
+                                                            long m, long k, long kp,
+                                                            uint8_t* __restrict__ q,
+                                                            float* __restrict__ scales) {
+    const long row = (long)blockIdx.x * 4 + wave_id();
+    if (row >= m) return;
+    const float s = quantize_row<T, 8>(x + row * ldx, k, kp, q + row * kp);
+    if (lane_id() == 0) scales[row] = s;
+}
+
+// Columns' largest magnitudes, as whole numbers, into amax (zero before).
+template <typename T>
+__global__ void __launch_bounds__(256) column_amax_kernel(const T* __restrict__ w, long ld, long k,
+                                                          long n, uint32_t* __restrict__ amax) {
+    const long c = (long)blockIdx.x * 256 + threadIdx.x;
+    if (c >= n) return;
+    float m = 0.f;
+    for (long r = blockIdx.y; r < k; r += gridDim.y) m = amax2(m, to_f(w[r * ld + c]));
+    atomicMax(amax + c, __float_as_uint(m));
+}
+
+// 64 x 64 tiles of the weight, quantised and turned through LDS: a row of q per channel.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_weight_kernel(const T* __restrict__ w, long ld, long k,
+                                                          long n, long kp,
+                                                          const uint32_t* __restrict__ amax,
+                                                          uint8_t* __restrict__ q) {
+    __shared__ uint8_t tile[64][68];
+    const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
+    for (long n0 = (long)blockIdx.x * 64; n0 < n; n0 += (long)gridDim.x * 64) {
+        for (long k0 = (long)blockIdx.y * 64; k0 < kp; k0 += (long)gridDim.y * 64) {
+            const long col = n0 + c;
+            const Quantizer qz(col < n ? scale_of(__uint_as_float(amax[col])) : 0.f);
+            for (int r = r0; r < 64; r += 4) {
+                const long row = k0 + r;
+                const float x = col < n && row < k ? to_f(w[row * ld + col]) : 0.f;
+                tile[c][r] = (uint8_t)qz(x);
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+                const int ch = i >> 4, b = 4 * (i & 15);
+                if (n0 + ch < n)
+                    *reinterpret_cast<uint32_t*>(q + (n0 + ch) * kp + k0 + b) =
+                        *reinterpret_cast<const uint32_t*>(&tile[ch][b]);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) column_scales_kernel(uint32_t* __restrict__ amax, long n) {
+    const long c = (long)blockIdx.x * 256 + threadIdx.x;
+    if (c < n) reinterpret_cast<float*>(amax)[c] = scale_of(__uint_as_float(amax[c]));
+}
+
+// --- epilogue -----------------------------------------------------------------------
+template <typename T>
+struct Out {
+    T* y;
+    long ldy;
+    const T* bias;      // [n] or NULL
+    const T* residual;  // or NULL
+    long ldr;
+    const float* sw;
+    int gelu;
+};
+
+// W columns n .. of row m, cnt = N - n of them in the matrix
+template <int W, typename T, bool RAGGED>
+__device__ __forceinline__ void finish(const Out<T>& o, long m, long n, long cnt, const int* acc,
+                                       float sx) {
+    typedef gf::Piece<W, T, RAGGED> P;
+    typedef gf::Piece<W, float, RAGGED> F;
+    const typename F::vec sw = F::load(o.sw + n, cnt);
+    float v[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = (float)acc[e] * sx * sw[e];
+    if (o.bias) {
+        const typename P::vec b = P::load(o.bias + n, cnt);
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] += (float)b[e];
+    }
+    if (o.gelu) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] = gelu::gelu_f<true>(v[e]);
+    }
+    if (o.residual) {
+        const typename P::vec r = P::load(o.residual + m * o.ldr + n, cnt);
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] += (float)r[e];
+    }
+    typename P::vec y;
+#pragma unroll
+    for (int e = 0; e < W; ++e) y[e] = (T)v[e];
+    P::store(o.y + m * o.ldy + n, y, cnt);
+}
+
+// --- few rows -------------------------------------------------------------------------
+// M <= 16 MT rows.  Bound by the weight, which is read once.  A wave takes 16 channels and
+// a range of k; the weights are the MFMA's A operand (16 x 16 x 64), read straight from
+// memory, 16 bytes a lane.  KW waves of a workgroup share their channels and split k; their
+// sums meet in LDS.  FUSED: the workgroup quantises the tokens into LDS itself, while
+// its first weights are on their way; otherwise they are read quantised.
+constexpr int kFewWaves = 8;
+constexpr int kAhead = 8;  // 64-byte steps of k whose weights a wave has in flight
+
+template <typename T, int MT, bool FUSED>
+__global__ void __launch_bounds__(64 * kFewWaves)
+few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
+           const float* __restrict__ xs, const uint8_t* __restrict__ wq, int M, int N, long k,
+           long kp, int kw, Out<T> o) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int w = wave_id(), l = lane_id(), r = l & 15, g = l >> 4;
+    const int cw = kFewWaves / kw, wk = w % kw;
+    const long n0 = ((long)blockIdx.x * cw + w / kw) * 16;
+    const int steps = (int)(kp / 64), s0 = steps * wk / kw, s1 = steps * (wk + 1) / kw;
+    const uint8_t* wp = wq + (n0 + r < N ? n0 + r : N - 1) * kp + 16 * g;
+    int4v a[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int s = s0 + i < s1 ? s0 + i : s0;
+        a[i] = *reinterpret_cast<const int4v*>(wp + 64L * s);
+    }
+    const long ldq = FUSED ? kp + 16 : kp;
+    float* sc = reinterpret_cast<float*>(lds);  // 16 MT scales
+    uint8_t* rows = lds + 64 * MT;
+    if constexpr (FUSED) {
+        for (int m = w; m < 16 * MT; m += kFewWaves) {
+            if (m < M) {
+                const float s = quantize_row<T, 2>(x + m * ldx, k, kp, rows + m * ldq);
+                if (l == 0) sc[m] = s;
+            } else {
+                for (long c = 16 * l; c < kp; c += 1024)
+                    *reinterpret_cast<int4v*>(rows + m * ldq + c) = int4v{};
+            }
+        }
+        __syncthreads();
+    }
+    int4v acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = int4v{};
+    const uint8_t* bp[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = 16 * t + r;
+        bp[t] = (FUSED ? rows + m * ldq : xq + (m < M ? m : M - 1) * ldq) + 16 * g;
+    }
+    for (int s = s0; s < s1; s += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (s + i >= s1) break;
+            const int4v wa = a[i];
+            if (s + i + kAhead < s1)
+                a[i] = *reinterpret_cast<const int4v*>(wp + 64L * (s + i + kAhead));
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int4v b = *reinterpret_cast<const int4v*>(bp[t] + 64L * (s + i));
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wa, b, acc[t], 0, 0, 0);
+            }
+        }
+    }
+    // lane l: row 16 t + r, channels n0 + 4 g .. + 3
+    if (kw > 1) {
+        if constexpr (FUSED) __syncthreads();  // the tokens have been read
+        int4v* part = reinterpret_cast<int4v*>(rows);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) part[(w * MT + t) * 64 + l] = acc[t];
+        __syncthreads();
+        if (wk != 0) return;
+        for (int j = 1; j < kw; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] += part[((w + j) * MT + t) * 64 + l];
+    }
+    const long n = n0 + 4 * g;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = 16 * t + r;
+        if (m >= M || n >= N) continue;
+        const int v[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+        finish<4, T, true>(o, m, n, N - n, v, FUSED ? sc[m] : xs[m]);
+    }
+}
+
+// --- many rows ------------------------------------------------------------------------
+// The tiles of gemm_fast.hpp with both operands k-contiguous and two 8-bit integers in the
+// place of each 16-bit element: 256 x 256 x 128 (eight waves of 128 x 64) or 128 x 128 x 128
+// (four of 64 x 64, two workgroups to a CU), copied straight into LDS one block ahead,
+// MFMA 32 x 32 x 32.  Rows are padded to whole blocks, so there is no tail in k.
+template <typename T, int TS, bool RAGGED>
+__global__ void __launch_bounds__(64 * gf::tile_waves<TS>(), TS == 128 ? 2 : 1)
+tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
+            Out<T> o) {
+    constexpr int TILE = gf::tile_bytes<TS>(), TNI = 2, TMJ = TS / 64, KS = 4;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+    const long tm_n = (M + TS - 1) / TS, tn_n = (N + TS - 1) / TS, nitems = tm_n * tn_n;
+    // XCD bands, then groups of 8 tile rows
+    auto decode = [&](long it, int& m0, int& n0) {
+        long id = it;
+        if (nitems % 8 == 0) id = (id % 8) * (nitems / 8) + id / 8;
+        const long span = 8 * tn_n, gi = id / span, first = gi * 8;
+        const long gsize = (tm_n - first) < 8 ? (tm_n - first) : 8;
+        m0 = __builtin_amdgcn_readfirstlane((int)((first + (id % span) % gsize) * TS));
+        n0 = __builtin_amdgcn_readfirstlane((int)(((id % span) / gsize) * TS));
+    };
+    const int w = mf::wave();
+    const int wm = (w & 1) * (TS / 2), wn = (w >> 1) * (32 * TNI);
+    auto As = [&](int b) { return smem + 2 * b * TILE; };
+    auto Bs = [&](int b) { return smem + (2 * b + 1) * TILE; };
+    long it = blockIdx.x;
+    if (it >= nitems) return;
+    long fit = it;
+    int fkt = 0, fm0, fn0;
+    bool fmore = true;
+    decode(fit, fm0, fn0);
+    auto fetch = [&](int b, int l) {
+        if (!fmore) return;
+        gf::copy_tile<true, TS>(A, fm0, (long)fkt * gf::BK, As(b), w, l);
+        gf::copy_tile<true, TS>(B, fn0, (long)fkt * gf::BK, Bs(b), w, l);
+        if (++fkt == niter) {
+            fkt = 0;
+            fit += gridDim.x;
+            fmore = fit < nitems;
+            if (fmore) decode(fit, fm0, fn0);
+        }
+    };
+    int m0 = fm0, n0 = fn0;
+    fetch(0, mf::lane());
+    mf::dma_wait();
+    __syncthreads();
+    int buf = 0;
+    for (;;) {
+        const int l = mf::tid_in((int)it) & 63;
+        fetch(buf ^ 1, l);
+        int16v acc[TNI][TMJ];
+#pragma unroll
+        for (int i = 0; i < TNI; ++i)
+#pragma unroll
+            for (int j = 0; j < TMJ; ++j) acc[i][j] = int16v{};
+        const bool act = m0 + wm < M && n0 + wn < N;
+        int4v fb[2][TNI], fa[2][TMJ];
+        auto read = [&](int c, int b, int ks) {
+#pragma unroll
+            for (int i = 0; i < TNI; ++i)
+                fb[c][i] = __builtin_bit_cast(int4v, gf::frag<true, TS>(Bs(b), wn + 32 * i, ks, l));
+#pragma unroll
+            for (int j = 0; j < TMJ; ++j)
+                fa[c][j] = __builtin_bit_cast(int4v, gf::frag<true, TS>(As(b), wm + 32 * j, ks, l));
+        };
+        auto mma_step = [&](int c) {
+#pragma unroll
+            for (int i = 0; i < TNI; ++i)
+#pragma unroll
+                for (int j = 0; j < TMJ; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[c][i], fa[c][j], acc[i][j],
+                                                                      0, 0, 0);
+            constexpr int NR = TNI + TMJ, NM = TMJ * TNI, R = NR < NM ? NR : NM;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // DS read
+            }
+            if constexpr (NM > R) __builtin_amdgcn_sched_group_barrier(0x008, NM - R, 0);
+        };
+        if (act) read(0, buf, 0);
+        for (int kt = 0; kt < niter; ++kt) {
+            __builtin_amdgcn_s_setprio(1);
+            if (act) {
+#pragma unroll
+                for (int ks = 0; ks + 1 < KS; ++ks) {
+                    read((ks + 1) & 1, buf, ks + 1);
+                    mma_step(ks & 1);
+                }
+            }
+            __builtin_amdgcn_s_setprio(0);
+            mf::dma_wait();
+            __syncthreads();
+            __builtin_amdgcn_s_setprio(1);
+            if (kt + 1 < niter) fetch(buf, l);
+            if (act) {
+                read(KS & 1, buf ^ 1, 0);  // after the last iteration: not used
+                mma_step((KS - 1) & 1);
+            }
+            buf ^= 1;
+        }
+        __builtin_amdgcn_s_setprio(0);
+        // lane l, tile (i, j): row m0 + wm + 32 j + (l & 31), columns n0 + wn + 32 i + 8 q +
+        // 4 (l >> 5) + e in acc[i][j][4 q + e]: through the free buffer, 32 rows at a time,
+        // into 8-column pieces
+        {
+            const int le = mf::tid_in(~(int)it) & 63;
+            char* wp = smem + 2 * (buf ^ 1) * TILE + (4096 * TNI) * w;
+            constexpr int WC = 32 * TNI, NP = WC / 16;
+            const long mw = m0 + wm, nw = n0 + wn;
+#pragma unroll
+            for (int j = 0; j < TMJ; ++j) {
+                const long r0 = mw + 32 * j;
+                if (r0 >= M) break;
+#pragma unroll
+                for (int i = 0; i < TNI; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<int4v*>(
+                            wp + gf::ep_off<TNI>(le & 31, 32 * i + 8 * q + 4 * (le >> 5))) =
+                            int4v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                                  acc[i][j][4 * q + 3]};
+#pragma unroll
+                for (int s = 0; s < NP; ++s) {
+                    const int p = 64 * s + le, row = p / (WC / 8), c8 = p % (WC / 8);
+                    const long m = r0 + row, n = nw + 8 * c8;
+                    const int4v v0 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, 8 * c8));
+                    const int4v v1 =
+                        *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, 8 * c8 + 4));
+                    if (m >= M || n >= N) continue;
+                    const int v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                    finish<8, T, RAGGED>(o, m, n, N - n, v, xs[m]);
+                }
+            }
+        }
+        it += gridDim.x;
+        if (it >= nitems) break;
+        __syncthreads();
+        decode(it, m0, n0);
+    }
+}
+
+}  // namespace i8
+}  // namespace efla

@@ -628,3 +628,139 @@ def clip_grad_norm(grads, max_norm: float) -> torch.Tensor:
     rc = lib().grad_clip_hip(gl._handle, float(max_norm), _p(norm), _stream(norm))
     check(rc, "grad_clip_hip")
     return norm
+
+
+# ---------------------------------------------------------------------------
+# generating text
+# ---------------------------------------------------------------------------
+def _elsewhere(t: torch.Tensor) -> bool:
+    """Whether a tensor is on another device than the current one."""
+    return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, select=None, finished=None,
+                end_token=None, keep_slots: bool = False):
+    """(scores fp32, parents int32, tokens int32, finished bool or None), each (batch, select):
+    of each text's beams * vocab continuations the ``select`` (default: beams) with the largest
+    ``scores[b, k] + log softmax(logits)[b * beams + k, v]``, ties to the lowest
+    ``k * vocab + v``; ``parents`` is k and ``tokens`` v.
+
+    logits (batch * beams, vocab), bf16, fp16 or fp32 (a row stride is fine); scores (batch,
+    beams) fp32.  A beam marked in ``finished`` (bool, (batch, beams)) only continues with
+    ``end_token``, at its own score.  With ``end_token`` the marks of the selected are returned:
+    their beam had one, or the token is ``end_token``.  A beam of score -inf (the unused ones
+    at a search's start) or with a NaN or +inf among its logits has no continuation: -inf.
+
+    In order of their scores; with ``keep_slots`` (select == beams) instead the best
+    continuation of each beam in that beam's place and the others in the free ones, so
+    that ``state.reorder`` has little to move.  Up to 64 beams and 64 selected."""
+    if isinstance(logits, torch.Tensor) and _elsewhere(logits):
+        with torch.cuda.device(logits.device):
+            return beam_select(logits, scores, select, finished, end_token, keep_slots)
+    _require(logits, "logits", contiguous=False)
+    dt = DTYPE_CODES.get(logits.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {logits.dtype}")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be 2-D with contiguous rows")
+    dev = logits.device
+    _require(scores, "scores", torch.float32, dev)
+    if scores.dim() != 2 or scores.numel() != logits.shape[0]:
+        raise ValueError("scores must be (batch, beams), one for each row of logits")
+    B, K = scores.shape
+    N, V = logits.shape
+    ld = logits.stride(0) if N > 1 else max(V, 1)
+    if ld < V:
+        raise ValueError("logits rows overlap")
+    n = K if select is None else int(select)
+    if not (1 <= K <= 64 and 1 <= n <= 64 and n <= K * V):
+        raise ValueError("1 to 64 beams, select 1 to 64 and at most beams * vocab")
+    if keep_slots and n != K:
+        raise ValueError("keep_slots needs select == beams")
+    if finished is not None:
+        _require(finished, "finished", torch.bool, dev)
+        if finished.shape != scores.shape:
+            raise ValueError("finished must be (batch, beams)")
+        if end_token is None:
+            raise ValueError("finished needs end_token")
+    if end_token is not None and not 0 <= end_token < V:
+        raise ValueError("end_token is outside of the vocabulary")
+    out = torch.empty(B, n, dtype=torch.float32, device=dev)
+    parents, tokens = torch.empty(2, B, n, dtype=torch.int32, device=dev).unbind(0)
+    ended = None if end_token is None else torch.empty(B, n, dtype=torch.bool, device=dev)
+    wsb = lib().beam_select_workspace_size(B, K, V, n)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    rc = lib().beam_select_hip(
+        _p(logits), _p(scores), _p(finished), _p(out), _p(parents), _p(tokens), _p(ended), B, K, V,
+        ld, n, -1 if end_token is None else int(end_token), int(keep_slots), dt, _p(ws), wsb,
+        _stream(logits))
+    check(rc, "beam_select_hip")
+    return out, parents, tokens, ended
+
+
+class Int8Weight:
+    """A (k, n) weight in 8-bit integers with an fp32 scale for each of its n channels, laid
+    out once for ``linear_int8``: ``scale = max |w| / 127`` over a column, ``w / scale`` to the
+    nearest (ties to even).  From bf16, fp16 or fp32 (a row stride is fine); k up to 131072.
+    A column with a NaN or an infinity gives NaN."""
+
+    def __init__(self, weight: torch.Tensor):
+        _require(weight, "weight", contiguous=False)
+        dt = DTYPE_CODES.get(weight.dtype)
+        if dt is None:
+            raise ValueError(f"unsupported dtype {weight.dtype}")
+        if weight.dim() != 2 or (weight.stride(1) != 1 and weight.shape[1] > 1):
+            raise ValueError("weight must be 2-D with contiguous rows")
+        self.k, self.n = weight.shape
+        ld = weight.stride(0) if self.k > 1 else self.n
+        size = lib().int8_weight_size(self.k, self.n)
+        if size == 0 or ld < self.n:
+            raise ValueError("weight must be (k, n) with 1 <= k <= 131072, rows apart")
+        self.packed = torch.empty(size, dtype=torch.uint8, device=weight.device)
+        with torch.cuda.device(weight.device):
+            rc = lib().int8_weight_pack_hip(_p(weight), ld, _p(self.packed), self.k, self.n, dt,
+                                            _stream(weight))
+        check(rc, "int8_weight_pack_hip")
+
+
+def linear_int8(x: torch.Tensor, weight: Int8Weight, bias=None, residual=None,
+                gelu: bool = False) -> torch.Tensor:
+    """act(x @ weight + bias) + residual with x quantised as the weight is, a scale for each
+    row, and the product summed in whole numbers; x's type, rounded once.  x (m, k) in bf16,
+    fp16 or fp32 (a row stride is fine), bias (n,), residual (m, n) of x's type; act is GELU
+    (tanh) with ``gelu``.  A row with a NaN or an infinity gives NaN."""
+    if not isinstance(weight, Int8Weight):
+        raise TypeError("weight must be an Int8Weight")
+    if _elsewhere(weight.packed):
+        with torch.cuda.device(weight.packed.device):
+            return linear_int8(x, weight, bias, residual, gelu)
+    _require(x, "x", None, weight.packed.device, contiguous=False)
+    dt = DTYPE_CODES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    if x.dim() != 2 or x.shape[1] != weight.k or (x.stride(1) != 1 and weight.k > 1):
+        raise ValueError("x must be (m, k) with contiguous rows, k the weight's")
+    m, k, n = x.shape[0], weight.k, weight.n
+    ldx = x.stride(0) if m > 1 else k
+    if ldx < k:
+        raise ValueError("x rows overlap")
+    if bias is not None:
+        _require(bias, "bias", x.dtype, x.device)
+        if bias.shape != (n,):
+            raise ValueError("bias must hold one value per channel")
+    ldr = n
+    if residual is not None:
+        _require(residual, "residual", x.dtype, x.device, contiguous=False)
+        if residual.shape != (m, n) or (residual.stride(1) != 1 and n > 1):
+            raise ValueError("residual must be (m, n) with contiguous rows")
+        ldr = residual.stride(0) if m > 1 else n
+        if ldr < n:
+            ldr = n
+            residual = residual.contiguous()
+    y = torch.empty(m, n, dtype=x.dtype, device=x.device)
+    wsb = lib().linear_int8_workspace_size(m, k)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
+    rc = lib().linear_int8_hip(_p(x), ldx, _p(weight.packed), _p(bias), _p(residual), ldr, _p(y), n,
+                               m, k, n, int(gelu), dt, _p(ws), wsb, _stream(x))
+    check(rc, "linear_int8_hip")
+    return y

@@ -109,3 +109,73 @@ def sharded_forward(q, k, v, beta, segments: int, initial_state=None):
         o, _ = efla.chunk_efla_fwd(x["q"], x["k"], x["v"], x["beta"], initial_state=s_in)
         outs.append(o)
     return torch.cat(outs, dim=1), states[-1]
+
+
+class StateList:
+    """The states that a beam search carries, laid out once: tensors of batch * beams
+    contiguous rows each (recurrent states, the texts so far; any type), one device.
+
+    It keeps the tensors and the device table of their addresses.  ``reorder`` writes into
+    ``outs`` (shaped and typed like the states), or in place without.  Making one copies
+    to the device and freeing one waits for it: for a graph, make it before the
+    capture and keep it."""
+
+    def __init__(self, states, beams: int, outs=None):
+        self.states = list(states)
+        self.outs = None if outs is None else list(outs)
+        self.beams = int(beams)
+        self._handle = None
+        if not self.states:
+            raise ValueError("no states")
+        first = self.states[0]
+        efla._require(first, "a state")
+        rows = first.shape[0] if first.dim() else 0
+        if not 1 <= self.beams <= 64 or first.dim() == 0 or rows % self.beams:
+            raise ValueError("1 to 64 beams, and states of batch * beams rows")
+        for t in self.states:
+            efla._require(t, "a state", None, first.device)
+            if t.dim() == 0 or t.shape[0] != rows:
+                raise ValueError("states differ in their number of rows")
+        if self.outs is not None:
+            if len(self.outs) != len(self.states):
+                raise ValueError("states and outs differ in number")
+            for t, s in zip(self.outs, self.states):
+                efla._require(t, "an output", s.dtype, first.device)
+                if t.shape != s.shape:
+                    raise ValueError("an output's shape differs from its state's")
+        n = len(self.states)
+        self.device = first.device
+        self.batch = rows // self.beams
+        ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.states])
+        outp = None if self.outs is None else \
+            (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.outs])
+        row = (ctypes.c_size_t * n)(*[t.numel() // rows * t.element_size() if rows else 0
+                                      for t in self.states])
+        handle = ctypes.c_void_p()
+        with torch.cuda.device(self.device):
+            rc = lib().state_list_create_hip(ctypes.byref(handle), ptrs, outp, row, n, self.batch,
+                                             self.beams)
+        check(rc, "state_list_create_hip")
+        self._handle = handle
+
+    def __reduce__(self):  # a copy has a table of its own
+        return type(self), (self.states, self.beams, self.outs)
+
+    def __del__(self):
+        if getattr(self, "_handle", None) and lib is not None:  # None: the program's end
+            lib().state_list_destroy_hip(self._handle)
+            self._handle = None
+
+
+def reorder(states: StateList, parents: torch.Tensor) -> None:
+    """Row (b, j) of every state becomes what row (b, parents[b, j]) was: the beams' states in
+    the order that ``nn.beam_select`` left them.  parents (batch, beams) int32; one outside of
+    0 .. beams - 1 leaves its row as it is.  In place, rows that stay are not touched."""
+    if not isinstance(states, StateList):
+        raise TypeError("states must be a StateList")
+    efla._require(parents, "parents", torch.int32, states.device)
+    if parents.shape != (states.batch, states.beams):
+        raise ValueError("parents must be (batch, beams)")
+    with torch.cuda.device(states.device):
+        rc = lib().state_reorder_hip(states._handle, parents.data_ptr(), efla._stream(parents))
+    check(rc, "state_reorder_hip")

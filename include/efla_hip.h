@@ -652,6 +652,85 @@ int preference_loss_forward_backward_hip(
     hipStream_t stream);
 
 /* ========================================================================
+ * Generating text: beam search's selection, its states, 8-bit integer products
+ *
+ * No reference counterpart: the reference trains (src/runtime/trainer.zig:152-185) and
+ * carries a state between calls (src/model/efla.zig:13-86), but generates nothing.
+ * All may be captured into a graph when they are given their workspace.
+ * ======================================================================== */
+
+/*
+ * Of each text's beams * vocab_size continuations the `select` best, in order:
+ *   value(k, v) = scores[k] + logits[k][v] - log sum_v exp logits[k][v],
+ * ties to the lowest k * vocab_size + v.  logits (batch * beams, vocab_size), row stride
+ * ld, F32, F16 or BF16; scores (batch, beams) fp32; out_scores fp32, out_parents (the beam,
+ * 0 .. beams - 1) and out_tokens int32, all (batch, select).
+ * finished (batch, beams) bytes or NULL: a beam that is marked has one continuation,
+ * end_token at the beam's own score, and its logits are not read.  out_finished (batch,
+ * select) bytes or NULL: the parent is marked or the token is end_token (it may be
+ * `finished` itself where select == beams).  Without both end_token is not looked at.
+ * A beam whose score is not finite, or whose logits hold a NaN, +inf or nothing above
+ * -inf, has no continuation: -inf for each.  Those come last, lowest first like all ties.
+ * keep_slots (select == beams): not in order, but the best continuation of a beam in that
+ * beam's place and the others in the free places, so that most states stay where they are.
+ * 1 .. 64 beams, select 1 .. 64 and no more than beams * vocab_size.
+ * Workspace (8-byte aligned) of at least beam_select_workspace_size() bytes (0: arguments out
+ * of range), or NULL: the library's cached one for `stream`.  Invalid arguments -> 1, sizes
+ * out of range (vocab_size or rows past 2^30 or 2^31) -> 9; batch == 0 -> 0.
+ */
+size_t beam_select_workspace_size(size_t batch, size_t beams, size_t vocab_size, size_t select);
+int beam_select_hip(const void* logits, const float* scores, const uint8_t* finished,
+                    float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                    uint8_t* out_finished, size_t batch, size_t beams, size_t vocab_size,
+                    size_t ld, size_t select, int32_t end_token, int keep_slots, int dtype,
+                    void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * A list of the states that beams carry: `count` tensors of batch * beams contiguous rows,
+ * tensor i's of row_bytes[i] bytes, at states[i]; outs[i] of the same shape, or outs NULL:
+ * in place.  The list keeps the addresses in a device table (made by a copy to the device,
+ * freed by state_list_destroy_hip, which waits for it) on the current device; the
+ * memory stays the caller's.  No two tensors may overlap (-> 1).  1 .. 64 beams.
+ * state_reorder_hip: row (b, j) of each output is row (b, parents[b][j]) of its state, as
+ * all rows were before the call; parents (batch, beams) int32 on the device.  A parent outside
+ * of 0 .. beams - 1 stands for j itself.  One launch; in place, rows that stay are not
+ * touched.  The current device has to be the list's (-> 101); one call at a time may use
+ * memory that another writes, as for any kernel.
+ */
+int state_list_create_hip(void** list, void* const* states, void* const* outs,
+                          const size_t* row_bytes, size_t count, size_t batch, size_t beams);
+int state_list_destroy_hip(void* list);
+int state_reorder_hip(const void* list, const int32_t* parents, hipStream_t stream);
+
+/*
+ * A weight (k, n) in 8-bit integers with a scale per channel (column):
+ *   scale_n = max_k |w_kn| / 127 in fp32, q_kn = w_kn / scale_n to the nearest, ties to even.
+ * int8_weight_size: bytes of the packed form (0: k or n out of range); `packed` is
+ * 128-byte aligned.  weight: F32, F16 or BF16, row stride ld.  A column with a NaN or an
+ * infinity has scale NaN.  k is at most 131072 (-> 9), so that sums stay below 2^31.
+ */
+size_t int8_weight_size(size_t k, size_t n);
+int int8_weight_pack_hip(const void* weight, size_t ld, void* packed, size_t k, size_t n,
+                         int dtype, hipStream_t stream);
+
+/*
+ * output = act(x w + bias) + residual, x (m, k) quantised like the weight, a scale per row, and
+ * the product summed in whole numbers: act((sum_k qx_mk qw_kn) sx_m sw_n + bias_n) +
+ * residual_mn in fp32, rounded once.  act is GELU's tanh form with `gelu`, else nothing;
+ * bias (n) and residual (m, n) may be NULL.  x, bias, residual and output are of `dtype`
+ * (F32, F16 or BF16), whatever the packed weight was made from; any row strides and element
+ * alignment; output may be residual itself, x neither.  A row of x with a NaN or an infinity
+ * gives a row of NaN.  Workspace (16-byte aligned) of at least linear_int8_workspace_size()
+ * bytes, or NULL: the library's cached one for `stream`.  Calls with the same row of x give
+ * the same bits in that row, whatever m is.  Codes as above; m == 0 -> 0.
+ */
+size_t linear_int8_workspace_size(size_t m, size_t k);
+int linear_int8_hip(const void* x, size_t ldx, const void* packed, const void* bias,
+                    const void* residual, size_t ld_residual, void* output, size_t ld_output,
+                    size_t m, size_t k, size_t n, int gelu, int dtype, void* workspace,
+                    size_t workspace_bytes, hipStream_t stream);
+
+/* ========================================================================
  * Sequence packing (host, no GPU)
  * ======================================================================== */
 
