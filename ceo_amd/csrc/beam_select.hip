@@ -36,6 +36,7 @@ namespace bs {
 constexpr int NT = 256, NWV = NT / kWave;
 constexpr int kMaxSelect = 64, kMaxBeams = 64;
 constexpr int kPlaces = 1024;  // candidates that LDS holds
+constexpr int kVectors = 512;  // and 16-byte vectors that have some
 
 // What is left of a slice: one of its best logits; none: token -1.
 struct Cand {
@@ -77,23 +78,25 @@ __device__ __forceinline__ float exp_diff(float d) {  // e^d
 // first element's place in its line, and slice s holds [s L, (s + 1) L) of that.
 template <typename T, int VPT>
 __global__ void __launch_bounds__(NT)
-slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
+slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
              const float* __restrict__ scores, const uint8_t* __restrict__ finished,
              float2* __restrict__ stats, Cand* __restrict__ cands) {
     constexpr int N = 16 / sizeof(T), L = NT * VPT * N;
     typedef __attribute__((__vector_size__(16))) T Vec;
+    __shared__ Vec piece[kVectors];
+    __shared__ int piece_at[kVectors];  // its first token
     __shared__ uint64_t place[kPlaces];
     __shared__ float wm[NWV], ws[NWV];
     __shared__ uint32_t wb[NWV];
     __shared__ uint64_t best[NWV];
-    __shared__ int count;
+    __shared__ int pieces, count;
     const long row = blockIdx.y;
     // a beam that offers no continuation is not read
     if ((finished && finished[row]) || !(fabsf(scores[row]) < INFINITY)) return;
     const T* p = logits + row * ld;
     const int shift = (int)((uintptr_t)p % 128 / sizeof(T));
     const long v0 = (long)blockIdx.x * L - shift;  // the slice's first token
-    if (threadIdx.x == 0) count = 0;
+    if (threadIdx.x == 0) pieces = count = 0;
 
     Vec x[VPT];
 #pragma unroll
@@ -107,12 +110,15 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
                 x[i][j] = v + j >= 0 && v + j < V ? p[v + j] : (T)-INFINITY;
         }
     }
-    float m = -INFINITY;
+    float vm[VPT], m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+        vm[i] = to_f(x[i][0]);
 #pragma unroll
-        for (int j = 0; j < N; ++j) m = fmaxf(m, to_f(x[i][j]));
-    m += 0.f;  // -0 is 0
+        for (int j = 1; j < N; ++j) vm[i] = fmaxf(vm[i], to_f(x[i][j]));
+        vm[i] = fmaxf(vm[i], -INFINITY) + 0.f;  // no NaN, and -0 is 0
+        m = fmaxf(m, vm[i]);
+    }
     // a thread without a logit above -inf: 0, or NaN from a NaN
     const float m0 = m == -INFINITY ? 0.f : m;
     float s = 0.f;
@@ -125,7 +131,7 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
     const float M0 = M == -INFINITY ? 0.f : M;
-    s *= exp_diff(m0 - M0 < 0.f ? m0 - M0 : 0.f);
+    s *= exp_diff(fminf(m0 - M0, 0.f));
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if (lane_id() == 0) {
@@ -137,6 +143,16 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
     uint32_t least = wb[0];
 #pragma unroll
     for (int k = 1; k < NWV; ++k) least = max(least, wb[k]);
+    // vectors that reach the bound
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        if (vm[i] == -INFINITY || ordered(vm[i]) < least) continue;
+        const int at = atomicAdd(&pieces, 1);
+        if (at < kVectors) {
+            piece[at] = x[i];
+            piece_at[at] = (int)(v0 + (long)(threadIdx.x + i * NT) * N);
+        }
+    }
     const long slot = row * gridDim.x + blockIdx.x;
     if (threadIdx.x == 0) {
         float W = wm[0];
@@ -148,30 +164,31 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
             sum += wm[k] == -INFINITY ? ws[k] : ws[k] * exp_diff(wm[k] - W);
         stats[slot] = make_float2(W, sum);
     }
-    // key: the logit, then the lower token
-    auto key_of = [&](int i, int j) {
-        const float z = to_f(x[i][j]) + 0.f;
-        const uint32_t v = (uint32_t)(v0 + (long)(threadIdx.x + i * NT) * N + j);
+    __syncthreads();
+    // key: the logit, then the lower token; 0: none
+    auto key_of = [](T logit, uint32_t v) {
+        const float z = to_f(logit) + 0.f;
         return z > -INFINITY ? (uint64_t)ordered(z) << 32 | (uint32_t)~v : 0ull;
     };
-    if (m > -INFINITY && ordered(m) >= least) {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const uint64_t key = key_of(i, j);
-                if (key == 0 || (uint32_t)(key >> 32) < least) continue;
-                const int at = atomicAdd(&count, 1);
-                if (at < kPlaces) place[at] = key;
-            }
-    }
-    __syncthreads();
-    const int c = count;
     Cand* out = cands + slot * n;
     auto write = [&](int rank, uint64_t key) {
         out[rank] = Cand{unordered((uint32_t)(key >> 32)), (int)~(uint32_t)key};
     };
-    if (c <= kPlaces) {
+    // their elements that do
+    const int np = pieces;
+    if (np <= kVectors) {
+        for (int i = threadIdx.x; i < np * N; i += NT) {
+            const T* e = reinterpret_cast<const T*>(&piece[i / N]);
+            const uint64_t key = key_of(e[i % N], (uint32_t)(piece_at[i / N] + i % N));
+            if (key != 0 && (uint32_t)(key >> 32) >= least) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kPlaces) place[at] = key;
+            }
+        }
+    }
+    __syncthreads();
+    const int c = count;
+    if (np <= kVectors && c <= kPlaces) {
         for (int i = threadIdx.x; i < c; i += NT) {
             const uint64_t mine = place[i];
             int rank = 0;
@@ -181,17 +198,17 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
         for (int i = c + threadIdx.x; i < n; i += NT) out[i] = Cand{0.f, -1};
         return;
     }
-    // too many: the best, then the best below it, n times (c > n: there are as many)
+    // too many (equal logits): the best, then the best below it, n times; read again, since
+    // the loop would keep every key in registers
     uint64_t last = ~0ull;
     for (int r = 0; r < n; ++r) {
         uint64_t top = 0;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const uint64_t key = key_of(i, j);
-                if (key < last && key > top) top = key;
-            }
+        for (int i = threadIdx.x; i < L; i += NT) {
+            const long v = v0 + i;
+            if (v < 0 || v >= V) continue;
+            const uint64_t key = key_of(p[v], (uint32_t)v);
+            if (key < last && key > top) top = key;
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             const uint64_t other = __shfl_xor(top, o);
@@ -204,7 +221,8 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
 #pragma unroll
         for (int k = 1; k < NWV; ++k)
             if (best[k] > last) last = best[k];
-        if (threadIdx.x == 0) write(r, last);
+        if (threadIdx.x == 0) out[r] = Cand{0.f, -1};
+        if (threadIdx.x == 0 && last != 0) write(r, last);
     }
 }
 
@@ -225,6 +243,7 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
             int beams, int n, int end_token, int keep_slots, float* __restrict__ out_scores,
             int* __restrict__ out_parents, int* __restrict__ out_tokens,
             uint8_t* __restrict__ out_finished) {
+    constexpr int H = 8;  // entries of a thread in flight
     __shared__ double offset[kMaxBeams];  // score - log sum exp; -inf: offers nothing
     __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
     __shared__ Best place[kPlaces];
@@ -233,53 +252,81 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     __shared__ uint32_t wb[NWV];
     __shared__ int count;
     const long text = blockIdx.x, row0 = text * beams;
+    const int per = slices * n, total = beams * per;
+    const Cand* mine = cands + row0 * per;
+    Cand c[H];
+    // H entries from `base` on, the threads' own; what beams that were not read left there
+    // is not looked at
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const int e = base + (int)threadIdx.x + i * NT;
+            c[i] = e < total ? mine[e] : Cand{0.f, -1};
+        }
+    };
+    fetch(0);
     if (threadIdx.x == 0) count = 0;
-    for (int k = wave_id(); k < beams; k += NWV) {
+    // 16 lanes to a beam
+    for (int k = threadIdx.x / 16; k < beams; k += NT / 16) {
+        const int l = threadIdx.x % 16;
         const float score = scores[row0 + k];
         const bool fin = finished && finished[row0 + k], ok = fabsf(score) < INFINITY;
         double lse = 0.0;
         if (ok && !fin) {
             const float2* st = stats + (row0 + k) * slices;
             float M = -INFINITY;
-            for (int i = lane_id(); i < slices; i += kWave) M = fmaxf(M, st[i].x);
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
             double s = 0.0;
-            for (int i = lane_id(); i < slices; i += kWave) {
+            // joined as they come: a slice without a logit above -inf has 0, or NaN from a NaN
+            for (int i = l; i < slices; i += 16) {
                 const float2 a = st[i];
-                // a slice without a logit above -inf: 0, or NaN from a NaN
-                s += a.x == -INFINITY ? (double)a.y : (double)a.y * exp((double)a.x - (double)M);
+                const float W = fmaxf(M, a.x);
+                s = (M < W ? s * exp((double)M - (double)W) : s) +
+                    (a.x < W ? (double)a.y * exp((double)a.x - (double)W) : (double)a.y);
+                M = W;
             }
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+            for (int o = 8; o > 0; o >>= 1) {
+                const float Mo = __shfl_xor(M, o, 16);
+                const double so = __shfl_xor(s, o, 16);
+                const float W = fmaxf(M, Mo);
+                s = (M < W ? s * exp((double)M - (double)W) : s) +
+                    (Mo < W ? so * exp((double)Mo - (double)W) : so);
+                M = W;
+            }
             lse = (double)M + log(s);
         }
-        if (lane_id() == 0) {
+        if (l == 0) {
             const bool live = ok && fabs(lse) < (double)INFINITY;
             state[k] = !live ? 2 : fin ? 1 : 0;
             offset[k] = live ? (double)score - lse : -(double)INFINITY;
         }
     }
     __syncthreads();
-    const int per = slices * n, total = beams * per;
-    // entry e, or a value of -inf; a finished beam has one
-    auto entry = [&](int e) {
-        const int k = e / per, i = e - k * per;
-        Best b{-(double)INFINITY, k, 0};
-        if (state[k] == 0) {
-            const Cand c = cands[(row0 + k) * per + i];
-            if (c.token >= 0) b = Best{(double)c.z + offset[k], k, c.token};
-        } else if (state[k] == 1 && i == 0) {
-            b = Best{offset[k], k, end_token};
+    // entry e's value from its logit; a finished beam has one entry
+    auto value_of = [&](int e, const Cand& x) {
+        Best b{-(double)INFINITY, 0, 0};
+        if (e >= total) return b;
+        b.beam = (int)((unsigned)e / (unsigned)per);
+        if (state[b.beam] == 0) {
+            if (x.token >= 0) {
+                b.value = (double)x.z + offset[b.beam];
+                b.token = x.token;
+            }
+        } else if (state[b.beam] == 1 && e == b.beam * per) {
+            b.value = offset[b.beam];
+            b.token = end_token;
         }
         return b;
     };
+    const bool held = total <= H * NT;
     uint64_t top = 0;
-    for (int e = threadIdx.x; e < total; e += NT) {
-        const Best b = entry(e);
-        if (b.value > -(double)INFINITY) {
+    for (int base = 0; base < total; base += H * NT) {
+        if (base) fetch(base);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const Best b = value_of(base + (int)threadIdx.x + i * NT, c[i]);
             const uint64_t o = ordered(b.value + 0.0);
-            if (o > top) top = o;
+            if (b.value > -(double)INFINITY && o > top) top = o;
         }
     }
     const uint32_t bound = wave_bound<4>((uint32_t)(top >> 32), n);
@@ -288,39 +335,44 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     uint32_t least = wb[0];
 #pragma unroll
     for (int k = 1; k < NWV; ++k) least = max(least, wb[k]);
-    for (int e = threadIdx.x; e < total; e += NT) {
-        const Best b = entry(e);
-        if (!(b.value > -(double)INFINITY) || (uint32_t)(ordered(b.value + 0.0) >> 32) < least)
-            continue;
-        const int at = atomicAdd(&count, 1);
-        if (at < kPlaces) place[at] = b;
+    for (int base = 0; base < total; base += H * NT) {
+        if (!held) fetch(base);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const Best b = value_of(base + (int)threadIdx.x + i * NT, c[i]);
+            if (!(b.value > -(double)INFINITY) ||
+                (uint32_t)(ordered(b.value + 0.0) >> 32) < least)
+                continue;
+            const int at = atomicAdd(&count, 1);
+            if (at < kPlaces) place[at] = b;
+        }
     }
     __syncthreads();
-    const int c = count;
-    if (c <= kPlaces) {
-        for (int i = threadIdx.x; i < c; i += NT) {
-            const Best mine = place[i];
+    const int found = count;
+    if (found <= kPlaces) {
+        for (int i = threadIdx.x; i < found; i += NT) {
+            const Best b = place[i];
             int rank = 0;
-            for (int k = 0; k < c; ++k) rank += better(place[k], mine);
-            if (rank < n) res[rank] = mine;
+            for (int k = 0; k < found; ++k) rank += better(place[k], b);
+            if (rank < n) res[rank] = b;
         }
     } else {
         // too many (equal values): the best, then the best behind it, n times
         Best last{(double)INFINITY, -1, -1};
         for (int r = 0; r < n; ++r) {
-            Best mine{-(double)INFINITY, beams, 0};
+            Best b{-(double)INFINITY, beams, 0};
             for (int e = threadIdx.x; e < total; e += NT) {
-                const Best b = entry(e);
-                if (b.value > -(double)INFINITY && better(last, b) && better(b, mine)) mine = b;
+                const Best x = value_of(e, mine[e]);
+                if (x.value > -(double)INFINITY && better(last, x) && better(x, b)) b = x;
             }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) {
-                const Best other{__shfl_xor(mine.value, o), __shfl_xor(mine.beam, o),
-                                 __shfl_xor(mine.token, o)};
-                if (better(other, mine)) mine = other;
+                const Best x{__shfl_xor(b.value, o), __shfl_xor(b.beam, o),
+                             __shfl_xor(b.token, o)};
+                if (better(x, b)) b = x;
             }
             __syncthreads();  // `wbest` has been read
-            if (lane_id() == 0) wbest[wave_id()] = mine;
+            if (lane_id() == 0) wbest[wave_id()] = b;
             __syncthreads();
             last = wbest[0];
 #pragma unroll
@@ -331,11 +383,11 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     }
     __syncthreads();
     // fewer finite values than asked for: the lowest pairs that are not among them
-    if (threadIdx.x == 0 && c < n) {
+    if (threadIdx.x == 0 && found < n) {
         int beam = 0, token = 0;
-        for (int r = c; r < n;) {
+        for (int r = found; r < n;) {
             bool taken = false;
-            for (int k = 0; k < c; ++k) taken |= res[k].beam == beam && res[k].token == token;
+            for (int k = 0; k < found; ++k) taken |= res[k].beam == beam && res[k].token == token;
             if (!taken) res[r++] = Best{-(double)INFINITY, beam, token};
             if (++token == V) token = 0, ++beam;
         }
@@ -396,7 +448,7 @@ static size_t scratch(size_t batch, size_t beams, size_t vocab, size_t n) {
 
 template <typename T>
 static void launch(const void* logits, const float* scores, const uint8_t* finished,
-                   const uint8_t* ws, size_t rows, size_t beams, size_t vocab, size_t ld, size_t n,
+                   const uint8_t* ws, size_t rows, size_t vocab, size_t ld, size_t n,
                    int vpt, size_t slices, hipStream_t st) {
     float2* stats = (float2*)ws;
     Cand* cands = (Cand*)(stats + rows * slices);
@@ -406,7 +458,7 @@ static void launch(const void* logits, const float* scores, const uint8_t* finis
         const size_t s0 = r0 * slices;
 #define BS_SLICE(VPT)                                                                          \
     EFLA_LAUNCH("beam_slice", (slice_kernel<T, VPT>), grid, dim3(NT), st, z + r0 * ld, (long)ld, \
-                (int)vocab, (int)beams, (int)n, scores + r0, finished ? finished + r0 : nullptr, \
+                (int)vocab, (int)n, scores + r0, finished ? finished + r0 : nullptr, \
                 stats + s0, cands + s0 * n)
         if (vpt == 1) BS_SLICE(1);
         else if (vpt == 2) BS_SLICE(2);
@@ -461,13 +513,13 @@ extern "C" int beam_select_hip(const void* logits, const float* scores, const ui
     const bool lines = (uintptr_t)logits % 128 == 0 && ld * size % 128 == 0;
     const size_t slices = bs::slices_of(vocab_size, size, vpt, lines);
     if (dtype == kDtypeBF16)
-        bs::launch<bf16>(logits, scores, finished, (const uint8_t*)ws, rows, beams, vocab_size, ld,
+        bs::launch<bf16>(logits, scores, finished, (const uint8_t*)ws, rows, vocab_size, ld,
                          select, vpt, slices, stream);
     else if (dtype == kDtypeF16)
-        bs::launch<f16>(logits, scores, finished, (const uint8_t*)ws, rows, beams, vocab_size, ld,
+        bs::launch<f16>(logits, scores, finished, (const uint8_t*)ws, rows, vocab_size, ld,
                         select, vpt, slices, stream);
     else
-        bs::launch<float>(logits, scores, finished, (const uint8_t*)ws, rows, beams, vocab_size, ld,
+        bs::launch<float>(logits, scores, finished, (const uint8_t*)ws, rows, vocab_size, ld,
                           select, vpt, slices, stream);
     EFLA_CHECK(hipPeekAtLastError());
     const float2* stats = (const float2*)ws;

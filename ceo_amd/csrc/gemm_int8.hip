@@ -80,8 +80,13 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     if (!fused((size_t)m, (size_t)kp)) {
         xs = (float*)ws;
         xq = ws + scales_bytes((size_t)m);
-        EFLA_LAUNCH("quantize_rows", quantize_rows_kernel<T>, dim3((unsigned)((m + 3) / 4)),
-                    dim3(256), st, x, ldx, m, k, kp, xq, xs);
+        const dim3 grid((unsigned)((m + 3) / 4)), block(256);
+        if (kp <= 1024)
+            EFLA_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 2>), grid, block, st, x, ldx, m, k,
+                        kp, xq, xs);
+        else
+            EFLA_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 8>), grid, block, st, x, ldx, m, k,
+                        kp, xq, xs);
         EFLA_CHECK(hipPeekAtLastError());
     }
     if (m <= (long)kFewRows) {

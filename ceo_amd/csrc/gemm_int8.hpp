@@ -48,6 +48,28 @@ struct Quantizer {
         if (t > half || (t == half && odd)) r += copysignf(1.f, d);
         return (int)r;
     }
+    // Eight of them, a byte each.  A fused multiply and add of 1.5 2^23 rounds x inv to a
+    // whole number that its low byte holds; x inv itself is off by 127 * 2^-23 at most, so
+    // only what lies within 2^-14 of a half is looked at again (one vector in sixty).
+    __device__ __forceinline__ uint2 pack(const float (&v)[8]) const {
+        constexpr float kRound = 12582912.f;
+        uint32_t w[8];
+        float far = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float t = fmaf(v[e], inv, kRound);
+            w[e] = __float_as_uint(t);
+            far = fmaxf(far, fabsf(fmaf(v[e], inv, kRound - t)));
+        }
+        if (zero || tiny || !(far < 0.5f - 0x1p-14f)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = (uint32_t)(*this)(v[e]);
+        }
+        auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+            return __builtin_amdgcn_perm(b, a, 0x0C0C0400u) | __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
+        };
+        return make_uint2(four(w[0], w[1], w[2], w[3]), four(w[4], w[5], w[6], w[7]));
+    }
 };
 
 // The larger magnitude, NaN if either is: magnitudes are compared as whole numbers, in
@@ -60,71 +82,83 @@ __device__ __forceinline__ float wave_amax(float m) {
     for (int o = 32; o > 0; o >>= 1) m = amax2(m, __shfl_xor(m, o));
     return m;
 }
-
-// 8 elements from p on, those past cnt zero
+// The largest magnitude of vectors of 8, two 16-bit ones at a time
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, long cnt, float (&v)[8]) {
-    const auto x = gf::Piece<8, T>::load(p, cnt);
+struct Amax {
+    typedef typename gf::Piece<8, T>::vec Vec;
+    typedef __attribute__((__vector_size__(8 * sizeof(uint16_t)))) uint16_t U8;
+    U8 m{};
+    __device__ __forceinline__ void add(Vec x) {
+        const U8 b = __builtin_bit_cast(U8, x) & (uint16_t)0x7FFF;
+        m = __builtin_elementwise_max(m, b);
+    }
+    __device__ __forceinline__ float get() const {
+        uint16_t t = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
-}
-
-__device__ __forceinline__ uint2 pack8(const Quantizer& q, const float (&v)[8]) {
-    uint32_t w[2] = {0, 0};
+        for (int e = 0; e < 8; ++e) t = t > m[e] ? t : m[e];
+        return (float)__builtin_bit_cast(T, t);
+    }
+};
+template <>
+struct Amax<float> {
+    typedef gf::Piece<8, float>::vec Vec;
+    float m = 0.f;
+    __device__ __forceinline__ void add(Vec x) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e / 4] |= ((uint32_t)q(v[e]) & 0xFFu) << (8 * (e & 3));
-    return make_uint2(w[0], w[1]);
-}
+        for (int e = 0; e < 8; ++e) m = amax2(m, x[e]);
+    }
+    __device__ __forceinline__ float get() const { return m; }
+};
 
 // One wave quantises a row: q gets kp bytes (zero behind k).  Rows of up to 64 * 8 * HOLD
 // elements stay in registers between the maximum and the quotients, longer ones are read
 // again.  Returns the scale.
 template <typename T, int HOLD>
 __device__ __forceinline__ float quantize_row(const T* x, long k, long kp, uint8_t* q) {
+    typedef gf::Piece<8, T> P8;
     const int l = lane_id();
-    float v[HOLD][8];
-    float m = 0.f;
+    typename P8::vec v[HOLD];
+    Amax<T> m;
     for (long c0 = 0; c0 < kp; c0 += 512 * HOLD) {
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
             const long c = c0 + 8 * (l + 64 * i);
-            if (c < k) {
-                load8<T>(x + c, k - c, v[i]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) m = amax2(m, v[i][e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-            }
+            v[i] = typename P8::vec{};
+            if (c < k) v[i] = P8::load(x + c, k - c);
         }
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i) m.add(v[i]);
     }
-    const float s = scale_of(wave_amax(m));
+    const float s = scale_of(wave_amax(m.get()));
     const Quantizer qz(s);
+    auto put = [&](long c, typename P8::vec x) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (float)x[e];
+        *reinterpret_cast<uint2*>(q + c) = qz.pack(f);
+    };
     if (kp <= 512 * HOLD) {
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
             const long c = 8 * (l + 64 * i);
-            if (c < kp) *reinterpret_cast<uint2*>(q + c) = pack8(qz, v[i]);
+            if (c < kp) put(c, v[i]);
         }
     } else {
-        for (long c = 8 * l; c < kp; c += 512) {
-            float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (c < k) load8<T>(x + c, k - c, y);
-            *reinterpret_cast<uint2*>(q + c) = pack8(qz, y);
-        }
+        for (long c = 8 * l; c < kp; c += 512)
+            put(c, c < k ? P8::load(x + c, k - c) : typename P8::vec{});
     }
     return s;
 }
 
 // Four rows to a workgroup, a wave each.  Bound by memory.
-template <typename T>
+template <typename T, int HOLD>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ldx,
                                                             long m, long k, long kp,
                                                             uint8_t* __restrict__ q,
                                                             float* __restrict__ scales) {
     const long row = (long)blockIdx.x * 4 + wave_id();
     if (row >= m) return;
-    const float s = quantize_row<T, 8>(x + row * ldx, k, kp, q + row * kp);
+    const float s = quantize_row<T, HOLD>(x + row * ldx, k, kp, q + row * kp);
     if (lane_id() == 0) scales[row] = s;
 }
 
@@ -192,14 +226,11 @@ __device__ __forceinline__ void finish(const Out<T>& o, long m, long n, long cnt
     typedef gf::Piece<W, T, RAGGED> P;
     typedef gf::Piece<W, float, RAGGED> F;
     const typename F::vec sw = F::load(o.sw + n, cnt);
+    typename P::vec b{};
+    if (o.bias) b = P::load(o.bias + n, cnt);
     float v[W];
 #pragma unroll
-    for (int e = 0; e < W; ++e) v[e] = (float)acc[e] * sx * sw[e];
-    if (o.bias) {
-        const typename P::vec b = P::load(o.bias + n, cnt);
-#pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += (float)b[e];
-    }
+    for (int e = 0; e < W; ++e) v[e] = fmaf((float)acc[e] * sx, sw[e], (float)b[e]);
     if (o.gelu) {
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] = gelu::gelu_f<true>(v[e]);
@@ -300,6 +331,60 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
         finish<4, T, true>(o, m, n, N - n, v, FUSED ? sc[m] : xs[m]);
     }
 }
+
+// The same for a lane of tile_kernel, whose 8 columns stay the same over its rows: their
+// scales and bias are read once, and four rows' scales and residuals ahead of their use
+// (read where they are used, each waited behind its branch).
+template <typename T, bool RAGGED>
+struct Columns {
+    typedef gf::Piece<8, T, RAGGED> P;
+    typedef gf::Piece<8, float, RAGGED> F;
+    long n, cnt;
+    float sw[8], bias[8];
+    __device__ __forceinline__ Columns(const Out<T>& o, long n, long N) : n(n), cnt(N - n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sw[e] = bias[e] = 0.f;
+        if (cnt <= 0) return;
+        const typename F::vec s = F::load(o.sw + n, cnt);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sw[e] = s[e];
+        if (!o.bias) return;
+        const typename P::vec b = P::load(o.bias + n, cnt);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bias[e] = (float)b[e];
+    }
+    struct Rows {  // rows m0, m0 + 8, + 16, + 24
+        float sx[4];
+        typename P::vec res[4];
+        __device__ __forceinline__ void load(const Out<T>& o, const Columns& c,
+                                             const float* __restrict__ xs, long m0, long M) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) sx[s] = xs[min(m0 + 8 * s, M - 1)];
+            if (!o.residual || c.cnt <= 0) return;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                res[s] = P::load(o.residual + min(m0 + 8 * s, M - 1) * o.ldr + c.n, c.cnt);
+        }
+    };
+    __device__ __forceinline__ void finish(const Out<T>& o, long m, const int (&acc)[8],
+                                           const Rows& r, int s) const {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf((float)acc[e] * r.sx[s], sw[e], bias[e]);
+        if (o.gelu) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = gelu::gelu_f<true>(v[e]);
+        }
+        if (o.residual) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += (float)r.res[s][e];
+        }
+        typename P::vec y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (T)v[e];
+        P::store(o.y + m * o.ldy + n, y, cnt);
+    }
+};
 
 // --- many rows ------------------------------------------------------------------------
 // The tiles of gemm_fast.hpp with both operands k-contiguous and two 8-bit integers in the
@@ -409,11 +494,14 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
         {
             const int le = mf::tid_in(~(int)it) & 63;
             char* wp = smem + 2 * (buf ^ 1) * TILE + (4096 * TNI) * w;
-            constexpr int WC = 32 * TNI, NP = WC / 16;
-            const long mw = m0 + wm, nw = n0 + wn;
+            const Columns<T, RAGGED> col(o, n0 + wn + 8 * (le & 7), N);
+            // (fp32 residuals and ragged ones leave no registers to read a pass ahead in)
+            constexpr bool AHEAD = sizeof(T) == 2 && !RAGGED;
+            typename Columns<T, RAGGED>::Rows rows[2];
+            if (AHEAD && m0 + wm < M) rows[0].load(o, col, xs, m0 + wm + (le >> 3), M);
 #pragma unroll
             for (int j = 0; j < TMJ; ++j) {
-                const long r0 = mw + 32 * j;
+                const long r0 = (long)m0 + wm + 32 * j;
                 if (r0 >= M) break;
 #pragma unroll
                 for (int i = 0; i < TNI; ++i)
@@ -423,16 +511,19 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
                             wp + gf::ep_off<TNI>(le & 31, 32 * i + 8 * q + 4 * (le >> 5))) =
                             int4v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                                   acc[i][j][4 * q + 3]};
+                // the next pass's scales and residual are on their way while this one is
+                // finished: its accumulators have left their registers
+                if (AHEAD && j + 1 < TMJ && r0 + 32 < M)
+                    rows[(j + 1) & 1].load(o, col, xs, r0 + 32 + (le >> 3), M);
+                if (!AHEAD) rows[j & 1].load(o, col, xs, r0 + (le >> 3), M);
 #pragma unroll
-                for (int s = 0; s < NP; ++s) {
-                    const int p = 64 * s + le, row = p / (WC / 8), c8 = p % (WC / 8);
-                    const long m = r0 + row, n = nw + 8 * c8;
-                    const int4v v0 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, 8 * c8));
-                    const int4v v1 =
-                        *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, 8 * c8 + 4));
-                    if (m >= M || n >= N) continue;
+                for (int s = 0; s < 4; ++s) {
+                    const int row = 8 * s + (le >> 3), c = 8 * (le & 7);
+                    const int4v v0 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, c));
+                    const int4v v1 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, c + 4));
                     const int v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                    finish<8, T, RAGGED>(o, m, n, N - n, v, xs[m]);
+                    if (r0 + row < M && col.cnt > 0)
+                        col.finish(o, r0 + row, v, rows[j & 1], s);
                 }
             }
         }
