@@ -20,7 +20,8 @@
 // (many equal logits) the best are taken out one by one.
 //
 // join_kernel: a workgroup per text joins the slices' sums (64 bits), and does the same
-// with the slices' best, whose values it forms in 64 bits.  -inf is never a candidate:
+// with the slices' best, whose values it forms in 64 bits.  The bound comes from the slices'
+// lists' first entries alone: hardly more than n entries reach their n-th largest.  -inf is never a candidate:
 // where fewer than `select` finite values exist, the rest are the lowest pairs (k, v)
 // that are not among them, which is what the order above gives.
 #include <hip/hip_runtime.h>
@@ -70,8 +71,9 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int n) {
     return got;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp_diff(float d) {  // e^d
-    return __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+    return __builtin_amdgcn_exp2f(d * kLog2e);
 }
 
 // A row's vectors start at cache lines: element i of the row is at i + shift, shift its
@@ -119,13 +121,22 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
         vm[i] = fmaxf(vm[i], -INFINITY) + 0.f;  // no NaN, and -0 is 0
         m = fmaxf(m, vm[i]);
     }
-    // a thread without a logit above -inf: 0, or NaN from a NaN
+    // The sum of 2^(z log2 e - c), c = m log2 e rounded: one fused operation and one exponential
+    // an element; what the rounding of c left out is taken back at the end, so that only
+    // z - m meets the constant's own error.  A thread without a logit above -inf: 0, or NaN
+    // from a NaN.  Where m log2 e would overflow (masks of the type's lowest value), floats are
+    // so far apart that any positive factor gives 1 for z = m and 0 below.
     const float m0 = m == -INFINITY ? 0.f : m;
+    const float f = fabsf(m0) > 0x1p126f ? 0x1p-64f : kLog2e, c0 = m0 * f;
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+        asm volatile("" : "+v"(x[i]));  // converted again: the fp32 values take four times the registers
 #pragma unroll
-        for (int j = 0; j < N; ++j) s += exp_diff(to_f(x[i][j]) - m0);
+        for (int j = 0; j < N; ++j)
+            s += __builtin_amdgcn_exp2f(fmaf(to_f(x[i][j]), f, -c0));
+    }
+    s *= __builtin_amdgcn_exp2f(-fmaf(m0, f, -c0));
     const uint32_t bound = wave_bound<sizeof(T) == 2 && !__is_same(T, f16) ? 16 : 12>(ordered(m), n);
     float M = m;
 #pragma unroll
@@ -192,6 +203,7 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
         for (int i = threadIdx.x; i < c; i += NT) {
             const uint64_t mine = place[i];
             int rank = 0;
+#pragma unroll 4
             for (int k = 0; k < c; ++k) rank += place[k] > mine;
             if (rank < n) write(rank, mine);
         }
@@ -237,34 +249,31 @@ __device__ __forceinline__ bool better(const Best& a, const Best& b) {
     return a.token < b.token;
 }
 
+// H entries of a thread are held; more than H * NT are read twice.
+template <int H>
 __global__ void __launch_bounds__(NT)
 join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, int slices,
             const float* __restrict__ scores, const uint8_t* __restrict__ finished, int V,
             int beams, int n, int end_token, int keep_slots, float* __restrict__ out_scores,
             int* __restrict__ out_parents, int* __restrict__ out_tokens,
             uint8_t* __restrict__ out_finished) {
-    constexpr int H = 8;  // entries of a thread in flight
     __shared__ double offset[kMaxBeams];  // score - log sum exp; -inf: offers nothing
     __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
     __shared__ Best place[kPlaces];
     __shared__ Best res[kMaxSelect];
     __shared__ Best wbest[NWV];
-    __shared__ uint32_t wb[NWV];
     __shared__ int count;
     const long text = blockIdx.x, row0 = text * beams;
     const int per = slices * n, total = beams * per;
     const Cand* mine = cands + row0 * per;
+    // on their way while the sums are joined (what beams that were not read left there is
+    // not looked at)
     Cand c[H];
-    // H entries from `base` on, the threads' own; what beams that were not read left there
-    // is not looked at
-    auto fetch = [&](int base) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-            const int e = base + (int)threadIdx.x + i * NT;
-            c[i] = e < total ? mine[e] : Cand{0.f, -1};
-        }
-    };
-    fetch(0);
+    for (int i = 0; i < H; ++i) {
+        const int e = (int)threadIdx.x + i * NT;
+        c[i] = e < total ? mine[e] : Cand{0.f, -1};
+    }
     if (threadIdx.x == 0) count = 0;
     // 16 lanes to a beam
     for (int k = threadIdx.x / 16; k < beams; k += NT / 16) {
@@ -275,24 +284,17 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         if (ok && !fin) {
             const float2* st = stats + (row0 + k) * slices;
             float M = -INFINITY;
+            for (int i = l; i < slices; i += 16) M = fmaxf(M, st[i].x);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 16));
             double s = 0.0;
-            // joined as they come: a slice without a logit above -inf has 0, or NaN from a NaN
             for (int i = l; i < slices; i += 16) {
                 const float2 a = st[i];
-                const float W = fmaxf(M, a.x);
-                s = (M < W ? s * exp((double)M - (double)W) : s) +
-                    (a.x < W ? (double)a.y * exp((double)a.x - (double)W) : (double)a.y);
-                M = W;
+                // a slice without a logit above -inf: 0, or NaN from a NaN
+                s += a.x < M ? (double)a.y * (double)exp_diff(a.x - M) : (double)a.y;
             }
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) {
-                const float Mo = __shfl_xor(M, o, 16);
-                const double so = __shfl_xor(s, o, 16);
-                const float W = fmaxf(M, Mo);
-                s = (M < W ? s * exp((double)M - (double)W) : s) +
-                    (Mo < W ? so * exp((double)Mo - (double)W) : so);
-                M = W;
-            }
+            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
             lse = (double)M + log(s);
         }
         if (l == 0) {
@@ -302,58 +304,57 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         }
     }
     __syncthreads();
-    // entry e's value from its logit; a finished beam has one entry
-    auto value_of = [&](int e, const Cand& x) {
+    // entry e from what the slice left; a finished beam has one entry
+    auto best_of = [&](int e, const Cand& x) {
         Best b{-(double)INFINITY, 0, 0};
         if (e >= total) return b;
         b.beam = (int)((unsigned)e / (unsigned)per);
         if (state[b.beam] == 0) {
-            if (x.token >= 0) {
-                b.value = (double)x.z + offset[b.beam];
-                b.token = x.token;
-            }
+            if (x.token >= 0) b.value = (double)x.z + offset[b.beam];
+            b.token = x.token;
         } else if (state[b.beam] == 1 && e == b.beam * per) {
             b.value = offset[b.beam];
             b.token = end_token;
         }
         return b;
     };
-    const bool held = total <= H * NT;
-    uint64_t top = 0;
-    for (int base = 0; base < total; base += H * NT) {
-        if (base) fetch(base);
+    // 0: not a candidate
+    auto key_of = [](double v) {
+        return v > -(double)INFINITY ? (uint32_t)(ordered(v + 0.0) >> 32) : 0u;
+    };
+    uint32_t key[H];
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-            const Best b = value_of(base + (int)threadIdx.x + i * NT, c[i]);
-            const uint64_t o = ordered(b.value + 0.0);
-            if (b.value > -(double)INFINITY && o > top) top = o;
-        }
-    }
-    const uint32_t bound = wave_bound<4>((uint32_t)(top >> 32), n);
-    if (lane_id() == 0) wb[wave_id()] = bound;
-    __syncthreads();
-    uint32_t least = wb[0];
+    for (int i = 0; i < H; ++i) key[i] = key_of(best_of((int)threadIdx.x + i * NT, c[i]).value);
+    // The bound, in every wave by itself: each lane takes the heads of some slices' lists, which
+    // are their largest.
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int j = lane_id(); j < beams * slices; j += kWave)
+        top = max(top, key_of(best_of(j * n, mine[j * n]).value));
+    const uint32_t least = max(wave_bound<4>(top, n), 1u);
+    auto take = [&](int e) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kPlaces) place[at] = best_of(e, mine[e]);
+    };
+    unsigned pass = 0;
 #pragma unroll
-    for (int k = 1; k < NWV; ++k) least = max(least, wb[k]);
-    for (int base = 0; base < total; base += H * NT) {
-        if (!held) fetch(base);
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-            const Best b = value_of(base + (int)threadIdx.x + i * NT, c[i]);
-            if (!(b.value > -(double)INFINITY) ||
-                (uint32_t)(ordered(b.value + 0.0) >> 32) < least)
-                continue;
-            const int at = atomicAdd(&count, 1);
-            if (at < kPlaces) place[at] = b;
-        }
-    }
+    for (int i = 0; i < H; ++i) pass |= (unsigned)(key[i] >= least) << i;
+    for (; pass; pass &= pass - 1) take((int)threadIdx.x + (__ffs(pass) - 1) * NT);
+    for (int e = threadIdx.x + H * NT; e < total; e += NT)
+        if (key_of(best_of(e, mine[e]).value) >= least) take(e);
     __syncthreads();
     const int found = count;
     if (found <= kPlaces) {
         for (int i = threadIdx.x; i < found; i += NT) {
             const Best b = place[i];
             int rank = 0;
-            for (int k = 0; k < found; ++k) rank += better(place[k], b);
+            // without branches, so that the reads need not wait for each other
+#pragma unroll 4
+            for (int k = 0; k < found; ++k) {
+                const Best x = place[k];
+                const bool before = (x.beam < b.beam) | ((x.beam == b.beam) & (x.token < b.token));
+                rank += (x.value > b.value) | ((x.value == b.value) & before);
+            }
             if (rank < n) res[rank] = b;
         }
     } else {
@@ -362,7 +363,7 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         for (int r = 0; r < n; ++r) {
             Best b{-(double)INFINITY, beams, 0};
             for (int e = threadIdx.x; e < total; e += NT) {
-                const Best x = value_of(e, mine[e]);
+                const Best x = best_of(e, mine[e]);
                 if (x.value > -(double)INFINITY && better(last, x) && better(x, b)) b = x;
             }
 #pragma unroll
@@ -382,39 +383,42 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         }
     }
     __syncthreads();
+    if (wave_id() != 0) return;
+    const int r = lane_id();
     // fewer finite values than asked for: the lowest pairs that are not among them
-    if (threadIdx.x == 0 && found < n) {
-        int beam = 0, token = 0;
-        for (int r = found; r < n;) {
-            bool taken = false;
-            for (int k = 0; k < found; ++k) taken |= res[k].beam == beam && res[k].token == token;
-            if (!taken) res[r++] = Best{-(double)INFINITY, beam, token};
-            if (++token == V) token = 0, ++beam;
+    if (found < n) {
+        if (r == 0) {
+            int beam = 0, token = 0;
+            for (int to = found; to < n;) {
+                bool taken = false;
+                for (int k = 0; k < found; ++k)
+                    taken |= res[k].beam == beam && res[k].token == token;
+                if (!taken) res[to++] = Best{-(double)INFINITY, beam, token};
+                if (++token == V) token = 0, ++beam;
+            }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    __syncthreads();
-    if (threadIdx.x >= n) return;
-    const int r = threadIdx.x;
-    const Best b = res[r];
+    const Best b = res[r < n ? r : n - 1];
     int to = r;
     if (keep_slots) {
         // the first child of a beam takes that beam's slot, the others the free ones in order
         uint64_t used = 0;
-        int rest = 0;
         bool first = true;
         for (int k = 0; k < n; ++k) {
-            const uint64_t bit = 1ull << res[k].beam;
-            if (k < r && (used & bit)) ++rest;
-            if (k == r) first = !(used & bit);
-            used |= bit;
+            const int other = __builtin_amdgcn_readlane(b.beam, k);
+            used |= 1ull << other;
+            if (k < r && other == b.beam) first = false;
         }
+        const uint64_t late = __ballot(!first && r < n);
         to = b.beam;
         if (!first) {
             uint64_t open = ~used;
-            for (int k = 0; k < rest; ++k) open &= open - 1;
+            for (int k = __popcll(late & ((1ull << r) - 1)); k > 0; --k) open &= open - 1;
             to = __ffsll((unsigned long long)open) - 1;
         }
     }
+    if (r >= n) return;
     const long at = text * n + to;
     out_scores[at] = (float)b.value;
     out_parents[at] = b.beam;
@@ -430,7 +434,7 @@ static size_t dtype_size(int d) {
 // Vectors a thread: as many as leave the chip four workgroups for each of its compute units.
 static int vectors(size_t rows, size_t vocab, size_t size) {
     const size_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    for (int v = 4; v > 1; v /= 2)
+    for (int v = 8; v > 1; v /= 2)
         if (rows * ((vocab * size + NT * 16 * v - 1) / (NT * 16 * v)) >= 4 * cus) return v;
     return 1;
 }
@@ -462,7 +466,8 @@ static void launch(const void* logits, const float* scores, const uint8_t* finis
                 stats + s0, cands + s0 * n)
         if (vpt == 1) BS_SLICE(1);
         else if (vpt == 2) BS_SLICE(2);
-        else BS_SLICE(4);
+        else if (vpt == 4) BS_SLICE(4);
+        else BS_SLICE(8);
 #undef BS_SLICE
     }
 }
@@ -523,9 +528,13 @@ extern "C" int beam_select_hip(const void* logits, const float* scores, const ui
                           select, vpt, slices, stream);
     EFLA_CHECK(hipPeekAtLastError());
     const float2* stats = (const float2*)ws;
-    EFLA_LAUNCH("beam_join", bs::join_kernel, dim3((unsigned)batch), dim3(bs::NT), stream, stats,
-                (const bs::Cand*)(stats + rows * slices), (int)slices, scores, finished,
-                (int)vocab_size, (int)beams, (int)select, (int)end_token, keep_slots, out_scores,
-                out_parents, out_tokens, out_finished);
+#define BS_JOIN(H)                                                                               \
+    EFLA_LAUNCH("beam_join", bs::join_kernel<H>, dim3((unsigned)batch), dim3(bs::NT), stream, stats, \
+                (const bs::Cand*)(stats + rows * slices), (int)slices, scores, finished,           \
+                (int)vocab_size, (int)beams, (int)select, (int)end_token, keep_slots, out_scores, \
+                out_parents, out_tokens, out_finished)
+    if (beams * slices * select <= bs::NT) BS_JOIN(1);
+    else BS_JOIN(8);
+#undef BS_JOIN
     return (int)hipPeekAtLastError();
 }
