@@ -36,7 +36,7 @@ namespace bs {
 
 constexpr int NT = 256, NWV = NT / kWave;
 constexpr int kMaxSelect = 64, kMaxBeams = 64;
-constexpr int kPlaces = 1024;  // candidates that LDS holds
+constexpr int kPlaces = 512;   // candidates that LDS holds
 constexpr int kVectors = 512;  // and 16-byte vectors that have some
 
 // What is left of a slice: one of its best logits; none: token -1.
@@ -71,6 +71,47 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int n) {
     return got;
 }
 
+// Over the wave, in every lane: within rows of 16 by lane permutations, then across them.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xF,
+                                                               0xF, true));
+}
+template <typename Op>
+__device__ __forceinline__ float wave_join(float x, Op op) {
+    x = op(x, dpp<0xB1>(x));   // quad_perm [1, 0, 3, 2]
+    x = op(x, dpp<0x4E>(x));   // quad_perm [2, 3, 0, 1]
+    x = op(x, dpp<0x141>(x));  // row_half_mirror
+    x = op(x, dpp<0x140>(x));  // row_mirror
+    x = op(x, __shfl_xor(x, 16));
+    return op(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float wave_max(float x) {
+    return wave_join(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    return wave_join(x, [](float a, float b) { return a + b; });
+}
+
+// The largest of a vector's floats, -inf where it has none (NaN is passed over).
+template <typename T, typename Vec>
+__device__ __forceinline__ float vec_max(Vec x) {
+    if constexpr (__is_same(T, f16)) {  // two at a time
+        typedef __attribute__((__vector_size__(4))) f16 Pair;
+        struct Pairs {
+            Pair p[4];
+        };
+        const Pairs q = __builtin_bit_cast(Pairs, x);
+        Pair m = __builtin_elementwise_max(__builtin_elementwise_max(q.p[0], q.p[1]),
+                                           __builtin_elementwise_max(q.p[2], q.p[3]));
+        return fmaxf((float)m[0], (float)m[1]);
+    }
+    constexpr int N = 16 / sizeof(T);
+    float m = to_f(x[0]);
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = fmaxf(m, to_f(x[j]));
+    return m;
+}
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp_diff(float d) {  // e^d
     return __builtin_amdgcn_exp2f(d * kLog2e);
@@ -88,8 +129,7 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
     __shared__ Vec piece[kVectors];
     __shared__ int piece_at[kVectors];  // its first token
     __shared__ uint64_t place[kPlaces];
-    __shared__ float wm[NWV], ws[NWV];
-    __shared__ uint32_t wb[NWV];
+    __shared__ float wm[NWV], ws[NWV], lanes[NT];
     __shared__ uint64_t best[NWV];
     __shared__ int pieces, count;
     const long row = blockIdx.y;
@@ -101,23 +141,27 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
     if (threadIdx.x == 0) pieces = count = 0;
 
     Vec x[VPT];
+    if (v0 >= 0 && v0 + L <= V) {  // the whole slice lies in the row
+        const Vec* q = reinterpret_cast<const Vec*>(p + v0);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const long v = v0 + (long)(threadIdx.x + i * NT) * N;
-        if (v >= 0 && v + N <= V) {
-            x[i] = *reinterpret_cast<const Vec*>(p + v);
-        } else {
+        for (int i = 0; i < VPT; ++i) x[i] = q[threadIdx.x + i * NT];
+    } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                x[i][j] = v + j >= 0 && v + j < V ? p[v + j] : (T)-INFINITY;
+        for (int i = 0; i < VPT; ++i) {
+            const long v = v0 + (long)(threadIdx.x + i * NT) * N;
+            if (v >= 0 && v + N <= V) {
+                x[i] = *reinterpret_cast<const Vec*>(p + v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    x[i][j] = v + j >= 0 && v + j < V ? p[v + j] : (T)-INFINITY;
+            }
         }
     }
     float vm[VPT], m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        vm[i] = to_f(x[i][0]);
-#pragma unroll
-        for (int j = 1; j < N; ++j) vm[i] = fmaxf(vm[i], to_f(x[i][j]));
+        vm[i] = vec_max<T>(x[i]);
         vm[i] = fmaxf(vm[i], -INFINITY) + 0.f;  // no NaN, and -0 is 0
         m = fmaxf(m, vm[i]);
     }
@@ -137,23 +181,19 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
             s += __builtin_amdgcn_exp2f(fmaf(to_f(x[i][j]), f, -c0));
     }
     s *= __builtin_amdgcn_exp2f(-fmaf(m0, f, -c0));
-    const uint32_t bound = wave_bound<sizeof(T) == 2 && !__is_same(T, f16) ? 16 : 12>(ordered(m), n);
-    float M = m;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const float M0 = M == -INFINITY ? 0.f : M;
-    s *= exp_diff(fminf(m0 - M0, 0.f));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    const float M = wave_max(m), M0 = M == -INFINITY ? 0.f : M;
+    s = wave_sum(s * exp_diff(fminf(m0 - M0, 0.f)));
     if (lane_id() == 0) {
         wm[wave_id()] = M;
         ws[wave_id()] = s;
-        wb[wave_id()] = bound;
     }
+    lanes[threadIdx.x] = m;
     __syncthreads();
-    uint32_t least = wb[0];
+    float group = lanes[lane_id()];
 #pragma unroll
-    for (int k = 1; k < NWV; ++k) least = max(least, wb[k]);
+    for (int k = 1; k < NWV; ++k) group = fmaxf(group, lanes[lane_id() + k * kWave]);
+    const uint32_t least =
+        wave_bound<sizeof(T) == 2 && !__is_same(T, f16) ? 16 : 12>(ordered(group), n);
     // vectors that reach the bound
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
