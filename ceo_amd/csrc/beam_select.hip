@@ -289,9 +289,13 @@ __device__ __forceinline__ bool better(const Best& a, const Best& b) {
     return a.token < b.token;
 }
 
-// H entries of a thread are held; more than H * NT are read twice.
-template <int H>
-__global__ void __launch_bounds__(NT)
+constexpr int kHeads = 2;
+
+// An entry a thread is held, NTJ of them; more are read twice.  (Eight entries a thread: 17 KB
+// of code that a workgroup runs through once, 8.5 us for 800 entries of each of 16 texts; 1024
+// threads 6.7.)
+template <int NTJ>
+__global__ void __launch_bounds__(NTJ)
 join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, int slices,
             const float* __restrict__ scores, const uint8_t* __restrict__ finished, int V,
             int beams, int n, int end_token, int keep_slots, float* __restrict__ out_scores,
@@ -301,42 +305,42 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
     __shared__ Best place[kPlaces];
     __shared__ Best res[kMaxSelect];
-    __shared__ Best wbest[NWV];
+    __shared__ Best wbest[NTJ / kWave];
     __shared__ int count;
     const long text = blockIdx.x, row0 = text * beams;
     const int per = slices * n, total = beams * per;
     const Cand* mine = cands + row0 * per;
-    // on their way while the sums are joined (what beams that were not read left there is
-    // not looked at)
-    Cand c[H];
+    // On their way while the sums are joined: an entry a thread, and the heads of a lane's
+    // first lists (what beams that were not read left there is not looked at).
+    const int e0 = (int)threadIdx.x;
+    const Cand held = e0 < total ? mine[e0] : Cand{0.f, -1};
+    Cand head[kHeads];
 #pragma unroll
-    for (int i = 0; i < H; ++i) {
-        const int e = (int)threadIdx.x + i * NT;
-        c[i] = e < total ? mine[e] : Cand{0.f, -1};
+    for (int i = 0; i < kHeads; ++i) {
+        const int j = lane_id() + i * kWave;
+        head[i] = j < beams * slices ? mine[j * n] : Cand{0.f, -1};
     }
     if (threadIdx.x == 0) count = 0;
     // 16 lanes to a beam
-    for (int k = threadIdx.x / 16; k < beams; k += NT / 16) {
+    for (int k = threadIdx.x / 16; k < beams; k += NTJ / 16) {
         const int l = threadIdx.x % 16;
+        const float2* st = stats + (row0 + k) * slices;
+        float2 a = l < slices ? st[l] : make_float2(-INFINITY, 0.f);
         const float score = scores[row0 + k];
         const bool fin = finished && finished[row0 + k], ok = fabsf(score) < INFINITY;
-        double lse = 0.0;
-        if (ok && !fin) {
-            const float2* st = stats + (row0 + k) * slices;
-            float M = -INFINITY;
-            for (int i = l; i < slices; i += 16) M = fmaxf(M, st[i].x);
+        float M = a.x;
+        for (int i = l + 16; i < slices; i += 16) M = fmaxf(M, st[i].x);
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 16));
-            double s = 0.0;
-            for (int i = l; i < slices; i += 16) {
-                const float2 a = st[i];
-                // a slice without a logit above -inf: 0, or NaN from a NaN
-                s += a.x < M ? (double)a.y * (double)exp_diff(a.x - M) : (double)a.y;
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
-            lse = (double)M + log(s);
+        for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 16));
+        double s = 0.0;
+        for (int i = l; i < slices; i += 16) {
+            if (i != l) a = st[i];
+            // a slice without a logit above -inf: 0, or NaN from a NaN
+            s += a.x < M ? (double)a.y * (double)exp_diff(a.x - M) : (double)a.y;
         }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
+        const double lse = fin ? 0.0 : (double)M + log(s);
         if (l == 0) {
             const bool live = ok && fabs(lse) < (double)INFINITY;
             state[k] = !live ? 2 : fin ? 1 : 0;
@@ -362,30 +366,29 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     auto key_of = [](double v) {
         return v > -(double)INFINITY ? (uint32_t)(ordered(v + 0.0) >> 32) : 0u;
     };
-    uint32_t key[H];
-#pragma unroll
-    for (int i = 0; i < H; ++i) key[i] = key_of(best_of((int)threadIdx.x + i * NT, c[i]).value);
+    const Best first = best_of(e0, held);
     // The bound, in every wave by itself: each lane takes the heads of some slices' lists, which
     // are their largest.
     uint32_t top = 0;
-#pragma unroll 4
-    for (int j = lane_id(); j < beams * slices; j += kWave)
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+        top = max(top, key_of(best_of((lane_id() + i * kWave) * n, head[i]).value));
+    for (int j = lane_id() + kHeads * kWave; j < beams * slices; j += kWave)
         top = max(top, key_of(best_of(j * n, mine[j * n]).value));
     const uint32_t least = max(wave_bound<4>(top, n), 1u);
-    auto take = [&](int e) {
+    auto take = [&](const Best& b) {
         const int at = atomicAdd(&count, 1);
-        if (at < kPlaces) place[at] = best_of(e, mine[e]);
+        if (at < kPlaces) place[at] = b;
     };
-    unsigned pass = 0;
-#pragma unroll
-    for (int i = 0; i < H; ++i) pass |= (unsigned)(key[i] >= least) << i;
-    for (; pass; pass &= pass - 1) take((int)threadIdx.x + (__ffs(pass) - 1) * NT);
-    for (int e = threadIdx.x + H * NT; e < total; e += NT)
-        if (key_of(best_of(e, mine[e]).value) >= least) take(e);
+    if (key_of(first.value) >= least) take(first);
+    for (int e = e0 + NTJ; e < total; e += NTJ) {
+        const Best b = best_of(e, mine[e]);
+        if (key_of(b.value) >= least) take(b);
+    }
     __syncthreads();
     const int found = count;
     if (found <= kPlaces) {
-        for (int i = threadIdx.x; i < found; i += NT) {
+        for (int i = threadIdx.x; i < found; i += NTJ) {
             const Best b = place[i];
             int rank = 0;
             // without branches, so that the reads need not wait for each other
@@ -402,7 +405,7 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         Best last{(double)INFINITY, -1, -1};
         for (int r = 0; r < n; ++r) {
             Best b{-(double)INFINITY, beams, 0};
-            for (int e = threadIdx.x; e < total; e += NT) {
+            for (int e = threadIdx.x; e < total; e += NTJ) {
                 const Best x = best_of(e, mine[e]);
                 if (x.value > -(double)INFINITY && better(last, x) && better(x, b)) b = x;
             }
@@ -417,7 +420,7 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
             __syncthreads();
             last = wbest[0];
 #pragma unroll
-            for (int k = 1; k < NWV; ++k)
+            for (int k = 1; k < NTJ / kWave; ++k)
                 if (better(wbest[k], last)) last = wbest[k];
             if (threadIdx.x == 0) res[r] = last;
         }
@@ -568,13 +571,13 @@ extern "C" int beam_select_hip(const void* logits, const float* scores, const ui
                           select, vpt, slices, stream);
     EFLA_CHECK(hipPeekAtLastError());
     const float2* stats = (const float2*)ws;
-#define BS_JOIN(H)                                                                               \
-    EFLA_LAUNCH("beam_join", bs::join_kernel<H>, dim3((unsigned)batch), dim3(bs::NT), stream, stats, \
-                (const bs::Cand*)(stats + rows * slices), (int)slices, scores, finished,           \
+#define BS_JOIN(NTJ)                                                                             \
+    EFLA_LAUNCH("beam_join", bs::join_kernel<NTJ>, dim3((unsigned)batch), dim3(NTJ), stream, stats, \
+                (const bs::Cand*)(stats + rows * slices), (int)slices, scores, finished,          \
                 (int)vocab_size, (int)beams, (int)select, (int)end_token, keep_slots, out_scores, \
                 out_parents, out_tokens, out_finished)
-    if (beams * slices * select <= bs::NT) BS_JOIN(1);
-    else BS_JOIN(8);
+    if (beams * slices * select <= 256) BS_JOIN(256);
+    else BS_JOIN(1024);
 #undef BS_JOIN
     return (int)hipPeekAtLastError();
 }
