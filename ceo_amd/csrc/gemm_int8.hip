@@ -18,32 +18,40 @@ static size_t dtype_size(int d) {
 }
 static size_t scales_bytes(size_t n) { return (size_t)up_to((long)(n * sizeof(float)), kLine); }
 
-// Rows up to which the weights are streamed (few_kernel).
-constexpr size_t kFewRows = 64;
-// Tokens that a workgroup quantises into LDS itself (64 KiB with their scales).
-constexpr size_t kFusedBytes = 63 << 10;
+// Whether the weights are streamed past few tokens (few_kernel) or go through tiles.  Up to 64
+// tokens, but for wide outputs, whose tiles fill half the chip, 32: a wave reads all tokens
+// for its 16 channels.  Measured (few / 128-tiles, us; 48 tokens, k x n): 1024 x 4096 8.8 /
+// 10.0, 4096 x 4096 19.4 / 24.3, 1024 x 32000 21.5 / 12.4, 1024 x 128000 70 / 38.
+static bool few(long m, long n) {
+    const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    return m <= 32 || (m <= 64 && (n + 127) / 128 < cus / 2);
+}
 
-template <typename T, int MT>
+// Fewer rows than this are quantised by a workgroup each, more by a wave.
+constexpr long kWaveRows = 2048;
+
+// Whether few_kernel quantises the tokens itself: a second launch is longer than what it takes
+// every workgroup.  (Registers: a lane holds 32 values of its row, 1024 threads of fp32 too many.)
+static bool fused(size_t m, size_t kp, size_t size) {
+    return m <= (size == 2 ? 32 : 16) && kp <= 1024;
+}
+
+template <typename T, int MT, int HOLD>
 static void few_launch(const T* x, long ldx, const uint8_t* xq, const float* xs, const uint8_t* wq,
                        long m, long n, long k, long kp, const Out<T>& o, hipStream_t st) {
+    constexpr long NW = kFewWaves<MT, HOLD>;
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const long tiles = (n + 15) / 16;
-    // waves that split k: until each SIMD has two
-    int kw = 1;
-    while (kw < kFewWaves && tiles * kw < 8 * cus && kp / 64 / (2 * kw) >= 2) kw *= 2;
-    const long cw = kFewWaves / kw;
-    const dim3 grid((unsigned)((tiles + cw - 1) / cw)), block(64 * kFewWaves);
-    const size_t parts = kw > 1 ? (size_t)kFewWaves * MT * 64 * 16 : 0;
-    const size_t rows = (size_t)16 * MT * (size_t)(kp + 16);
-    const size_t head = 64 * MT;
-    if (!xq) {
-        const size_t lds = head + std::max(parts, rows);
-        EFLA_LAUNCH_LDS("linear_int8", (few_kernel<T, MT, true>), grid, block, lds, st, x, ldx, xq,
-                        xs, wq, (int)m, (int)n, k, kp, kw, o);
-    } else {
-        EFLA_LAUNCH_LDS("linear_int8", (few_kernel<T, MT, false>), grid, block, head + parts, st, x,
-                        ldx, xq, xs, wq, (int)m, (int)n, k, kp, kw, o);
-    }
+    // waves that split k: until three quarters of the compute units have a workgroup
+    long kw = 1;
+    while (kw < NW && tiles * kw < NW * cus * 3 / 4 && kp / 64 / (2 * kw) >= 2) kw *= 2;
+    const long cw = NW / kw;
+    const dim3 grid((unsigned)((tiles + cw - 1) / cw)), block(64 * NW);
+    const size_t parts = kw > 1 ? (size_t)NW * MT * 64 * 16 : 0;
+    const size_t rows = HOLD ? (size_t)16 * MT * (size_t)(kp + 16) : 0;
+    const size_t lds = 64 * MT + std::max(parts, rows);
+    EFLA_LAUNCH_LDS("linear_int8", (few_kernel<T, MT, HOLD>), grid, block, lds, st, x, ldx, xq, xs,
+                    wq, (int)m, (int)n, k, kp, (int)kw, o);
 }
 
 template <typename T, int TS, bool RAGGED>
@@ -57,14 +65,9 @@ static void tile_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, l
                 st, A, B, m, n, (int)(kp / kLine), xs, o);
 }
 
-// rows that the kernel quantises itself
-static bool fused(size_t m, size_t kp) {
-    return m <= kFewRows && up_to((long)m, 16) * (long)(kp + 16) <= (long)kFusedBytes;
-}
-
-static size_t scratch(size_t m, size_t k) {
+static size_t scratch(size_t m, size_t k, size_t size) {
     const size_t kp = (size_t)up_to((long)k, kLine);
-    return fused(m, kp) ? 0 : scales_bytes(m) + m * kp;
+    return fused(m, kp, size) ? 0 : scales_bytes(m) + m * kp;
 }
 
 template <typename T>
@@ -77,22 +80,33 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     const Out<T> o{y, ldy, bias, residual, ldr, sw, gelu};
     float* xs = nullptr;
     uint8_t* xq = nullptr;
-    if (!fused((size_t)m, (size_t)kp)) {
+    if (!fused((size_t)m, (size_t)kp, sizeof(T))) {
         xs = (float*)ws;
         xq = ws + scales_bytes((size_t)m);
-        const dim3 grid((unsigned)((m + 3) / 4)), block(256);
-        if (kp <= 1024)
-            EFLA_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 2>), grid, block, st, x, ldx, m, k,
-                        kp, xq, xs);
-        else
-            EFLA_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 8>), grid, block, st, x, ldx, m, k,
-                        kp, xq, xs);
+#define I8_QUANT(LPR, HOLD)                                                                      \
+    EFLA_LAUNCH("quantize_rows", (quantize_rows_kernel<T, LPR, HOLD>),                            \
+                dim3((unsigned)(LPR == 64 ? (m + 3) / 4 : m)), dim3(256), st, x, ldx, m, k, kp, xq, \
+                xs)
+        if (m < kWaveRows && kp > 512) I8_QUANT(256, 2);
+        else if (kp <= 1024) I8_QUANT(64, 2);
+        else I8_QUANT(64, 8);
+#undef I8_QUANT
         EFLA_CHECK(hipPeekAtLastError());
     }
-    if (m <= (long)kFewRows) {
-        if (m <= 16) few_launch<T, 1>(x, ldx, xq, xs, wq, m, n, k, kp, o, st);
-        else if (m <= 32) few_launch<T, 2>(x, ldx, xq, xs, wq, m, n, k, kp, o, st);
-        else few_launch<T, 4>(x, ldx, xq, xs, wq, m, n, k, kp, o, st);
+    if (few(m, n)) {
+#define I8_FEW(MT, HOLD) few_launch<T, MT, HOLD>(x, ldx, xq, xs, wq, m, n, k, kp, o, st)
+        if (!xq && m <= 16) {
+            I8_FEW(1, 4);
+        } else if (!xq) {
+            if constexpr (sizeof(T) == 2) I8_FEW(2, 4);
+        } else if (m <= 16) {
+            I8_FEW(1, 0);
+        } else if (m <= 32) {
+            I8_FEW(2, 0);
+        } else {
+            I8_FEW(4, 0);
+        }
+#undef I8_FEW
         return (int)hipPeekAtLastError();
     }
     const size_t a = 8 * sizeof(T);
@@ -150,7 +164,7 @@ extern "C" int int8_weight_pack_hip(const void* weight, size_t ld, void* packed,
 
 extern "C" size_t linear_int8_workspace_size(size_t m, size_t k) {
     if (k == 0 || k > i8::kMaxK || m > 0x3FFFFFFFull) return 0;
-    return i8::scratch(m, k);
+    return i8::scratch(m, k, 4);
 }
 
 extern "C" int linear_int8_hip(const void* x, size_t ldx, const void* packed, const void* bias,
@@ -169,7 +183,7 @@ extern "C" int linear_int8_hip(const void* x, size_t ldx, const void* packed, co
     if (((uintptr_t)x | (uintptr_t)output | (uintptr_t)bias | (uintptr_t)residual) % size ||
         (uintptr_t)packed % i8::kLine)
         return kInvalidValue;
-    const size_t need = i8::scratch(m, k);
+    const size_t need = i8::scratch(m, k, size);
     void* ws = workspace;
     WsLease lease;
     if (need != 0 && !ws) {

@@ -28,47 +28,43 @@ __device__ __forceinline__ float scale_of(float amax) {
     return amax < INFINITY ? amax / 127.f : NAN;
 }
 
-// x / scale to the nearest whole number, ties to even, as an exact quotient would round.
-// x times the reciprocal is off by a few units in the last place, so the whole number
-// can miss by one next to a half; x - r scale, which one fused operation gives
+// x / scale to the nearest whole number, ties to even, as an exact quotient would round:
+// eight of them, a byte each.  A fused multiply and add of 1.5 2^23 rounds x inv to a whole
+// number that its low byte holds.  inv is 1 / scale rounded, so x inv is off by 127 * 2^-23 at
+// most, and the whole number by one at most, next to a half: what lies within 2^-14 of one
+// (one vector in sixty) is looked at again.  There x - r scale, which one fused operation gives
 // without rounding (x and scale have 24 bits, r 7, and the difference is below scale),
 // says on which side of the half x lies.
+// A row of zeros, or one that holds NaN or an infinity, has inv 0: 0 everywhere.
 struct Quantizer {
-    float scale, inv, half;
-    bool zero, tiny;
+    float scale, inv;
     __device__ __forceinline__ explicit Quantizer(float s)
-        : scale(s), inv(1.f / s), half(0.5f * s), zero(!(s > 0.f)), tiny(s < 0x1p-100f) {}
-    __device__ __forceinline__ int operator()(float x) const {
-        if (zero) return 0;  // a row of zeros, or one that is NaN
-        if (tiny)            // the reciprocal or the half may leave the normal range
-            return (int)fminf(fmaxf(rintf(x / scale), -127.f), 127.f);
-        float r = rintf(x * inv);
-        const float d = fmaf(-r, scale, x), t = fabsf(d);
-        const bool odd = (int)r & 1;
-        if (t > half || (t == half && odd)) r += copysignf(1.f, d);
-        return (int)r;
-    }
-    // Eight of them, a byte each.  A fused multiply and add of 1.5 2^23 rounds x inv to a
-    // whole number that its low byte holds; x inv itself is off by 127 * 2^-23 at most, so
-    // only what lies within 2^-14 of a half is looked at again (one vector in sixty).
-    __device__ __forceinline__ uint2 pack(const float (&v)[8]) const {
+        : scale(s), inv(s > 0.f ? 1.f / s : 0.f) {}
+    template <typename Vec>
+    __device__ __forceinline__ uint2 operator()(const Vec& x) const {
         constexpr float kRound = 12582912.f;
-        uint32_t w[8];
-        float far = 0.f;
+        float v[8], t[8], far = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float t = fmaf(v[e], inv, kRound);
-            w[e] = __float_as_uint(t);
-            far = fmaxf(far, fabsf(fmaf(v[e], inv, kRound - t)));
+            v[e] = (float)x[e];
+            t[e] = fmaf(v[e], inv, kRound);
+            far = fmaxf(far, fabsf(fmaf(v[e], inv, kRound - t[e])));
         }
-        if (zero || tiny || !(far < 0.5f - 0x1p-14f)) {
+        if (far > 0.5f - 0x1p-14f) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = (uint32_t)(*this)(v[e]);
+            for (int e = 0; e < 8; ++e) {
+                const float d = fmaf(kRound - t[e], scale, v[e]), a = fabsf(d), h = 0.5f * scale;
+                const bool odd = __float_as_uint(t[e]) & 1;
+                t[e] += a > h || (a == h && odd) ? copysignf(1.f, d) : 0.f;
+            }
         }
-        auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-            return __builtin_amdgcn_perm(b, a, 0x0C0C0400u) | __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
+        auto four = [&](int e) {
+            const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[e + 1]), __float_as_uint(t[e]),
+                                                      0x0C0C0400u);
+            return lo | __builtin_amdgcn_perm(__float_as_uint(t[e + 3]), __float_as_uint(t[e + 2]),
+                                              0x04000C0Cu);
         };
-        return make_uint2(four(w[0], w[1], w[2], w[3]), four(w[4], w[5], w[6], w[7]));
+        return make_uint2(four(0), four(4));
     }
 };
 
@@ -77,9 +73,20 @@ struct Quantizer {
 __device__ __forceinline__ float amax2(float a, float x) {
     return __uint_as_float(max(__float_as_uint(a), __float_as_uint(x) & 0x7FFFFFFFu));
 }
-__device__ __forceinline__ float wave_amax(float m) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = amax2(m, __shfl_xor(m, o));
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xF,
+                                                               0xF, true));
+}
+// over N = 16, 32 or 64 neighbouring lanes, in each of them
+template <int N>
+__device__ __forceinline__ float lanes_amax(float m) {
+    m = amax2(m, dpp<0xB1>(m));   // quad_perm [1, 0, 3, 2]
+    m = amax2(m, dpp<0x4E>(m));   // quad_perm [2, 3, 0, 1]
+    m = amax2(m, dpp<0x141>(m));  // row_half_mirror
+    m = amax2(m, dpp<0x140>(m));  // row_mirror
+    if constexpr (N > 16) m = amax2(m, __shfl_xor(m, 16));
+    if constexpr (N > 32) m = amax2(m, __shfl_xor(m, 32));
     return m;
 }
 // The largest magnitude of vectors of 8, two 16-bit ones at a time
@@ -110,56 +117,98 @@ struct Amax<float> {
     __device__ __forceinline__ float get() const { return m; }
 };
 
-// One wave quantises a row: q gets kp bytes (zero behind k).  Rows of up to 64 * 8 * HOLD
-// elements stay in registers between the maximum and the quotients, longer ones are read
-// again.  Returns the scale.
-template <typename T, int HOLD>
-__device__ __forceinline__ float quantize_row(const T* x, long k, long kp, uint8_t* q) {
+// A row of k elements in LPR threads (lr: this one's place), the first 8 LPR HOLD of them in
+// registers.  Whole vectors and the last, partial one are loaded apart: a vector that may be
+// put together from elements is taken apart where its two ways meet, and that waits for
+// its load (a row of 4096 in one wave: 8 loads one by one, 9.5 us; 4.2 together).
+template <typename T, int LPR, int HOLD>
+struct Row {
     typedef gf::Piece<8, T> P8;
-    const int l = lane_id();
-    typename P8::vec v[HOLD];
-    Amax<T> m;
-    for (long c0 = 0; c0 < kp; c0 += 512 * HOLD) {
+    typedef typename P8::vec Vec;
+    static constexpr long kHeld = 8L * LPR * HOLD;
+    Vec v[HOLD], last;
+    __device__ __forceinline__ static Vec at(const T* x, long c, long k) {  // whole, or zero
+        Vec y{};
+        if (c + 8 <= k) y = *reinterpret_cast<const typename P8::uvec*>(x + c);
+        return y;
+    }
+    __device__ __forceinline__ void load(const T* x, long k, int lr) {
 #pragma unroll
-        for (int i = 0; i < HOLD; ++i) {
-            const long c = c0 + 8 * (l + 64 * i);
-            v[i] = typename P8::vec{};
-            if (c < k) v[i] = P8::load(x + c, k - c);
+        for (int i = 0; i < HOLD; ++i) v[i] = at(x, 8 * (lr + LPR * i), k);
+        last = Vec{};
+        if (k % 8 && lr == k / 8 % LPR) {
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+                if (e < k % 8) last[e] = x[k / 8 * 8 + e];
         }
+    }
+    __device__ __forceinline__ float amax(const T* x, long k, int lr) const {  // of this thread's
+        Amax<T> m;
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) m.add(v[i]);
+        m.add(last);
+        for (long c = kHeld + 8 * lr; c < k; c += 8 * LPR) m.add(at(x, c, k));
+        return m.get();
     }
-    const float s = scale_of(wave_amax(m.get()));
-    const Quantizer qz(s);
-    auto put = [&](long c, typename P8::vec x) {
-        float f[8];
+    // q: kp bytes, zero behind k
+    __device__ __forceinline__ void store(const T* x, long k, long kp, int lr, float scale,
+                                          uint8_t* q) {
+        // Below the normal range's reciprocals (never in fp16) everything is taken 2^64 times as
+        // large, which is exact.  A scale with few bits may leave more than 127 steps: cut off.
+        if (scale < 0x1p-100f && scale > 0.f) {
+            const float s = scale;
+            auto up = [&](Vec& y) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (float)x[e];
-        *reinterpret_cast<uint2*>(q + c) = qz.pack(f);
-    };
-    if (kp <= 512 * HOLD) {
+                for (int e = 0; e < 8; ++e)
+                    y[e] = (T)(fminf(fmaxf((float)y[e], -127.f * s), 127.f * s) * 0x1p64f);
+            };
+#pragma unroll
+            for (int i = 0; i < HOLD; ++i) up(v[i]);
+            up(last);
+            const Quantizer qz(s * 0x1p64f);
+            for (long c = kHeld + 8 * lr; c < kp; c += 8 * LPR) {
+                Vec y = at(x, c, k);
+                up(y);
+                *reinterpret_cast<uint2*>(q + c) = qz(y);
+            }
+            scale *= 0x1p64f;
+            kp = kp < kHeld ? kp : kHeld;
+        }
+        const Quantizer qz(scale);
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
-            const long c = 8 * (l + 64 * i);
-            if (c < kp) put(c, v[i]);
+            const long c = 8 * (lr + LPR * i);
+            if (c < kp) *reinterpret_cast<uint2*>(q + c) = qz(v[i]);
         }
-    } else {
-        for (long c = 8 * l; c < kp; c += 512)
-            put(c, c < k ? P8::load(x + c, k - c) : typename P8::vec{});
+        for (long c = kHeld + 8 * lr; c < kp; c += 8 * LPR)
+            *reinterpret_cast<uint2*>(q + c) = qz(at(x, c, k));
+        if (k % 8 && lr == k / 8 % LPR) *reinterpret_cast<uint2*>(q + k / 8 * 8) = qz(last);
     }
-    return s;
-}
+};
 
-// Four rows to a workgroup, a wave each.  Bound by memory.
-template <typename T, int HOLD>
+// LPR threads to a row: a wave, four rows to a workgroup, or (few rows) the whole workgroup,
+// where one wave's chain of instructions is what a row takes.  Bound by memory.
+template <typename T, int LPR, int HOLD>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ldx,
                                                             long m, long k, long kp,
                                                             uint8_t* __restrict__ q,
                                                             float* __restrict__ scales) {
-    const long row = (long)blockIdx.x * 4 + wave_id();
-    if (row >= m) return;
-    const float s = quantize_row<T, HOLD>(x + row * ldx, k, kp, q + row * kp);
-    if (lane_id() == 0) scales[row] = s;
+    __shared__ float part[4];
+    const long row = LPR == 64 ? (long)blockIdx.x * 4 + wave_id() : (long)blockIdx.x;
+    const int lr = threadIdx.x & (LPR - 1);
+    if (row >= m) return;  // whole waves; never where the workgroup shares a row
+    x += row * ldx;
+    Row<T, LPR, HOLD> r;
+    r.load(x, k, lr);
+    float a = lanes_amax<64>(r.amax(x, k, lr));
+    if constexpr (LPR == 256) {
+        if (lane_id() == 0) part[wave_id()] = a;
+        __syncthreads();
+        a = amax2(amax2(part[0], part[1]), amax2(part[2], part[3]));
+    }
+    const float s = scale_of(a);
+    r.store(x, k, kp, lr, s, q + row * kp);
+    if (lr == 0) scales[row] = s;
 }
 
 // Columns' largest magnitudes, as whole numbers, into amax (zero before).
@@ -173,32 +222,35 @@ __global__ void __launch_bounds__(256) column_amax_kernel(const T* __restrict__ 
     atomicMax(amax + c, __float_as_uint(m));
 }
 
-// 64 x 64 tiles of the weight, quantised and turned through LDS: a row of q per channel.
+// 64 x 64 tiles of the weight, turned through LDS and quantised: a row of q per channel.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_weight_kernel(const T* __restrict__ w, long ld, long k,
                                                           long n, long kp,
                                                           const uint32_t* __restrict__ amax,
                                                           uint8_t* __restrict__ q) {
-    __shared__ uint8_t tile[64][68];
+    __shared__ float tile[64][65];
     const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
-    for (long n0 = (long)blockIdx.x * 64; n0 < n; n0 += (long)gridDim.x * 64) {
-        for (long k0 = (long)blockIdx.y * 64; k0 < kp; k0 += (long)gridDim.y * 64) {
-            const long col = n0 + c;
-            const Quantizer qz(col < n ? scale_of(__uint_as_float(amax[col])) : 0.f);
-            for (int r = r0; r < 64; r += 4) {
-                const long row = k0 + r;
-                const float x = col < n && row < k ? to_f(w[row * ld + col]) : 0.f;
-                tile[c][r] = (uint8_t)qz(x);
+    const long n0 = (long)blockIdx.x * 64;
+    for (long k0 = (long)blockIdx.y * 64; k0 < kp; k0 += (long)gridDim.y * 64) {
+        for (int r = r0; r < 64; r += 4)
+            tile[r][c] = n0 + c < n && k0 + r < k ? to_f(w[(k0 + r) * ld + n0 + c]) : 0.f;
+        __syncthreads();
+        // a row of 64 in 8 threads
+        for (int i = threadIdx.x; i < 512; i += 256) {
+            const long col = n0 + (i >> 3);
+            if (col >= n) continue;
+            float s = scale_of(__uint_as_float(amax[col]));
+            const bool tiny = s < 0x1p-100f;  // as in Row::store
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = tile[8 * (i & 7) + e][i >> 3];
+                if (tiny) v[e] = fminf(fmaxf(v[e], -127.f * s), 127.f * s) * 0x1p64f;
             }
-            __syncthreads();
-            for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-                const int ch = i >> 4, b = 4 * (i & 15);
-                if (n0 + ch < n)
-                    *reinterpret_cast<uint32_t*>(q + (n0 + ch) * kp + k0 + b) =
-                        *reinterpret_cast<const uint32_t*>(&tile[ch][b]);
-            }
-            __syncthreads();
+            const Quantizer qz(tiny ? s * 0x1p64f : s);
+            *reinterpret_cast<uint2*>(q + col * kp + k0 + 8 * (i & 7)) = qz(v);
         }
+        __syncthreads();
     }
 }
 
@@ -219,72 +271,65 @@ struct Out {
     int gelu;
 };
 
-// W columns n .. of row m, cnt = N - n of them in the matrix
-template <int W, typename T, bool RAGGED>
-__device__ __forceinline__ void finish(const Out<T>& o, long m, long n, long cnt, const int* acc,
-                                       float sx) {
-    typedef gf::Piece<W, T, RAGGED> P;
-    typedef gf::Piece<W, float, RAGGED> F;
-    const typename F::vec sw = F::load(o.sw + n, cnt);
-    typename P::vec b{};
-    if (o.bias) b = P::load(o.bias + n, cnt);
-    float v[W];
-#pragma unroll
-    for (int e = 0; e < W; ++e) v[e] = fmaf((float)acc[e] * sx, sw[e], (float)b[e]);
-    if (o.gelu) {
-#pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = gelu::gelu_f<true>(v[e]);
-    }
-    if (o.residual) {
-        const typename P::vec r = P::load(o.residual + m * o.ldr + n, cnt);
-#pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += (float)r[e];
-    }
-    typename P::vec y;
-#pragma unroll
-    for (int e = 0; e < W; ++e) y[e] = (T)v[e];
-    P::store(o.y + m * o.ldy + n, y, cnt);
-}
-
 // --- few rows -------------------------------------------------------------------------
 // M <= 16 MT rows.  Bound by the weight, which is read once.  A wave takes 16 channels and
 // a range of k; the weights are the MFMA's A operand (16 x 16 x 64), read straight from
-// memory, 16 bytes a lane.  KW waves of a workgroup share their channels and split k; their
-// sums meet in LDS.  FUSED: the workgroup quantises the tokens into LDS itself, while
-// its first weights are on their way; otherwise they are read quantised.
-constexpr int kFewWaves = 8;
+// memory, 16 bytes a lane.  kw waves of a workgroup share their channels and split k; their
+// sums meet in LDS.  HOLD > 0: the workgroup quantises the tokens into LDS itself, all rows at
+// once, 32 lanes to a row (8 HOLD elements of each lane in registers).  Loads return in
+// the order in which they are issued, so the tokens are asked for before the weights and
+// quantised while those are on their way, and what the epilogue needs right behind.  HOLD 0:
+// the tokens are read quantised.
 constexpr int kAhead = 8;  // 64-byte steps of k whose weights a wave has in flight
+// waves of a workgroup: enough that 32 lanes have a row
+template <int MT, int HOLD>
+constexpr int kFewWaves = HOLD > 0 ? 8 * MT : 8;
 
-template <typename T, int MT, bool FUSED>
-__global__ void __launch_bounds__(64 * kFewWaves)
+template <typename T, int MT, int HOLD>
+__global__ void __launch_bounds__((64 * kFewWaves<MT, HOLD>), sizeof(T) == 2 ? 4 : 2)
 few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
            const float* __restrict__ xs, const uint8_t* __restrict__ wq, int M, int N, long k,
            long kp, int kw, Out<T> o) {
+    constexpr bool FUSED = HOLD > 0;
+    constexpr int NW = kFewWaves<MT, HOLD>;
+    typedef gf::Piece<4, T> P;
+    typedef gf::Piece<4, float> F;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int w = wave_id(), l = lane_id(), r = l & 15, g = l >> 4;
-    const int cw = kFewWaves / kw, wk = w % kw;
+    const int cw = NW / kw, wk = w % kw;
     const long n0 = ((long)blockIdx.x * cw + w / kw) * 16;
     const int steps = (int)(kp / 64), s0 = steps * wk / kw, s1 = steps * (wk + 1) / kw;
     const uint8_t* wp = wq + (n0 + r < N ? n0 + r : N - 1) * kp + 16 * g;
+    constexpr int LPR = 32;
+    const int own = threadIdx.x / LPR, lr = threadIdx.x % LPR;
+    Row<T, LPR, FUSED ? HOLD : 1> row;
+    if constexpr (FUSED) row.load(x + own * ldx, own < M ? k : 0, lr);
     int4v a[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
         const int s = s0 + i < s1 ? s0 + i : s0;
         a[i] = *reinterpret_cast<const int4v*>(wp + 64L * s);
     }
+    // lane l ends up with rows 16 t + r, channels n .. n + 3
+    const long n = n0 + 4 * g;
+    const bool mine = wk == 0 && n < N;
+    typename F::vec sw{};
+    typename P::vec bias{}, res[MT];
+    if (mine) {
+        sw = F::load(o.sw + n, N - n);
+        if (o.bias) bias = P::load(o.bias + n, N - n);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (o.residual && 16 * t + r < M)
+                res[t] = P::load(o.residual + (16 * t + r) * o.ldr + n, N - n);
+    }
     const long ldq = FUSED ? kp + 16 : kp;
     float* sc = reinterpret_cast<float*>(lds);  // 16 MT scales
     uint8_t* rows = lds + 64 * MT;
     if constexpr (FUSED) {
-        for (int m = w; m < 16 * MT; m += kFewWaves) {
-            if (m < M) {
-                const float s = quantize_row<T, 2>(x + m * ldx, k, kp, rows + m * ldq);
-                if (l == 0) sc[m] = s;
-            } else {
-                for (long c = 16 * l; c < kp; c += 1024)
-                    *reinterpret_cast<int4v*>(rows + m * ldq + c) = int4v{};
-            }
-        }
+        const float s = scale_of(lanes_amax<LPR>(row.amax(x, 0, lr)));
+        row.store(x, own < M ? k : 0, kp, lr, s, rows + own * ldq);
+        if (lr == 0) sc[own] = s;
         __syncthreads();
     }
     int4v acc[MT];
@@ -310,7 +355,6 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
             }
         }
     }
-    // lane l: row 16 t + r, channels n0 + 4 g .. + 3
     if (kw > 1) {
         if constexpr (FUSED) __syncthreads();  // the tokens have been read
         int4v* part = reinterpret_cast<int4v*>(rows);
@@ -322,17 +366,24 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t] += part[((w + j) * MT + t) * 64 + l];
     }
-    const long n = n0 + 4 * g;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int m = 16 * t + r;
-        if (m >= M || n >= N) continue;
-        const int v[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
-        finish<4, T, true>(o, m, n, N - n, v, FUSED ? sc[m] : xs[m]);
+        if (m >= M || !mine) continue;
+        const float sx = FUSED ? sc[m] : xs[m];
+        typename P::vec y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float v = fmaf((float)acc[t][e] * sx, sw[e], (float)bias[e]);
+            if (o.gelu) v = gelu::gelu_f<true>(v);
+            if (o.residual) v += (float)res[t][e];
+            y[e] = (T)v;
+        }
+        P::store(o.y + m * o.ldy + n, y, N - n);
     }
 }
 
-// The same for a lane of tile_kernel, whose 8 columns stay the same over its rows: their
+// The epilogue of a lane of tile_kernel, whose 8 columns stay the same over its rows: their
 // scales and bias are read once, and four rows' scales and residuals ahead of their use
 // (read where they are used, each waited behind its branch).
 template <typename T, bool RAGGED>
