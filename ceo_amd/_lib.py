@@ -143,7 +143,7 @@ _SIGS = {
     "state_reorder_hip": (i32, [vp, vp, vp]),
     "int8_weight_size": (sz, [sz, sz]),
     "int8_weight_pack_hip": (i32, [vp, sz, vp, sz, sz, i32, vp]),
-    "linear_int8_workspace_size": (sz, [sz, sz]),
+    "linear_int8_workspace_size": (sz, [sz, sz, sz, i32]),
     "linear_int8_hip": (i32, [vp, sz, vp, vp, vp, sz, vp, sz, sz, sz, sz, i32, i32, vp, sz, vp]),
     # sequence packing (host)
     "efla_pack_sequences": (i32, [vp, vp, sz, sz, vp, vp, vp, vp, ctypes.POINTER(sz),

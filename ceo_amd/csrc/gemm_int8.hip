@@ -27,7 +27,8 @@ static bool few(long m, long n) {
     return m <= 32 || (m <= 64 && (n + 127) / 128 < cus / 2);
 }
 
-// Fewer rows than this are quantised by a workgroup each, more by a wave.
+// Fewer rows than this are quantised by a workgroup each, more by a wave, unless a wave's registers
+// do not hold the row.
 constexpr long kWaveRows = 2048;
 
 // Whether few_kernel quantises the tokens itself: a second launch is longer than what it takes
@@ -54,18 +55,18 @@ static void few_launch(const T* x, long ldx, const uint8_t* xq, const float* xs,
                     wq, (int)m, (int)n, k, kp, (int)kw, o);
 }
 
-template <typename T, int TS, bool RAGGED>
+template <typename T, int TS, int FORM>
 static void tile_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
                         long kp, const Out<T>& o, hipStream_t st) {
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const long items = ((m + TS - 1) / TS) * ((n + TS - 1) / TS);
     const dim3 grid((unsigned)std::min(items, TS == 256 ? cus : 2 * cus));
     const gf::Opnd A{(const char*)xq, kp / 2, (int)m}, B{(const char*)wq, kp / 2, (int)n};
-    EFLA_LAUNCH("linear_int8", (tile_kernel<T, TS, RAGGED>), grid, dim3(64 * gf::tile_waves<TS>()),
+    EFLA_LAUNCH("linear_int8", (tile_kernel<T, TS, FORM>), grid, dim3(64 * gf::tile_waves<TS>()),
                 st, A, B, m, n, (int)(kp / kLine), xs, o);
 }
 
-static size_t scratch(size_t m, size_t k, size_t size) {
+static size_t scratch(size_t m, size_t k, size_t n, size_t size) {
     const size_t kp = (size_t)up_to((long)k, kLine);
     return fused(m, kp, size) ? 0 : scales_bytes(m) + m * kp;
 }
@@ -87,7 +88,8 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     EFLA_LAUNCH("quantize_rows", (quantize_rows_kernel<T, LPR, HOLD>),                            \
                 dim3((unsigned)(LPR == 64 ? (m + 3) / 4 : m)), dim3(256), st, x, ldx, m, k, kp, xq, \
                 xs)
-        if (m < kWaveRows && kp > 512) I8_QUANT(256, 2);
+        if (kp > 4096) I8_QUANT(256, 8);
+        else if (m < kWaveRows && kp > 512) I8_QUANT(256, 2);
         else if (kp <= 1024) I8_QUANT(64, 2);
         else I8_QUANT(64, 8);
 #undef I8_QUANT
@@ -115,10 +117,16 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
                        (!residual || ((uintptr_t)residual % a == 0 && ldr % 8 == 0));
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const bool large = ((m + 255) / 256) * ((n + 255) / 256) >= cus;
-    if (large && whole) tile_launch<T, 256, false>(xq, xs, wq, m, n, kp, o, st);
-    else if (large) tile_launch<T, 256, true>(xq, xs, wq, m, n, kp, o, st);
-    else if (whole) tile_launch<T, 128, false>(xq, xs, wq, m, n, kp, o, st);
-    else tile_launch<T, 128, true>(xq, xs, wq, m, n, kp, o, st);
+    // past the L2s from their 32 MB on (16384 x 1024 x 4096 with a residual 113 -> 104 us, without
+    // any 88 to 92 either way)
+    const bool past = (size_t)m * (size_t)n * sizeof(T) >= (size_t)32 << 20;
+#define I8_TILE(TS, FORM) tile_launch<T, TS, FORM>(xq, xs, wq, m, n, kp, o, st)
+    if (large && whole && past) I8_TILE(256, kPast);
+    else if (large && whole) I8_TILE(256, kWhole);
+    else if (large) I8_TILE(256, kRagged);
+    else if (whole) I8_TILE(128, kWhole);
+    else I8_TILE(128, kRagged);
+#undef I8_TILE
     return (int)hipPeekAtLastError();
 }
 
@@ -162,9 +170,11 @@ extern "C" int int8_weight_pack_hip(const void* weight, size_t ld, void* packed,
     return i8::pack((const float*)weight, (long)ld, (uint8_t*)packed, (long)k, (long)n, stream);
 }
 
-extern "C" size_t linear_int8_workspace_size(size_t m, size_t k) {
-    if (k == 0 || k > i8::kMaxK || m > 0x3FFFFFFFull) return 0;
-    return i8::scratch(m, k, 4);
+extern "C" size_t linear_int8_workspace_size(size_t m, size_t k, size_t n, int dtype) {
+    const size_t size = i8::dtype_size(dtype);
+    if (size == 0 || k == 0 || k > i8::kMaxK || n == 0 || n > 0x3FFFFFFFull || m > 0x3FFFFFFFull)
+        return 0;
+    return i8::scratch(m, k, n, size);
 }
 
 extern "C" int linear_int8_hip(const void* x, size_t ldx, const void* packed, const void* bias,
@@ -183,7 +193,7 @@ extern "C" int linear_int8_hip(const void* x, size_t ldx, const void* packed, co
     if (((uintptr_t)x | (uintptr_t)output | (uintptr_t)bias | (uintptr_t)residual) % size ||
         (uintptr_t)packed % i8::kLine)
         return kInvalidValue;
-    const size_t need = i8::scratch(m, k, size);
+    const size_t need = i8::scratch(m, k, n, size);
     void* ws = workspace;
     WsLease lease;
     if (need != 0 && !ws) {

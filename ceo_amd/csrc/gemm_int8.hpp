@@ -383,11 +383,16 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
     }
 }
 
+// What the output's pieces are: whole and aligned, of any alignment and length, or whole and
+// stored past the L2s (an output that they do not hold takes the operands' place in them).
+enum Form { kWhole, kRagged, kPast };
+
 // The epilogue of a lane of tile_kernel, whose 8 columns stay the same over its rows: their
 // scales and bias are read once, and four rows' scales and residuals ahead of their use
 // (read where they are used, each waited behind its branch).
-template <typename T, bool RAGGED>
+template <typename T, int FORM>
 struct Columns {
+    static constexpr bool RAGGED = FORM == kRagged;
     typedef gf::Piece<8, T, RAGGED> P;
     typedef gf::Piece<8, float, RAGGED> F;
     long n, cnt;
@@ -433,7 +438,11 @@ struct Columns {
         typename P::vec y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = (T)v[e];
-        P::store(o.y + m * o.ldy + n, y, cnt);
+        T* to = o.y + m * o.ldy + n;
+        if constexpr (FORM == kPast)
+            __builtin_nontemporal_store(y, reinterpret_cast<typename P::vec*>(to));
+        else
+            P::store(to, y, cnt);
     }
 };
 
@@ -442,7 +451,7 @@ struct Columns {
 // place of each 16-bit element: 256 x 256 x 128 (eight waves of 128 x 64) or 128 x 128 x 128
 // (four of 64 x 64, two workgroups to a CU), copied straight into LDS one block ahead,
 // MFMA 32 x 32 x 32.  Rows are padded to whole blocks, so there is no tail in k.
-template <typename T, int TS, bool RAGGED>
+template <typename T, int TS, int FORM>
 __global__ void __launch_bounds__(64 * gf::tile_waves<TS>(), TS == 128 ? 2 : 1)
 tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
             Out<T> o) {
@@ -545,10 +554,10 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
         {
             const int le = mf::tid_in(~(int)it) & 63;
             char* wp = smem + 2 * (buf ^ 1) * TILE + (4096 * TNI) * w;
-            const Columns<T, RAGGED> col(o, n0 + wn + 8 * (le & 7), N);
+            const Columns<T, FORM> col(o, n0 + wn + 8 * (le & 7), N);
             // (fp32 residuals and ragged ones leave no registers to read a pass ahead in)
-            constexpr bool AHEAD = sizeof(T) == 2 && !RAGGED;
-            typename Columns<T, RAGGED>::Rows rows[2];
+            constexpr bool AHEAD = sizeof(T) == 2 && FORM != kRagged;
+            typename Columns<T, FORM>::Rows rows[2];
             if (AHEAD && m0 + wm < M) rows[0].load(o, col, xs, m0 + wm + (le >> 3), M);
 #pragma unroll
             for (int j = 0; j < TMJ; ++j) {

@@ -758,7 +758,7 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, bias=None, residual=None,
             ldr = n
             residual = residual.contiguous()
     y = torch.empty(m, n, dtype=x.dtype, device=x.device)
-    wsb = lib().linear_int8_workspace_size(m, k)
+    wsb = lib().linear_int8_workspace_size(m, k, n, dt)
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
     rc = lib().linear_int8_hip(_p(x), ldx, _p(weight.packed), _p(bias), _p(residual), ldr, _p(y), n,
                                m, k, n, int(gelu), dt, _p(ws), wsb, _stream(x))

@@ -157,13 +157,14 @@ class StateList:
                                              self.beams)
         check(rc, "state_list_create_hip")
         self._handle = handle
+        self._destroy = lib().state_list_destroy_hip  # the module may go before its lists
 
     def __reduce__(self):  # a copy has a table of its own
         return type(self), (self.states, self.beams, self.outs)
 
     def __del__(self):
-        if getattr(self, "_handle", None) and lib is not None:  # None: the program's end
-            lib().state_list_destroy_hip(self._handle)
+        if getattr(self, "_handle", None):
+            self._destroy(self._handle)
             self._handle = None
 
 
@@ -176,6 +177,8 @@ def reorder(states: StateList, parents: torch.Tensor) -> None:
     efla._require(parents, "parents", torch.int32, states.device)
     if parents.shape != (states.batch, states.beams):
         raise ValueError("parents must be (batch, beams)")
-    with torch.cuda.device(states.device):
-        rc = lib().state_reorder_hip(states._handle, parents.data_ptr(), efla._stream(parents))
+    if parents.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(states.device):
+            return reorder(states, parents)
+    rc = lib().state_reorder_hip(states._handle, parents.data_ptr(), efla._stream(parents))
     check(rc, "state_reorder_hip")

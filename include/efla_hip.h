@@ -721,10 +721,10 @@ int int8_weight_pack_hip(const void* weight, size_t ld, void* packed, size_t k, 
  * (F32, F16 or BF16), whatever the packed weight was made from; any row strides and element
  * alignment; output may be residual itself, x neither.  A row of x with a NaN or an infinity
  * gives a row of NaN.  Workspace (16-byte aligned) of at least linear_int8_workspace_size()
- * bytes, or NULL: the library's cached one for `stream`.  Calls with the same row of x give
+ * bytes (0: none, or arguments out of range), or NULL: the library's cached one for `stream`.  Calls with the same row of x give
  * the same bits in that row, whatever m is.  Codes as above; m == 0 -> 0.
  */
-size_t linear_int8_workspace_size(size_t m, size_t k);
+size_t linear_int8_workspace_size(size_t m, size_t k, size_t n, int dtype);
 int linear_int8_hip(const void* x, size_t ldx, const void* packed, const void* bias,
                     const void* residual, size_t ld_residual, void* output, size_t ld_output,
                     size_t m, size_t k, size_t n, int gelu, int dtype, void* workspace,
