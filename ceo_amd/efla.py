@@ -145,9 +145,16 @@ def _q_shapes(q, k, v, beta, cu_seqlens):
 SAVE_STATES = 1  # EFLA_FWD_SAVE_STATES
 
 
+STEP_TOKENS = 6  # continued from a carried state without a workspace: no chunk, fp32 throughout
+
+
 def chunk_efla_fwd(q, k, v, beta, initial_state=None, output_final_state=False,
-                   cu_seqlens=None, workspace=None, save_states=False):
+                   cu_seqlens=None, workspace=None, save_states=False, out_state=None):
     """Returns (o, final_state or None).
+
+    ``out_state`` ((N,H,K,V) fp32) receives the final state instead of a new tensor.  It may be
+    ``initial_state`` itself, updated in place, for up to ``STEP_TOKENS`` tokens of
+    equal-length sequences without a ``workspace``: a generated token.
 
     With ``save_states`` the chunk start states (and, for bf16, each chunk's
     P = tril(Q K^T)) are also written into ``workspace`` (which must then be a
@@ -160,9 +167,19 @@ def chunk_efla_fwd(q, k, v, beta, initial_state=None, output_final_state=False,
         _require(initial_state, "initial_state", torch.float32, q.device)
         if initial_state.shape != (N, H, K, V):
             raise ValueError("initial_state must be (N,H,K,V) fp32")
+    st = None
+    if out_state is not None:
+        _require(out_state, "out_state", torch.float32, q.device)
+        if out_state.shape != (N, H, K, V):
+            raise ValueError("out_state must be (N,H,K,V) fp32")
+        if initial_state is not None and out_state.data_ptr() == initial_state.data_ptr() and \
+                (T > STEP_TOKENS or cu_seqlens is not None or workspace is not None):
+            raise ValueError(f"a state in place takes up to {STEP_TOKENS} tokens of equal-length "
+                             "sequences and no workspace")
+        st = out_state
     o = torch.empty(B, T, H, V, dtype=q.dtype, device=q.device)
-    st = torch.empty(N, H, K, V, dtype=torch.float32, device=q.device) \
-        if output_final_state else None
+    if output_final_state and st is None:
+        st = torch.empty(N, H, K, V, dtype=torch.float32, device=q.device)
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     args = (_p(q), _p(k), _p(v), _p(beta), _p(initial_state), _p(o), _p(st), _p(cu_seqlens),
             B, T, N if cu_seqlens is not None else 0, H, K, V, 64, dt, _p(workspace), ws_bytes,
