@@ -55,15 +55,25 @@ static void few_launch(const T* x, long ldx, const uint8_t* xq, const float* xs,
                     wq, (int)m, (int)n, k, kp, (int)kw, o);
 }
 
+static long tiles(long m, long n, long ts) { return ((m + ts - 1) / ts) * ((n + ts - 1) / ts); }
+
 template <typename T, int TS, int FORM>
 static void tile_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
                         long kp, const Out<T>& o, hipStream_t st) {
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const long items = ((m + TS - 1) / TS) * ((n + TS - 1) / TS);
+    const long items = tiles(m, n, TS);
     const dim3 grid((unsigned)std::min(items, TS == 256 ? cus : 2 * cus));
     const gf::Opnd A{(const char*)xq, kp / 2, (int)m}, B{(const char*)wq, kp / 2, (int)n};
     EFLA_LAUNCH("linear_int8", (tile_kernel<T, TS, FORM>), grid, dim3(64 * gf::tile_waves<TS>()),
                 st, A, B, m, n, (int)(kp / kLine), xs, o);
+}
+
+template <typename T, int FORM>
+static void deep_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
+                        long kp, const Out<T>& o, hipStream_t st) {
+    const gf::Opnd A{(const char*)xq, kp / 2, (int)m}, B{(const char*)wq, kp / 2, (int)n};
+    EFLA_LAUNCH("linear_int8", (deep_tile_kernel<T, FORM>), dim3((unsigned)tiles(m, n, 128)),
+                dim3(256), st, A, B, m, n, (int)(kp / kLine), xs, o);
 }
 
 static size_t scratch(size_t m, size_t k, size_t n, size_t size) {
@@ -116,7 +126,7 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
                        (!bias || (uintptr_t)bias % a == 0) &&
                        (!residual || ((uintptr_t)residual % a == 0 && ldr % 8 == 0));
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const bool large = ((m + 255) / 256) * ((n + 255) / 256) >= cus;
+    const bool large = tiles(m, n, 256) >= cus, deep = tiles(m, n, 128) <= cus;
     // past the L2s from their 32 MB on (16384 x 1024 x 4096 with a residual 113 -> 104 us, without
     // any 88 to 92 either way)
     const bool past = (size_t)m * (size_t)n * sizeof(T) >= (size_t)32 << 20;
@@ -124,6 +134,8 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     if (large && whole && past) I8_TILE(256, kPast);
     else if (large && whole) I8_TILE(256, kWhole);
     else if (large) I8_TILE(256, kRagged);
+    else if (deep && whole) deep_launch<T, kWhole>(xq, xs, wq, m, n, kp, o, st);
+    else if (deep) deep_launch<T, kRagged>(xq, xs, wq, m, n, kp, o, st);
     else if (whole) I8_TILE(128, kWhole);
     else I8_TILE(128, kRagged);
 #undef I8_TILE

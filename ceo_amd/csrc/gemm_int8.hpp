@@ -451,6 +451,83 @@ struct Columns {
 // place of each 16-bit element: 256 x 256 x 128 (eight waves of 128 x 64) or 128 x 128 x 128
 // (four of 64 x 64, two workgroups to a CU), copied straight into LDS one block ahead,
 // MFMA 32 x 32 x 32.  Rows are padded to whole blocks, so there is no tail in k.
+
+// Waits until at most N vector memory operations are under way, whatever the other counters.
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
+}
+
+// A wave's part of the output, rows mw .., columns nw ..: lane l holds for tile (i, j) row
+// mw + 32 j + (l & 31) and columns nw + 32 i + 8 q + 4 (l >> 5) + e in acc[i][j][4 q + e].  They go
+// through the wave's 8 KB of free LDS at wp, 32 rows at a time, into 8-column pieces.
+template <typename T, int FORM, int TMJ>
+__device__ __forceinline__ void tile_epilogue(const Out<T>& o, const int16v (&acc)[2][TMJ],
+                                              const float* __restrict__ xs, long mw, long nw,
+                                              long M, long N, int l, char* wp) {
+    const Columns<T, FORM> col(o, nw + 8 * (l & 7), N);
+    // (fp32 residuals and ragged ones leave no registers to read a pass ahead in)
+    constexpr bool AHEAD = sizeof(T) == 2 && FORM != kRagged;
+    typename Columns<T, FORM>::Rows rows[2];
+    if (AHEAD && mw < M) rows[0].load(o, col, xs, mw + (l >> 3), M);
+#pragma unroll
+    for (int j = 0; j < TMJ; ++j) {
+        const long r0 = mw + 32 * j;
+        if (r0 >= M) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<int4v*>(wp + gf::ep_off<2>(l & 31, 32 * i + 8 * q + 4 * (l >> 5))) =
+                    int4v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                          acc[i][j][4 * q + 3]};
+        // the next pass's scales and residual are on their way while this one is
+        // finished: its accumulators have left their registers
+        if (AHEAD && j + 1 < TMJ && r0 + 32 < M)
+            rows[(j + 1) & 1].load(o, col, xs, r0 + 32 + (l >> 3), M);
+        if (!AHEAD) rows[j & 1].load(o, col, xs, r0 + (l >> 3), M);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int row = 8 * s + (l >> 3), c = 8 * (l & 7);
+            const int4v v0 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<2>(row, c));
+            const int4v v1 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<2>(row, c + 4));
+            const int v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+            if (r0 + row < M && col.cnt > 0) col.finish(o, r0 + row, v, rows[j & 1], s);
+        }
+    }
+}
+
+// Fragments and products of one 32-deep step of a tile's block, reads of the next between them
+template <int TS, int TMJ>
+struct Steps {
+    int4v fb[2][2], fa[2][TMJ];
+    __device__ __forceinline__ void read(int c, const char* as, const char* bs, int wm, int wn,
+                                         int ks, int l) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            fb[c][i] = __builtin_bit_cast(int4v, gf::frag<true, TS>(bs, wn + 32 * i, ks, l));
+#pragma unroll
+        for (int j = 0; j < TMJ; ++j)
+            fa[c][j] = __builtin_bit_cast(int4v, gf::frag<true, TS>(as, wm + 32 * j, ks, l));
+    }
+    __device__ __forceinline__ void mma(int c, int16v (&acc)[2][TMJ]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < TMJ; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[c][i], fa[c][j], acc[i][j], 0,
+                                                                  0, 0);
+        // one LDS read between consecutive MFMAs
+        constexpr int NR = 2 + TMJ, NM = TMJ * 2, R = NR < NM ? NR : NM;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // DS read
+        }
+        if constexpr (NM > R) __builtin_amdgcn_sched_group_barrier(0x008, NM - R, 0);
+    }
+};
+
 template <typename T, int TS, int FORM>
 __global__ void __launch_bounds__(64 * gf::tile_waves<TS>(), TS == 128 ? 2 : 1)
 tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
@@ -502,30 +579,9 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
 #pragma unroll
             for (int j = 0; j < TMJ; ++j) acc[i][j] = int16v{};
         const bool act = m0 + wm < M && n0 + wn < N;
-        int4v fb[2][TNI], fa[2][TMJ];
-        auto read = [&](int c, int b, int ks) {
-#pragma unroll
-            for (int i = 0; i < TNI; ++i)
-                fb[c][i] = __builtin_bit_cast(int4v, gf::frag<true, TS>(Bs(b), wn + 32 * i, ks, l));
-#pragma unroll
-            for (int j = 0; j < TMJ; ++j)
-                fa[c][j] = __builtin_bit_cast(int4v, gf::frag<true, TS>(As(b), wm + 32 * j, ks, l));
-        };
-        auto mma_step = [&](int c) {
-#pragma unroll
-            for (int i = 0; i < TNI; ++i)
-#pragma unroll
-                for (int j = 0; j < TMJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[c][i], fa[c][j], acc[i][j],
-                                                                      0, 0, 0);
-            constexpr int NR = TNI + TMJ, NM = TMJ * TNI, R = NR < NM ? NR : NM;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // DS read
-            }
-            if constexpr (NM > R) __builtin_amdgcn_sched_group_barrier(0x008, NM - R, 0);
-        };
+        Steps<TS, TMJ> st;
+        auto read = [&](int c, int b, int ks) { st.read(c, As(b), Bs(b), wm, wn, ks, l); };
+        auto mma_step = [&](int c) { st.mma(c, acc); };
         if (act) read(0, buf, 0);
         for (int kt = 0; kt < niter; ++kt) {
             __builtin_amdgcn_s_setprio(1);
@@ -548,50 +604,68 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
             buf ^= 1;
         }
         __builtin_amdgcn_s_setprio(0);
-        // lane l, tile (i, j): row m0 + wm + 32 j + (l & 31), columns n0 + wn + 32 i + 8 q +
-        // 4 (l >> 5) + e in acc[i][j][4 q + e]: through the free buffer, 32 rows at a time,
-        // into 8-column pieces
         {
             const int le = mf::tid_in(~(int)it) & 63;
             char* wp = smem + 2 * (buf ^ 1) * TILE + (4096 * TNI) * w;
-            const Columns<T, FORM> col(o, n0 + wn + 8 * (le & 7), N);
-            // (fp32 residuals and ragged ones leave no registers to read a pass ahead in)
-            constexpr bool AHEAD = sizeof(T) == 2 && FORM != kRagged;
-            typename Columns<T, FORM>::Rows rows[2];
-            if (AHEAD && m0 + wm < M) rows[0].load(o, col, xs, m0 + wm + (le >> 3), M);
-#pragma unroll
-            for (int j = 0; j < TMJ; ++j) {
-                const long r0 = (long)m0 + wm + 32 * j;
-                if (r0 >= M) break;
-#pragma unroll
-                for (int i = 0; i < TNI; ++i)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<int4v*>(
-                            wp + gf::ep_off<TNI>(le & 31, 32 * i + 8 * q + 4 * (le >> 5))) =
-                            int4v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                                  acc[i][j][4 * q + 3]};
-                // the next pass's scales and residual are on their way while this one is
-                // finished: its accumulators have left their registers
-                if (AHEAD && j + 1 < TMJ && r0 + 32 < M)
-                    rows[(j + 1) & 1].load(o, col, xs, r0 + 32 + (le >> 3), M);
-                if (!AHEAD) rows[j & 1].load(o, col, xs, r0 + (le >> 3), M);
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int row = 8 * s + (le >> 3), c = 8 * (le & 7);
-                    const int4v v0 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, c));
-                    const int4v v1 = *reinterpret_cast<const int4v*>(wp + gf::ep_off<TNI>(row, c + 4));
-                    const int v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                    if (r0 + row < M && col.cnt > 0)
-                        col.finish(o, r0 + row, v, rows[j & 1], s);
-                }
-            }
+            tile_epilogue<T, FORM>(o, acc, xs, (long)m0 + wm, (long)n0 + wn, M, N, le, wp);
         }
         it += gridDim.x;
         if (it >= nitems) break;
         __syncthreads();
         decode(it, m0, n0);
     }
+}
+
+// The same for outputs of no more 128 x 128 tiles than there are compute units, each of which has
+// one alone: four buffers, three blocks under way.  Operations end in order, so the wait for a
+// block counts those behind it.  (This / two buffers, us: 65 x 1024 x 1024 9.3 / 10.2, 65 x 4096 x
+// 1024 22.4 / 24.2, 65 x 1024 x 32000 11.1 / 11.9, 517 x 1001 x 3088 10.6 / 11.4.)  What is left
+// is one wave's chain on each SIMD, 0.54 us a block.
+constexpr int kDeep = 4;
+
+template <typename T, int FORM>
+__global__ void __launch_bounds__(256)
+deep_tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
+                 Out<T> o) {
+    constexpr int TS = 128, TMJ = 2, KS = 4, TILE = gf::tile_bytes<TS>();
+    constexpr int DMA = 2 * (TS / 8 / gf::tile_waves<TS>());  // instructions a wave and block
+    __shared__ __attribute__((aligned(1024))) char smem[kDeep * 2 * TILE];
+    const int tm_n = (int)((M + TS - 1) / TS);
+    const int m0 = (int)(blockIdx.x % tm_n) * TS, n0 = (int)(blockIdx.x / tm_n) * TS;
+    const int w = mf::wave(), l = mf::lane();
+    const int wm = (w & 1) * (TS / 2), wn = (w >> 1) * 64;
+    auto fetch = [&](int kt) {
+        if (kt >= niter) return;
+        char* to = smem + (kt % kDeep) * 2 * TILE;
+        gf::copy_tile<true, TS>(A, m0, (long)kt * gf::BK, to, w, l);
+        gf::copy_tile<true, TS>(B, n0, (long)kt * gf::BK, to + TILE, w, l);
+    };
+#pragma unroll
+    for (int kt = 0; kt + 1 < kDeep; ++kt) fetch(kt);
+    int16v acc[2][TMJ];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < TMJ; ++j) acc[i][j] = int16v{};
+    Steps<TS, TMJ> st;
+    for (int kt = 0; kt < niter; ++kt) {
+        const int behind = niter - 1 - kt;  // blocks after this one: two at most are under way
+        if (behind >= 2) wait_vm<2 * DMA>();
+        else if (behind == 1) wait_vm<DMA>();
+        else mf::dma_wait();
+        __syncthreads();
+        // every wave has read the block before: its buffer takes the one three ahead
+        fetch(kt + kDeep - 1);
+        const char *as = smem + (kt % kDeep) * 2 * TILE, *bs = as + TILE;
+        st.read(0, as, bs, wm, wn, 0, l);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if (ks + 1 < KS) st.read((ks + 1) & 1, as, bs, wm, wn, ks + 1, l);
+            st.mma(ks & 1, acc);
+        }
+    }
+    __syncthreads();  // the last block has been read
+    tile_epilogue<T, FORM>(o, acc, xs, (long)m0 + wm, (long)n0 + wn, M, N, l, smem + 8192 * w);
 }
 
 }  // namespace i8
