@@ -36,7 +36,8 @@ namespace bs {
 
 constexpr int NT = 256, NWV = NT / kWave;
 constexpr int kMaxSelect = 64, kMaxBeams = 64;
-constexpr int kPlaces = 512;   // candidates that LDS holds
+constexpr int kPlaces = 512;   // candidates that LDS holds, a slice's
+constexpr int kJoinPlaces = 2048;  // and a text's
 constexpr int kVectors = 512;  // and 16-byte vectors that have some
 
 // What is left of a slice: one of its best logits; none: token -1.
@@ -70,6 +71,26 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int n) {
     }
     return got;
 }
+
+// The same from 256 keys in LDS, one a thread, for larger n, of which 64 groups say little (the
+// least of 64 groups' largest lets 300 of 2000 logits through, the 64th of 256 groups' 75;
+// up to 32 that costs more than it saves).  The keys have the thread in their low byte,
+// so that no two are equal.  A barrier is behind the keys and one in front of *got, which
+// holds 0 before.
+__device__ __forceinline__ uint32_t with_thread(uint32_t key) {
+    return (key & ~255u) | (threadIdx.x & 255u);
+}
+__device__ __forceinline__ void block_bound(const uint32_t (&keys)[256], int n, uint32_t* got) {
+    const uint32_t mine = keys[threadIdx.x];
+    int rank = 0;
+#pragma unroll 2
+    for (int k = 0; k < 256; k += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(&keys[k]);
+        rank += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+    }
+    if (rank == n - 1) *got = mine & ~255u;
+}
+constexpr int kFewSelect = 32;  // up to here wave_bound does
 
 // Over the wave, in every lane: within rows of 16 by lane permutations, then across them.
 template <int CTRL>
@@ -129,7 +150,9 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
     __shared__ Vec piece[kVectors];
     __shared__ int piece_at[kVectors];  // its first token
     __shared__ uint64_t place[kPlaces];
-    __shared__ float wm[NWV], ws[NWV], lanes[NT];
+    __shared__ float wm[NWV], ws[NWV];
+    __shared__ __attribute__((aligned(16))) uint32_t lanes[NT];
+    __shared__ uint32_t exact;
     __shared__ uint64_t best[NWV];
     __shared__ int pieces, count;
     const long row = blockIdx.y;
@@ -138,7 +161,7 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
     const T* p = logits + row * ld;
     const int shift = (int)((uintptr_t)p % 128 / sizeof(T));
     const long v0 = (long)blockIdx.x * L - shift;  // the slice's first token
-    if (threadIdx.x == 0) pieces = count = 0;
+    if (threadIdx.x == 0) pieces = count = 0, exact = 0;
 
     Vec x[VPT];
     if (v0 >= 0 && v0 + L <= V) {  // the whole slice lies in the row
@@ -187,13 +210,19 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
         wm[wave_id()] = M;
         ws[wave_id()] = s;
     }
-    lanes[threadIdx.x] = m;
+    lanes[threadIdx.x] = n <= kFewSelect ? ordered(m) : with_thread(ordered(m));
     __syncthreads();
-    float group = lanes[lane_id()];
+    uint32_t least;
+    if (n <= kFewSelect) {
+        uint32_t group = lanes[lane_id()];
 #pragma unroll
-    for (int k = 1; k < NWV; ++k) group = fmaxf(group, lanes[lane_id() + k * kWave]);
-    const uint32_t least =
-        wave_bound<sizeof(T) == 2 && !__is_same(T, f16) ? 16 : 12>(ordered(group), n);
+        for (int k = 1; k < NWV; ++k) group = max(group, lanes[lane_id() + k * kWave]);
+        least = wave_bound<sizeof(T) == 2 && !__is_same(T, f16) ? 16 : 12>(group, n);
+    } else {
+        block_bound(lanes, n, &exact);
+        __syncthreads();
+        least = exact;
+    }
     // vectors that reach the bound
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -303,24 +332,32 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
             uint8_t* __restrict__ out_finished) {
     __shared__ double offset[kMaxBeams];  // score - log sum exp; -inf: offers nothing
     __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
-    __shared__ Best place[kPlaces];
+    __shared__ Best place[kJoinPlaces];
     __shared__ Best res[kMaxSelect];
     __shared__ Best wbest[NTJ / kWave];
+    __shared__ __attribute__((aligned(16))) uint32_t groups[256];
+    __shared__ uint32_t exact;
     __shared__ int count;
     const long text = blockIdx.x, row0 = text * beams;
     const int per = slices * n, total = beams * per;
     const Cand* mine = cands + row0 * per;
-    // On their way while the sums are joined: an entry a thread, and the heads of a lane's
-    // first lists (what beams that were not read left there is not looked at).
+    // On their way while the sums are joined: an entry a thread, and the lists' heads, a few to
+    // each lane or (many to select) one to each of 256 threads.  Where there are fewer lists,
+    // their second entries are among them, and so on.  (What beams that were not read
+    // left there is not looked at.)
     const int e0 = (int)threadIdx.x;
     const Cand held = e0 < total ? mine[e0] : Cand{0.f, -1};
+    const int lists = beams * slices;
+    const bool few = n <= kFewSelect;
+    int from[kHeads];
     Cand head[kHeads];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
-        const int j = lane_id() + i * kWave;
-        head[i] = j < beams * slices ? mine[j * n] : Cand{0.f, -1};
+        const int j = few ? lane_id() + i * kWave : e0 + i * 256, depth = j / lists;
+        from[i] = depth < n ? (j - depth * lists) * n + depth : total;
+        head[i] = depth < n ? mine[from[i]] : Cand{0.f, -1};
     }
-    if (threadIdx.x == 0) count = 0;
+    if (threadIdx.x == 0) count = 0, exact = 0;
     // 16 lanes to a beam
     for (int k = threadIdx.x / 16; k < beams; k += NTJ / 16) {
         const int l = threadIdx.x % 16;
@@ -367,18 +404,28 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         return v > -(double)INFINITY ? (uint32_t)(ordered(v + 0.0) >> 32) : 0u;
     };
     const Best first = best_of(e0, held);
-    // The bound, in every wave by itself: each lane takes the heads of some slices' lists, which
-    // are their largest.
+    // The bound from the largest of some lists: 64 lanes', in every wave by itself, or 256 threads'.
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kHeads; ++i)
-        top = max(top, key_of(best_of((lane_id() + i * kWave) * n, head[i]).value));
-    for (int j = lane_id() + kHeads * kWave; j < beams * slices; j += kWave)
+        top = max(top, key_of(best_of(from[i], head[i]).value));
+    for (int j = (few ? lane_id() + kHeads * kWave : e0 + kHeads * 256); j < lists;
+         j += few ? kWave : 256)
         top = max(top, key_of(best_of(j * n, mine[j * n]).value));
-    const uint32_t least = max(wave_bound<4>(top, n), 1u);
+    uint32_t least;
+    if (few) {
+        least = wave_bound<4>(top, n);
+    } else {
+        if (e0 < 256) groups[e0] = with_thread(top);
+        __syncthreads();
+        if (e0 < 256) block_bound(groups, n, &exact);
+        __syncthreads();
+        least = exact;
+    }
+    least = max(least, 1u);
     auto take = [&](const Best& b) {
         const int at = atomicAdd(&count, 1);
-        if (at < kPlaces) place[at] = b;
+        if (at < kJoinPlaces) place[at] = b;
     };
     if (key_of(first.value) >= least) take(first);
     for (int e = e0 + NTJ; e < total; e += NTJ) {
@@ -387,7 +434,7 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     }
     __syncthreads();
     const int found = count;
-    if (found <= kPlaces) {
+    if (found <= kJoinPlaces) {
         for (int i = threadIdx.x; i < found; i += NTJ) {
             const Best b = place[i];
             int rank = 0;
