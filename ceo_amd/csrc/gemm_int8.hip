@@ -20,8 +20,8 @@ static size_t scales_bytes(size_t n) { return (size_t)up_to((long)(n * sizeof(fl
 
 // Whether the weights are streamed past few tokens (few_kernel) or go through tiles.  Up to 64
 // tokens, but for wide outputs, whose tiles fill half the chip, 32: a wave reads all tokens
-// for its 16 channels.  Measured (few / 128-tiles, us; 48 tokens, k x n): 1024 x 4096 8.8 /
-// 10.0, 4096 x 4096 19.4 / 24.3, 1024 x 32000 21.5 / 12.4, 1024 x 128000 70 / 38.
+// for its 16 channels.  Measured (few / 128-tiles, us; 48 tokens, k x n): 1024 x 4096 7.3 / 8.0,
+// 4096 x 4096 12.8 / 19.1, 1024 x 32000 21.5 / 10.4, 1024 x 128000 70 / 36.
 static bool few(long m, long n) {
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     return m <= 32 || (m <= 64 && (n + 127) / 128 < cus / 2);
@@ -32,27 +32,30 @@ static bool few(long m, long n) {
 constexpr long kWaveRows = 2048;
 
 // Whether few_kernel quantises the tokens itself: a second launch is longer than what it takes
-// every workgroup.  (Registers: a lane holds 32 values of its row, 1024 threads of fp32 too many.)
-static bool fused(size_t m, size_t kp, size_t size) {
-    return m <= (size == 2 ? 32 : 16) && kp <= 1024;
+// every workgroup, while rows are short, or the tokens 8 and the weights small (4 x 4096 x 1024
+// 9.0 us, apart 6.5 + 3.4 and the second launch).  What a wave's registers and 64 KiB of
+// LDS hold: 16-bit tokens, 32 of 1024 or 8 of 4096 values.
+static bool fused(size_t m, size_t n, size_t kp, size_t size) {
+    if (kp <= 1024) return m <= (size == 2 ? 32 : 16);
+    return size == 2 && m <= 8 && kp <= 4096 && n <= 16384;
 }
 
-template <typename T, int MT, int HOLD>
+template <typename T, int MT, int LPR, int HOLD>
 static void few_launch(const T* x, long ldx, const uint8_t* xq, const float* xs, const uint8_t* wq,
                        long m, long n, long k, long kp, const Out<T>& o, hipStream_t st) {
-    constexpr long NW = kFewWaves<MT, HOLD>;
+    constexpr long NW = kFewWaves<MT, LPR, HOLD>;
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const long tiles = (n + 15) / 16;
+    const long cols = (n + 15) / 16;
     // waves that split k: until three quarters of the compute units have a workgroup
     long kw = 1;
-    while (kw < NW && tiles * kw < NW * cus * 3 / 4 && kp / 64 / (2 * kw) >= 2) kw *= 2;
+    while (kw < NW && cols * kw < NW * cus * 3 / 4 && kp / 64 / (2 * kw) >= 2) kw *= 2;
     const long cw = NW / kw;
-    const dim3 grid((unsigned)((tiles + cw - 1) / cw)), block(64 * NW);
+    const dim3 grid((unsigned)((cols + cw - 1) / cw)), block(64 * NW);
     const size_t parts = kw > 1 ? (size_t)NW * MT * 64 * 16 : 0;
-    const size_t rows = HOLD ? (size_t)16 * MT * (size_t)(kp + 16) : 0;
+    const size_t rows = HOLD ? (size_t)(64 * NW / LPR) * (size_t)(kp + 16) : 0;
     const size_t lds = 64 * MT + std::max(parts, rows);
-    EFLA_LAUNCH_LDS("linear_int8", (few_kernel<T, MT, HOLD>), grid, block, lds, st, x, ldx, xq, xs,
-                    wq, (int)m, (int)n, k, kp, (int)kw, o);
+    EFLA_LAUNCH_LDS("linear_int8", (few_kernel<T, MT, LPR, HOLD>), grid, block, lds, st, x, ldx,
+                    xq, xs, wq, (int)m, (int)n, k, kp, (int)kw, o);
 }
 
 static long tiles(long m, long n, long ts) { return ((m + ts - 1) / ts) * ((n + ts - 1) / ts); }
@@ -69,16 +72,16 @@ static void tile_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, l
 }
 
 template <typename T, int FORM>
-static void deep_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
+static void lone_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
                         long kp, const Out<T>& o, hipStream_t st) {
     const gf::Opnd A{(const char*)xq, kp / 2, (int)m}, B{(const char*)wq, kp / 2, (int)n};
-    EFLA_LAUNCH("linear_int8", (deep_tile_kernel<T, FORM>), dim3((unsigned)tiles(m, n, 128)),
-                dim3(256), st, A, B, m, n, (int)(kp / kLine), xs, o);
+    EFLA_LAUNCH("linear_int8", (lone_tile_kernel<T, FORM>), dim3((unsigned)tiles(m, n, 128)),
+                dim3(512), st, A, B, m, n, (int)(kp / kLine), xs, o);
 }
 
 static size_t scratch(size_t m, size_t k, size_t n, size_t size) {
     const size_t kp = (size_t)up_to((long)k, kLine);
-    return fused(m, kp, size) ? 0 : scales_bytes(m) + m * kp;
+    return fused(m, n, kp, size) ? 0 : scales_bytes(m) + m * kp;
 }
 
 template <typename T>
@@ -91,7 +94,7 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     const Out<T> o{y, ldy, bias, residual, ldr, sw, gelu};
     float* xs = nullptr;
     uint8_t* xq = nullptr;
-    if (!fused((size_t)m, (size_t)kp, sizeof(T))) {
+    if (!fused((size_t)m, (size_t)n, (size_t)kp, sizeof(T))) {
         xs = (float*)ws;
         xq = ws + scales_bytes((size_t)m);
 #define I8_QUANT(LPR, HOLD)                                                                      \
@@ -106,17 +109,20 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
         EFLA_CHECK(hipPeekAtLastError());
     }
     if (few(m, n)) {
-#define I8_FEW(MT, HOLD) few_launch<T, MT, HOLD>(x, ldx, xq, xs, wq, m, n, k, kp, o, st)
-        if (!xq && m <= 16) {
-            I8_FEW(1, 4);
+#define I8_FEW(MT, LPR, HOLD) \
+    few_launch<T, MT, LPR, HOLD>(x, ldx, xq, xs, wq, m, n, k, kp, o, st)
+        if (!xq && kp > 1024) {
+            if constexpr (sizeof(T) == 2) I8_FEW(1, 64, 8);
+        } else if (!xq && m <= 16) {
+            I8_FEW(1, 32, 4);
         } else if (!xq) {
-            if constexpr (sizeof(T) == 2) I8_FEW(2, 4);
+            if constexpr (sizeof(T) == 2) I8_FEW(2, 32, 4);
         } else if (m <= 16) {
-            I8_FEW(1, 0);
+            I8_FEW(1, 32, 0);
         } else if (m <= 32) {
-            I8_FEW(2, 0);
+            I8_FEW(2, 32, 0);
         } else {
-            I8_FEW(4, 0);
+            I8_FEW(4, 32, 0);
         }
 #undef I8_FEW
         return (int)hipPeekAtLastError();
@@ -126,7 +132,7 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
                        (!bias || (uintptr_t)bias % a == 0) &&
                        (!residual || ((uintptr_t)residual % a == 0 && ldr % 8 == 0));
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const bool large = tiles(m, n, 256) >= cus, deep = tiles(m, n, 128) <= cus;
+    const bool large = tiles(m, n, 256) >= cus, lone = tiles(m, n, 128) <= cus;
     // past the L2s from their 32 MB on (16384 x 1024 x 4096 with a residual 113 -> 104 us, without
     // any 88 to 92 either way)
     const bool past = (size_t)m * (size_t)n * sizeof(T) >= (size_t)32 << 20;
@@ -134,8 +140,8 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     if (large && whole && past) I8_TILE(256, kPast);
     else if (large && whole) I8_TILE(256, kWhole);
     else if (large) I8_TILE(256, kRagged);
-    else if (deep && whole) deep_launch<T, kWhole>(xq, xs, wq, m, n, kp, o, st);
-    else if (deep) deep_launch<T, kRagged>(xq, xs, wq, m, n, kp, o, st);
+    else if (lone && whole) lone_launch<T, kWhole>(xq, xs, wq, m, n, kp, o, st);
+    else if (lone) lone_launch<T, kRagged>(xq, xs, wq, m, n, kp, o, st);
     else if (whole) I8_TILE(128, kWhole);
     else I8_TILE(128, kRagged);
 #undef I8_TILE

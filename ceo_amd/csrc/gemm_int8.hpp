@@ -276,22 +276,24 @@ struct Out {
 // a range of k; the weights are the MFMA's A operand (16 x 16 x 64), read straight from
 // memory, 16 bytes a lane.  kw waves of a workgroup share their channels and split k; their
 // sums meet in LDS.  HOLD > 0: the workgroup quantises the tokens into LDS itself, all rows at
-// once, 32 lanes to a row (8 HOLD elements of each lane in registers).  Loads return in
+// once, LPR lanes to a row (8 HOLD elements of each lane in registers).  Loads return in
 // the order in which they are issued, so the tokens are asked for before the weights and
 // quantised while those are on their way, and what the epilogue needs right behind.  HOLD 0:
-// the tokens are read quantised.
+// the tokens are read quantised (32 channels a wave, so that they are read half as often: 48 x 4096
+// x 1024 16.1 us, 11.9 with 16).
 constexpr int kAhead = 8;  // 64-byte steps of k whose weights a wave has in flight
 // waves of a workgroup: enough that 32 lanes have a row
-template <int MT, int HOLD>
-constexpr int kFewWaves = HOLD > 0 ? 8 * MT : 8;
+template <int MT, int LPR, int HOLD>
+constexpr int kFewWaves = HOLD > 0 && LPR == 32 ? 8 * MT : 8;
 
-template <typename T, int MT, int HOLD>
-__global__ void __launch_bounds__((64 * kFewWaves<MT, HOLD>), sizeof(T) == 2 ? 4 : 2)
+template <typename T, int MT, int LPR, int HOLD>
+__global__ void __launch_bounds__((64 * kFewWaves<MT, LPR, HOLD>),
+                                  sizeof(T) == 2 && HOLD <= 4 ? 4 : 2)
 few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
            const float* __restrict__ xs, const uint8_t* __restrict__ wq, int M, int N, long k,
            long kp, int kw, Out<T> o) {
     constexpr bool FUSED = HOLD > 0;
-    constexpr int NW = kFewWaves<MT, HOLD>;
+    constexpr int NW = kFewWaves<MT, LPR, HOLD>;
     typedef gf::Piece<4, T> P;
     typedef gf::Piece<4, float> F;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -300,7 +302,6 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
     const long n0 = ((long)blockIdx.x * cw + w / kw) * 16;
     const int steps = (int)(kp / 64), s0 = steps * wk / kw, s1 = steps * (wk + 1) / kw;
     const uint8_t* wp = wq + (n0 + r < N ? n0 + r : N - 1) * kp + 16 * g;
-    constexpr int LPR = 32;
     const int own = threadIdx.x / LPR, lr = threadIdx.x % LPR;
     Row<T, LPR, FUSED ? HOLD : 1> row;
     if constexpr (FUSED) row.load(x + own * ldx, own < M ? k : 0, lr);
@@ -335,11 +336,13 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
     int4v acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = int4v{};
+    // (64 lanes a row: LDS has 8 rows, whose products rows 8 to 15 repeat)
     const uint8_t* bp[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int m = 16 * t + r;
-        bp[t] = (FUSED ? rows + m * ldq : xq + (m < M ? m : M - 1) * ldq) + 16 * g;
+        bp[t] = (FUSED ? rows + (LPR == 64 ? r & 7 : m) * ldq : xq + (m < M ? m : M - 1) * ldq) +
+                16 * g;
     }
     for (int s = s0; s < s1; s += kAhead) {
 #pragma unroll
@@ -451,12 +454,6 @@ struct Columns {
 // place of each 16-bit element: 256 x 256 x 128 (eight waves of 128 x 64) or 128 x 128 x 128
 // (four of 64 x 64, two workgroups to a CU), copied straight into LDS one block ahead,
 // MFMA 32 x 32 x 32.  Rows are padded to whole blocks, so there is no tail in k.
-
-// Waits until at most N vector memory operations are under way, whatever the other counters.
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
-}
 
 // A wave's part of the output, rows mw .., columns nw ..: lane l holds for tile (i, j) row
 // mw + 32 j + (l & 31) and columns nw + 32 i + 8 q + 4 (l >> 5) + e in acc[i][j][4 q + e].  They go
@@ -617,55 +614,88 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
 }
 
 // The same for outputs of no more 128 x 128 tiles than there are compute units, each of which has
-// one alone: four buffers, three blocks under way.  Operations end in order, so the wait for a
-// block counts those behind it.  (This / two buffers, us: 65 x 1024 x 1024 9.3 / 10.2, 65 x 4096 x
-// 1024 22.4 / 24.2, 65 x 1024 x 32000 11.1 / 11.9, 517 x 1001 x 3088 10.6 / 11.4.)  What is left
-// is one wave's chain on each SIMD, 0.54 us a block.
-constexpr int kDeep = 4;
-
+// one alone: eight waves in two groups of four that take the blocks of k in turn, two
+// buffers each, and add up in LDS.  A lone tile waits for its one wave a SIMD, not for its
+// loads: four waves with two buffers, with three blocks under way, and this, us:
+//   65 x 1024 x 1024 10.2 / 9.3 / 7.9   65 x 4096 x 1024 24.2 / 22.4 / 18.3
+//   65 x 1024 x 32000 11.9 / 11.1 / 10.8   517 x 1001 x 3088 fp16 11.4 / 10.6 / 9.4
 template <typename T, int FORM>
-__global__ void __launch_bounds__(256)
-deep_tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
+__global__ void __launch_bounds__(512, 2)
+lone_tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
                  Out<T> o) {
     constexpr int TS = 128, TMJ = 2, KS = 4, TILE = gf::tile_bytes<TS>();
-    constexpr int DMA = 2 * (TS / 8 / gf::tile_waves<TS>());  // instructions a wave and block
-    __shared__ __attribute__((aligned(1024))) char smem[kDeep * 2 * TILE];
+    __shared__ __attribute__((aligned(1024))) char smem[4 * 2 * TILE];
     const int tm_n = (int)((M + TS - 1) / TS);
     const int m0 = (int)(blockIdx.x % tm_n) * TS, n0 = (int)(blockIdx.x / tm_n) * TS;
-    const int w = mf::wave(), l = mf::lane();
+    const int wave = mf::wave(), w = wave & 3, group = wave >> 2, l = mf::lane();
     const int wm = (w & 1) * (TS / 2), wn = (w >> 1) * 64;
-    auto fetch = [&](int kt) {
-        if (kt >= niter) return;
-        char* to = smem + (kt % kDeep) * 2 * TILE;
-        gf::copy_tile<true, TS>(A, m0, (long)kt * gf::BK, to, w, l);
-        gf::copy_tile<true, TS>(B, n0, (long)kt * gf::BK, to + TILE, w, l);
+    // the group's block i is block 2 i + group
+    const int mine = (niter + 1 - group) / 2, most = (niter + 1) / 2;
+    char* base = smem + group * 4 * TILE;
+    auto fetch = [&](int i) {
+        if (i >= mine) return;
+        const long k0 = (2L * i + group) * gf::BK;
+        char* to = base + (i & 1) * 2 * TILE;
+        gf::copy_tile<true, TS>(A, m0, k0, to, w, l);
+        gf::copy_tile<true, TS>(B, n0, k0, to + TILE, w, l);
     };
-#pragma unroll
-    for (int kt = 0; kt + 1 < kDeep; ++kt) fetch(kt);
+    fetch(0);
     int16v acc[2][TMJ];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < TMJ; ++j) acc[i][j] = int16v{};
     Steps<TS, TMJ> st;
-    for (int kt = 0; kt < niter; ++kt) {
-        const int behind = niter - 1 - kt;  // blocks after this one: two at most are under way
-        if (behind >= 2) wait_vm<2 * DMA>();
-        else if (behind == 1) wait_vm<DMA>();
-        else mf::dma_wait();
+    for (int i = 0; i < most; ++i) {
+        mf::dma_wait();
         __syncthreads();
-        // every wave has read the block before: its buffer takes the one three ahead
-        fetch(kt + kDeep - 1);
-        const char *as = smem + (kt % kDeep) * 2 * TILE, *bs = as + TILE;
-        st.read(0, as, bs, wm, wn, 0, l);
+        // every wave has read the block before: its buffer takes the next
+        fetch(i + 1);
+        if (i < mine) {
+            const char *as = base + (i & 1) * 2 * TILE, *bs = as + TILE;
+            st.read(0, as, bs, wm, wn, 0, l);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if (ks + 1 < KS) st.read((ks + 1) & 1, as, bs, wm, wn, ks + 1, l);
-            st.mma(ks & 1, acc);
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) st.read((ks + 1) & 1, as, bs, wm, wn, ks + 1, l);
+                st.mma(ks & 1, acc);
+            }
         }
     }
-    __syncthreads();  // the last block has been read
-    tile_epilogue<T, FORM>(o, acc, xs, (long)m0 + wm, (long)n0 + wn, M, N, l, smem + 8192 * w);
+    // the second group's sums through LDS, 16 KB a wave; each group then finishes half of the rows
+    __syncthreads();
+    int4v* part = reinterpret_cast<int4v*>(smem) + 1024 * w;
+    auto pass = [&](int j, bool put) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                int4v& at = part[((j * 2 + i) * 4 + q) * 64 + l];
+                int4v v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                        acc[i][j][4 * q + 3]};
+                if (put) {
+                    at = v;
+                } else {
+                    v += at;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
+                }
+            }
+    };
+    // rows 32 j of a wave's 64 are group j's
+    if (group == 0) pass(1, true);
+    else pass(0, true);
+    __syncthreads();
+    int16v half[2][1];
+    if (group == 0) {
+        pass(0, false);
+        half[0][0] = acc[0][0], half[1][0] = acc[1][0];
+    } else {
+        pass(1, false);
+        half[0][0] = acc[0][1], half[1][0] = acc[1][1];
+    }
+    __syncthreads();
+    tile_epilogue<T, FORM, 1>(o, half, xs, (long)m0 + wm + 32 * group, (long)n0 + wn, M, N, l,
+                              smem + 8192 * wave);
 }
 
 }  // namespace i8
