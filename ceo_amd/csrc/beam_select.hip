@@ -7,7 +7,8 @@
 // else.  A beam whose score is not finite, or whose logits have no finite sum of
 // exponentials (a NaN, +inf, -inf everywhere), offers nothing: its values are -inf.
 //
-// The logits are read once and nothing of their size is written.  Two launches:
+// The logits are read once and nothing of their size is written.  Two launches (or one where a
+// text is small, text_kernel):
 //
 // slice_kernel: a workgroup takes a slice of one row, 1 to 4 16-byte vectors a thread, in
 // registers.  Maximum and sum of exponentials are each thread's own first (no barrier
@@ -318,6 +319,112 @@ __device__ __forceinline__ bool better(const Best& a, const Best& b) {
     return a.token < b.token;
 }
 
+// Whole numbers in the values' order, 0: not a candidate.
+__device__ __forceinline__ uint32_t key_of(double v) {
+    return v > -(double)INFINITY ? (uint32_t)(ordered(v + 0.0) >> 32) : 0u;
+}
+
+// What a text's selection is written to.
+struct Selected {
+    float* scores;
+    int* parents;
+    int* tokens;
+    uint8_t* finished;
+};
+
+// The n best of the candidates in `place`, or, where it has not held them all (equal values), of
+// those that `each` hands to a function, a thread its own, into `res` in order; all threads.
+template <int NTJ, typename Each>
+__device__ __forceinline__ void rank(int found, int n, int beams, const Best* place, Best* res,
+                                     Best* wbest, Each each) {
+    if (found <= kJoinPlaces) {
+        for (int i = threadIdx.x; i < found; i += NTJ) {
+            const Best b = place[i];
+            int rank = 0;
+            // without branches, so that the reads need not wait for each other
+#pragma unroll 4
+            for (int k = 0; k < found; ++k) {
+                const Best x = place[k];
+                const bool before = (x.beam < b.beam) | ((x.beam == b.beam) & (x.token < b.token));
+                rank += (x.value > b.value) | ((x.value == b.value) & before);
+            }
+            if (rank < n) res[rank] = b;
+        }
+    } else {
+        // the best, then the best behind it, n times
+        Best last{(double)INFINITY, -1, -1};
+        for (int r = 0; r < n; ++r) {
+            Best b{-(double)INFINITY, beams, 0};
+            each([&](const Best& x) {
+                if (x.value > -(double)INFINITY && better(last, x) && better(x, b)) b = x;
+            });
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                const Best x{__shfl_xor(b.value, o), __shfl_xor(b.beam, o),
+                             __shfl_xor(b.token, o)};
+                if (better(x, b)) b = x;
+            }
+            __syncthreads();  // `wbest` has been read
+            if (lane_id() == 0) wbest[wave_id()] = b;
+            __syncthreads();
+            last = wbest[0];
+#pragma unroll
+            for (int k = 1; k < NTJ / kWave; ++k)
+                if (better(wbest[k], last)) last = wbest[k];
+            if (threadIdx.x == 0) res[r] = last;
+        }
+    }
+    __syncthreads();
+}
+
+// The selected, the first wave's.
+__device__ __forceinline__ void write(Best* res, int found, int n, int V, long text, long row0,
+                                      const uint8_t* finished, int end_token, int keep_slots,
+                                      const Selected& out) {
+    if (wave_id() != 0) return;
+    const int r = lane_id();
+    // fewer finite values than asked for: the lowest pairs that are not among them
+    if (found < n) {
+        if (r == 0) {
+            int beam = 0, token = 0;
+            for (int to = found; to < n;) {
+                bool taken = false;
+                for (int k = 0; k < found; ++k)
+                    taken |= res[k].beam == beam && res[k].token == token;
+                if (!taken) res[to++] = Best{-(double)INFINITY, beam, token};
+                if (++token == V) token = 0, ++beam;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    const Best b = res[r < n ? r : n - 1];
+    int to = r;
+    if (keep_slots) {
+        // the first child of a beam takes that beam's slot, the others the free ones in order
+        uint64_t used = 0;
+        bool first = true;
+        for (int k = 0; k < n; ++k) {
+            const int other = __builtin_amdgcn_readlane(b.beam, k);
+            used |= 1ull << other;
+            if (k < r && other == b.beam) first = false;
+        }
+        const uint64_t late = __ballot(!first && r < n);
+        to = b.beam;
+        if (!first) {
+            uint64_t open = ~used;
+            for (int k = __popcll(late & ((1ull << r) - 1)); k > 0; --k) open &= open - 1;
+            to = __ffsll((unsigned long long)open) - 1;
+        }
+    }
+    if (r >= n) return;
+    const long at = text * n + to;
+    out.scores[at] = (float)b.value;
+    out.parents[at] = b.beam;
+    out.tokens[at] = b.token;
+    if (out.finished)
+        out.finished[at] = (finished && finished[row0 + b.beam]) || b.token == end_token;
+}
+
 constexpr int kHeads = 2;
 
 // An entry a thread is held, NTJ of them; more are read twice.  (Eight entries a thread: 17 KB
@@ -327,9 +434,7 @@ template <int NTJ>
 __global__ void __launch_bounds__(NTJ)
 join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, int slices,
             const float* __restrict__ scores, const uint8_t* __restrict__ finished, int V,
-            int beams, int n, int end_token, int keep_slots, float* __restrict__ out_scores,
-            int* __restrict__ out_parents, int* __restrict__ out_tokens,
-            uint8_t* __restrict__ out_finished) {
+            int beams, int n, int end_token, int keep_slots, Selected out) {
     __shared__ double offset[kMaxBeams];  // score - log sum exp; -inf: offers nothing
     __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
     __shared__ Best place[kJoinPlaces];
@@ -399,10 +504,6 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         }
         return b;
     };
-    // 0: not a candidate
-    auto key_of = [](double v) {
-        return v > -(double)INFINITY ? (uint32_t)(ordered(v + 0.0) >> 32) : 0u;
-    };
     const Best first = best_of(e0, held);
     // The bound from the largest of some lists: 64 lanes', in every wave by itself, or 256 threads'.
     uint32_t top = 0;
@@ -434,87 +535,133 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     }
     __syncthreads();
     const int found = count;
-    if (found <= kJoinPlaces) {
-        for (int i = threadIdx.x; i < found; i += NTJ) {
-            const Best b = place[i];
-            int rank = 0;
-            // without branches, so that the reads need not wait for each other
-#pragma unroll 4
-            for (int k = 0; k < found; ++k) {
-                const Best x = place[k];
-                const bool before = (x.beam < b.beam) | ((x.beam == b.beam) & (x.token < b.token));
-                rank += (x.value > b.value) | ((x.value == b.value) & before);
-            }
-            if (rank < n) res[rank] = b;
-        }
-    } else {
-        // too many (equal values): the best, then the best behind it, n times
-        Best last{(double)INFINITY, -1, -1};
-        for (int r = 0; r < n; ++r) {
-            Best b{-(double)INFINITY, beams, 0};
-            for (int e = threadIdx.x; e < total; e += NTJ) {
-                const Best x = best_of(e, mine[e]);
-                if (x.value > -(double)INFINITY && better(last, x) && better(x, b)) b = x;
-            }
+    rank<NTJ>(found, n, beams, place, res, wbest, [&](auto f) {
+        for (int e = e0; e < total; e += NTJ) f(best_of(e, mine[e]));
+    });
+    write(res, found, n, V, text, row0, finished, end_token, keep_slots, out);
+}
+
+// A whole text in a workgroup, for texts of few logits (kTextLogits), where a second launch is
+// longer than the work: each beam is some waves', and what slice_kernel and join_kernel
+// do follows in one place.  The logits that the bound leaves are few threads', which
+// read theirs again.  A call through Python, this and both launches, us (bf16 unless said):
+//   1 x 2 x 798 11.0 / 15.5   1 x 4 x 8000 11.2 / 15.3   256 x 4 x 8000 11.2 / 15.3
+//   85 x 5 x 7936 fp32 11.2 / 15.9   1000 x 4 x 2000 22 / 30   1 x 4 x 32000 20.3 / 15.3
+constexpr int kTextThreads = 1024, kTextBeams = kTextThreads / kWave;
+constexpr size_t kTextLogits = 49152;
+
+template <typename T>
+__global__ void __launch_bounds__(kTextThreads)
+text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
+            const float* __restrict__ scores, const uint8_t* __restrict__ finished, int end_token,
+            int keep_slots, Selected out) {
+    constexpr int N = 16 / sizeof(T), NTJ = kTextThreads, W = NTJ / kWave, U = 4;
+    typedef __attribute__((__vector_size__(16))) T Vec;
+    __shared__ double offset[kTextBeams];  // score - log sum exp; -inf: offers nothing
+    __shared__ Best place[kJoinPlaces];
+    __shared__ Best res[kMaxSelect];
+    __shared__ Best wbest[W];
+    __shared__ float wm[W], ws[W];
+    __shared__ uint32_t groups[NTJ];
+    __shared__ int count;
+    const long text = blockIdx.x, row0 = text * beams;
+    if (threadIdx.x == 0) count = 0;
+    const int waves = W / beams, P = waves * kWave;  // a beam's
+    const int k = wave_id() / waves, t = (int)threadIdx.x - k * P;
+    const bool has = k < beams;
+    const float score = has ? scores[row0 + k] : -INFINITY;
+    const bool ok = fabsf(score) < INFINITY, fin = has && finished && finished[row0 + k];
+    const bool live = ok && !fin;  // a beam that offers no continuation is not read
+    // the row's vectors from 16-byte boundaries on, and the elements before and behind them
+    const T* p = logits + (row0 + (has ? k : 0)) * ld;
+    const int to16 = (int)(-(uintptr_t)p % 16 / sizeof(T)), head = to16 < V ? to16 : V;
+    const int nv = live ? (V - head) / N : 0, edges = live ? V - nv * N : 0;
+    const Vec* q = reinterpret_cast<const Vec*>(p + head);
+    const int edge = t < head ? t : t + nv * N;
+    float m = -INFINITY, s = 0.f;
+    auto add = [&](float top, auto sum_of) {  // logits whose largest is `top`
+        const float now = fmaxf(m, top) + 0.f, m0 = now == -INFINITY ? 0.f : now;
+        s = s * exp_diff(fminf(m - m0, 0.f)) + sum_of(m0);
+        m = now;
+    };
+    for (int v0 = t; v0 < nv; v0 += U * P) {
+        Vec x[U];
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                const Best x{__shfl_xor(b.value, o), __shfl_xor(b.beam, o),
-                             __shfl_xor(b.token, o)};
-                if (better(x, b)) b = x;
-            }
-            __syncthreads();  // `wbest` has been read
-            if (lane_id() == 0) wbest[wave_id()] = b;
-            __syncthreads();
-            last = wbest[0];
+        for (int i = 0; i < U; ++i) {
 #pragma unroll
-            for (int k = 1; k < NTJ / kWave; ++k)
-                if (better(wbest[k], last)) last = wbest[k];
-            if (threadIdx.x == 0) res[r] = last;
+            for (int j = 0; j < N; ++j) x[i][j] = (T)-INFINITY;
+            if (v0 + i * P < nv) x[i] = q[v0 + i * P];
         }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < U; ++i) top = fmaxf(top, vec_max<T>(x[i]));
+        add(top, [&](float m0) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum += exp_diff(to_f(x[i][j]) - m0);
+            return sum;
+        });
+    }
+    if (t < edges) {
+        const float z = to_f(p[edge]);
+        add(z, [&](float m0) { return exp_diff(z - m0); });
+    }
+    const float M = wave_max(m), M0 = M == -INFINITY ? 0.f : M;
+    const float sum = wave_sum(s * exp_diff(fminf(m == -INFINITY ? 0.f : m - M0, 0.f)));
+    if (lane_id() == 0) {
+        wm[wave_id()] = M;
+        ws[wave_id()] = sum;
     }
     __syncthreads();
-    if (wave_id() != 0) return;
-    const int r = lane_id();
-    // fewer finite values than asked for: the lowest pairs that are not among them
-    if (found < n) {
-        if (r == 0) {
-            int beam = 0, token = 0;
-            for (int to = found; to < n;) {
-                bool taken = false;
-                for (int k = 0; k < found; ++k)
-                    taken |= res[k].beam == beam && res[k].token == token;
-                if (!taken) res[to++] = Best{-(double)INFINITY, beam, token};
-                if (++token == V) token = 0, ++beam;
-            }
+    if (has && t == 0) {
+        float Mb = -INFINITY;
+        for (int i = 0; i < waves; ++i) Mb = fmaxf(Mb, wm[k * waves + i]);
+        double S = 0.0;
+        for (int i = 0; i < waves; ++i) {
+            const float a = wm[k * waves + i], b = ws[k * waves + i];
+            S += a < Mb ? (double)b * (double)exp_diff(a - Mb) : (double)b;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const double lse = fin ? 0.0 : (double)Mb + log(S);
+        offset[k] = ok && fabs(lse) < (double)INFINITY ? (double)score - lse : -(double)INFINITY;
     }
-    const Best b = res[r < n ? r : n - 1];
-    int to = r;
-    if (keep_slots) {
-        // the first child of a beam takes that beam's slot, the others the free ones in order
-        uint64_t used = 0;
-        bool first = true;
-        for (int k = 0; k < n; ++k) {
-            const int other = __builtin_amdgcn_readlane(b.beam, k);
-            used |= 1ull << other;
-            if (k < r && other == b.beam) first = false;
+    __syncthreads();
+    const double off = has ? offset[k] : -(double)INFINITY;
+    // a thread's candidates whose keys are no less than `from`, and some that are; a finished
+    // beam has one
+    auto each = [&](uint32_t from, auto f) {
+        if (!(off > -(double)INFINITY)) return;
+        if (fin) {
+            if (t == 0) f(Best{off, k, end_token});
+            return;
         }
-        const uint64_t late = __ballot(!first && r < n);
-        to = b.beam;
-        if (!first) {
-            uint64_t open = ~used;
-            for (int k = __popcll(late & ((1ull << r) - 1)); k > 0; --k) open &= open - 1;
-            to = __ffsll((unsigned long long)open) - 1;
+        for (int v = t; v < nv; v += P) {
+            const Vec x = q[v];
+            if (key_of((double)(vec_max<T>(x) + 0.f) + off) < from) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                f(Best{(double)(to_f(x[j]) + 0.f) + off, k, head + v * N + j});
         }
-    }
-    if (r >= n) return;
-    const long at = text * n + to;
-    out_scores[at] = (float)b.value;
-    out_parents[at] = b.beam;
-    out_tokens[at] = b.token;
-    if (out_finished)
-        out_finished[at] = (finished && finished[row0 + b.beam]) || b.token == end_token;
+        if (t < edges) f(Best{(double)(to_f(p[edge]) + 0.f) + off, k, edge});
+    };
+    const uint32_t mine = fin ? (t == 0 ? key_of(off) : 0u) : key_of((double)m + off);
+    groups[threadIdx.x] = mine;
+    __syncthreads();
+    uint32_t group = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) group = max(group, groups[lane_id() + i * kWave]);
+    const uint32_t least = max(wave_bound<4>(group, n), 1u);
+    if (mine >= least)
+        each(least, [&](const Best& b) {
+            if (key_of(b.value) < least) return;
+            const int at = atomicAdd(&count, 1);
+            if (at < kJoinPlaces) place[at] = b;
+        });
+    __syncthreads();
+    const int found = count;
+    rank<NTJ>(found, n, beams, place, res, wbest, [&](auto f) { each(1, f); });
+    write(res, found, n, V, text, row0, finished, end_token, keep_slots, out);
 }
 
 static size_t dtype_size(int d) {
@@ -534,7 +681,13 @@ static size_t slices_of(size_t vocab, size_t size, int vpt, bool lines) {
     return (vocab + shift + l - 1) / l;
 }
 
+// Whether a text is one workgroup's.
+static bool one_workgroup(size_t beams, size_t vocab, size_t n) {
+    return beams <= kTextBeams && n <= kFewSelect && beams * vocab <= kTextLogits;
+}
+
 static size_t scratch(size_t batch, size_t beams, size_t vocab, size_t n) {
+    if (one_workgroup(beams, vocab, n)) return 0;
     // whatever the type and the alignment: 4-byte logits, one vector a thread
     const size_t slices = slices_of(vocab, 4, 1, false);
     return batch * beams * slices * (sizeof(float2) + n * sizeof(Cand));
@@ -595,6 +748,18 @@ extern "C" int beam_select_hip(const void* logits, const float* scores, const ui
     if (vocab_size > 0x3FFFFFFFull || !mul_ok(batch, beams, &rows) || rows > 0x7FFFFFFFull ||
         !mul_ok(rows, ld, size, &elems) || elems > (1ull << 62))
         return kInvalidConfiguration;
+    const bs::Selected out{out_scores, out_parents, out_tokens, out_finished};
+    if (bs::one_workgroup(beams, vocab_size, select)) {
+#define BS_TEXT(T)                                                                                \
+    EFLA_LAUNCH("beam_text", bs::text_kernel<T>, dim3((unsigned)batch), dim3(bs::kTextThreads),  \
+                stream, (const T*)logits, (long)ld, (int)vocab_size, (int)beams, (int)select,    \
+                scores, finished, (int)end_token, keep_slots, out)
+        if (dtype == kDtypeBF16) BS_TEXT(bf16);
+        else if (dtype == kDtypeF16) BS_TEXT(f16);
+        else BS_TEXT(float);
+#undef BS_TEXT
+        return (int)hipPeekAtLastError();
+    }
     const size_t need = bs::scratch(batch, beams, vocab_size, select);
     void* ws = workspace;
     WsLease lease;
@@ -621,8 +786,7 @@ extern "C" int beam_select_hip(const void* logits, const float* scores, const ui
 #define BS_JOIN(NTJ)                                                                             \
     EFLA_LAUNCH("beam_join", bs::join_kernel<NTJ>, dim3((unsigned)batch), dim3(NTJ), stream, stats, \
                 (const bs::Cand*)(stats + rows * slices), (int)slices, scores, finished,          \
-                (int)vocab_size, (int)beams, (int)select, (int)end_token, keep_slots, out_scores, \
-                out_parents, out_tokens, out_finished)
+                (int)vocab_size, (int)beams, (int)select, (int)end_token, keep_slots, out)
     if (beams * slices * select <= 256) BS_JOIN(256);
     else BS_JOIN(1024);
 #undef BS_JOIN

@@ -689,7 +689,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, select=None, finishe
     parents, tokens = torch.empty(2, B, n, dtype=torch.int32, device=dev).unbind(0)
     ended = None if end_token is None else torch.empty(B, n, dtype=torch.bool, device=dev)
     wsb = lib().beam_select_workspace_size(B, K, V, n)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     rc = lib().beam_select_hip(
         _p(logits), _p(scores), _p(finished), _p(out), _p(parents), _p(tokens), _p(ended), B, K, V,
         ld, n, -1 if end_token is None else int(end_token), int(keep_slots), dt, _p(ws), wsb,

@@ -37,9 +37,10 @@ def test_select_refusals(L):
     assert _select(L, keep=1, n=4) == 1                          # slots are the beams'
     assert _select(L, fin=P) == 1 and _select(L, of=P) == 1      # without an end token
     assert _select(L, fin=P, end=100) == 1 and _select(L, of=P, end=-2) == 1
-    need = L.beam_select_workspace_size(2, 3, 100, 3)
-    assert need > 0 and _select(L, wsb=need - 1) == 1
-    assert _select(L, ws=ctypes.c_void_p(4100)) == 1
+    big = dict(vocab=50000, ld=50000)
+    need = L.beam_select_workspace_size(2, 3, 50000, 3)
+    assert need > 0 and _select(L, wsb=need - 1, **big) == 1
+    assert _select(L, ws=ctypes.c_void_p(4100), **big) == 1
     assert _select(L, vocab=1 << 30, ld=1 << 30) == 9
     assert _select(L, batch=BIG) == 9
     assert _select(L, ld=BIG) == 9
@@ -48,13 +49,16 @@ def test_select_refusals(L):
 
 
 def test_select_workspace_holds_every_cut(L):
-    """Monotonic in the vocabulary and the rows, 0 out of range."""
+    """Monotonic in the vocabulary and the rows, 0 where a text is one workgroup's and out of
+    range."""
     size = L.beam_select_workspace_size
     last = 0
-    for v in (1, 31, 1000, 4096, 50257, 128003, 1 << 20):
+    for v in (6145, 50257, 128003, 1 << 20):
         got = size(4, 8, v, 8)
         assert got >= max(last, 4 * 8 * (8 + 8 * 8))
         last = got
+    assert size(4, 8, 6144, 8) == 0 and size(4, 8, 1, 8) == 0
+    assert size(4, 17, 100, 8) > 0 and size(4, 8, 100, 33) > 0
     assert size(1, 65, 100, 3) == 0 and size(1, 3, 100, 65) == 0 and size(1, 3, 1 << 30, 3) == 0
     assert size(BIG, 3, 100, 3) == 0
 

@@ -132,6 +132,9 @@ def texts(B, K, V, dtype, seed=0, scale=2.5):
     (1, 1, 1, 1), (1, 1, 2, 2), (2, 3, 1, 3), (1, 4, 7, 8), (3, 2, 63, 4), (2, 5, 257, 5),
     (1, 4, 4099, 4), (2, 8, 5003, 16), (5, 16, 1000, 32), (1, 64, 300, 64), (2, 64, 129, 64),
     (1, 2, 50257, 64), (40, 4, 2048, 4), (300, 4, 9000, 8), (1, 1, 131072, 1), (2, 3, 128003, 6),
+    # a text is one workgroup's up to 49152 logits, 16 beams and 32 selected
+    (2, 4, 12288, 4), (2, 4, 12289, 4), (3, 16, 3071, 32), (3, 17, 500, 17), (3, 16, 500, 33),
+    (2, 7, 7001, 14), (2, 1, 49153, 2), (600, 2, 300, 2),
 ])
 def test_select(dtype, B, K, V, n):
     announce(f"select {dtype} {B} {K} {V} {n}")
@@ -196,8 +199,9 @@ def test_select_masks(dtype):
 @pytest.mark.parametrize("n", [1, 4, 64])
 def test_select_ties(dtype, n):
     """Equal logits, in whole rows and in places, and -0 beside 0: the lowest token first."""
-    z = torch.zeros(2 * 4, 8192, dtype=dtype)
     s = torch.tensor([[-1.0, -1.0, -2.0, -1.5], [-3.0, -math.inf, -2.5, -2.5]])
+    check_select(torch.zeros(2 * 4, 20480, dtype=dtype), s, n, exact=True)
+    z = torch.zeros(2 * 4, 8192, dtype=dtype)
     check_select(z, s, n, exact=True)
     z[:, 5::2] = -0.0
     check_select(z, s, n, exact=True)
