@@ -60,6 +60,18 @@ static void few_launch(const T* x, long ldx, const uint8_t* xq, const float* xs,
 
 static long tiles(long m, long n, long ts) { return ((m + ts - 1) / ts) * ((n + ts - 1) / ts); }
 
+// Whether 256-tiles, one to a compute unit, are the faster ones, 128-tiles two: rounds of what the
+// chip holds, of 1.67 / 1.0 us a block of k and 7.3 / 4.4 us for the epilogue and the
+// first block.  (Measured with either, us: 16384 x 1024 x 1024 24.5 / 27.7, 16384 x 2048 x 1024 38 / 44,
+// 16384 x 1024 x 4096 88 / 95, 1463 x 80 x 12070 21.7 / 20.1.)
+static bool large_tiles(long m, long n, long kp) {
+    const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    const double it = (double)(kp / kLine);
+    const long big = (tiles(m, n, 256) + cus - 1) / cus;
+    const long small = (tiles(m, n, 128) + 2 * cus - 1) / (2 * cus);
+    return (double)big * (1.67 * it + 7.3) < (double)small * (1.0 * it + 4.4);
+}
+
 template <typename T, int TS, int FORM>
 static void tile_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
                         long kp, const Out<T>& o, hipStream_t st) {
@@ -132,7 +144,7 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
                        (!bias || (uintptr_t)bias % a == 0) &&
                        (!residual || ((uintptr_t)residual % a == 0 && ldr % 8 == 0));
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const bool large = tiles(m, n, 256) >= cus, lone = tiles(m, n, 128) <= cus;
+    const bool lone = tiles(m, n, 128) <= cus, large = !lone && large_tiles(m, n, kp);
     // past the L2s from their 32 MB on (16384 x 1024 x 4096 with a residual 113 -> 104 us, without
     // any 88 to 92 either way)
     const bool past = (size_t)m * (size_t)n * sizeof(T) >= (size_t)32 << 20;
