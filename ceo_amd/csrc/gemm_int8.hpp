@@ -271,6 +271,21 @@ struct Out {
     int gelu;
 };
 
+// acc sx sw + bias.  A token of values near the type's largest: acc sx may pass fp32's range
+// where the weights are small, so it is taken 2^-64 times as large (acc is below 2^31).
+template <typename T, typename Acc, typename Sw, typename Bias, int N>
+__device__ __forceinline__ void scaled(float (&v)[N], const Acc& acc, float sx, const Sw& sw,
+                                       const Bias& bias) {
+    if (!__is_same(T, f16) && __builtin_expect(sx > 0x1p96f, 0)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            v[e] = fmaf((float)acc[e] * (sx * 0x1p-64f) * sw[e], 0x1p64f, (float)bias[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = fmaf((float)acc[e] * sx, sw[e], (float)bias[e]);
+    }
+}
+
 // --- few rows -------------------------------------------------------------------------
 // M <= 16 MT rows.  Bound by the weight, which is read once.  A wave takes 16 channels and
 // a range of k; the weights are the MFMA's A operand (16 x 16 x 64), read straight from
@@ -374,13 +389,14 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
         const int m = 16 * t + r;
         if (m >= M || !mine) continue;
         const float sx = FUSED ? sc[m] : xs[m];
+        float v[4];
+        scaled<T>(v, acc[t], sx, sw, bias);
         typename P::vec y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float v = fmaf((float)acc[t][e] * sx, sw[e], (float)bias[e]);
-            if (o.gelu) v = gelu::gelu_f<true>(v);
-            if (o.residual) v += (float)res[t][e];
-            y[e] = (T)v;
+            if (o.gelu) v[e] = gelu::gelu_f<true>(v[e]);
+            if (o.residual) v[e] += (float)res[t][e];
+            y[e] = (T)v[e];
         }
         P::store(o.y + m * o.ldy + n, y, N - n);
     }
@@ -428,8 +444,7 @@ struct Columns {
     __device__ __forceinline__ void finish(const Out<T>& o, long m, const int (&acc)[8],
                                            const Rows& r, int s) const {
         float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf((float)acc[e] * r.sx[s], sw[e], bias[e]);
+        scaled<T>(v, acc, r.sx[s], sw, bias);
         if (o.gelu) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = gelu::gelu_f<true>(v[e]);

@@ -491,6 +491,17 @@ def test_linear_special_rows(m, dtype):
         check_linear(x, w)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k,n", [(3, 300, 40), (40, 2000, 40), (100, 300, 40), (2100, 256, 3088)])
+def test_linear_large_tokens_small_weights(m, k, n, dtype):
+    """A sum times its token's scale is past fp32's range, the result is not."""
+    x, w, b, r = operands(m, k, n, dtype)
+    x, w = (x.float() * 4e36).to(dtype), (w.float() * 1e-36).to(dtype)
+    x[0] = 0
+    check_linear(x, w)
+    check_linear(x, w, b, r)
+
+
 @pytest.mark.parametrize("m", [1, 80])
 def test_linear_quotients_on_halves(m):
     """Values on and next to half a step: to the even one, as the exact quotient decides.  The
