@@ -37,6 +37,7 @@ namespace bs {
 
 constexpr int NT = 256, NWV = NT / kWave;
 constexpr int kMaxSelect = 64, kMaxBeams = 64;
+constexpr size_t kMaxBatch = (1 << 22) - 1;  // 1024 threads each, fewer than 2^32 in a launch
 constexpr int kPlaces = 512;   // candidates that LDS holds, a slice's
 constexpr int kJoinPlaces = 2048;  // and a text's
 constexpr int kVectors = 512;  // and 16-byte vectors that have some
@@ -723,7 +724,7 @@ using namespace efla;
 extern "C" size_t beam_select_workspace_size(size_t batch, size_t beams, size_t vocab_size,
                                              size_t select) {
     if (beams > bs::kMaxBeams || select > bs::kMaxSelect || vocab_size > 0x3FFFFFFFull ||
-        batch > (1ull << 31) / (beams ? beams : 1))
+        batch > bs::kMaxBatch)
         return 0;
     return bs::scratch(batch, beams, vocab_size, select);
 }
@@ -745,7 +746,7 @@ extern "C" int beam_select_hip(const void* logits, const float* scores, const ui
     if (!logits || !scores || !out_scores || !out_parents || !out_tokens) return kInvalidValue;
     if ((uintptr_t)logits % size) return kInvalidValue;
     size_t rows, elems;
-    if (vocab_size > 0x3FFFFFFFull || !mul_ok(batch, beams, &rows) || rows > 0x7FFFFFFFull ||
+    if (vocab_size > 0x3FFFFFFFull || batch > bs::kMaxBatch || !mul_ok(batch, beams, &rows) ||
         !mul_ok(rows, ld, size, &elems) || elems > (1ull << 62))
         return kInvalidConfiguration;
     const bs::Selected out{out_scores, out_parents, out_tokens, out_finished};

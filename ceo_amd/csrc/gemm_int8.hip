@@ -12,6 +12,8 @@ namespace efla {
 namespace i8 {
 
 constexpr size_t kMaxK = 131072;  // 127^2 of them stay below 2^31
+// a row's 256 threads, and 4 a channel, are fewer than 2^32 in a launch
+constexpr size_t kMaxM = (1 << 24) - 1, kMaxN = (1 << 29) - 1;
 
 static size_t dtype_size(int d) {
     return d == kDtypeF32 ? 4 : d == kDtypeF16 || d == kDtypeBF16 ? 2 : 0;
@@ -183,7 +185,7 @@ static int pack(const T* w, long ld, uint8_t* packed, long k, long n, hipStream_
 using namespace efla;
 
 extern "C" size_t int8_weight_size(size_t k, size_t n) {
-    if (k == 0 || k > i8::kMaxK || n == 0 || n > 0x3FFFFFFFull) return 0;
+    if (k == 0 || k > i8::kMaxK || n == 0 || n > i8::kMaxN) return 0;
     return i8::scales_bytes(n) + n * (size_t)i8::up_to((long)k, i8::kLine);
 }
 
@@ -192,7 +194,7 @@ extern "C" int int8_weight_pack_hip(const void* weight, size_t ld, void* packed,
     const size_t size = i8::dtype_size(dtype);
     if (size == 0 || k == 0 || n == 0 || ld < n || !weight || !packed) return kInvalidValue;
     if ((uintptr_t)weight % size || (uintptr_t)packed % i8::kLine) return kInvalidValue;
-    if (k > i8::kMaxK || n > 0x3FFFFFFFull || ld > (1ull << 40)) return kInvalidConfiguration;
+    if (k > i8::kMaxK || n > i8::kMaxN || ld > (1ull << 40)) return kInvalidConfiguration;
     if (dtype == kDtypeBF16)
         return i8::pack((const bf16*)weight, (long)ld, (uint8_t*)packed, (long)k, (long)n, stream);
     if (dtype == kDtypeF16)
@@ -202,7 +204,7 @@ extern "C" int int8_weight_pack_hip(const void* weight, size_t ld, void* packed,
 
 extern "C" size_t linear_int8_workspace_size(size_t m, size_t k, size_t n, int dtype) {
     const size_t size = i8::dtype_size(dtype);
-    if (size == 0 || k == 0 || k > i8::kMaxK || n == 0 || n > 0x3FFFFFFFull || m > 0x3FFFFFFFull)
+    if (size == 0 || k == 0 || k > i8::kMaxK || n == 0 || n > i8::kMaxN || m > i8::kMaxM)
         return 0;
     return i8::scratch(m, k, n, size);
 }
@@ -214,7 +216,7 @@ extern "C" int linear_int8_hip(const void* x, size_t ldx, const void* packed, co
                                hipStream_t stream) {
     const size_t size = i8::dtype_size(dtype);
     if (size == 0 || k == 0 || n == 0) return kInvalidValue;
-    if (k > i8::kMaxK || n > 0x3FFFFFFFull || m > 0x3FFFFFFFull || ldx > (1ull << 40) ||
+    if (k > i8::kMaxK || n > i8::kMaxN || m > i8::kMaxM || ldx > (1ull << 40) ||
         ld_output > (1ull << 40) || ld_residual > (1ull << 40))
         return kInvalidConfiguration;
     if (m == 0) return kSuccess;

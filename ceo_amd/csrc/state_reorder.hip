@@ -28,6 +28,7 @@ constexpr int NT = 256;
 constexpr int kMaxBeams = 64;
 // 16-byte vectors for up to this many beams (64 registers); more go in 4-byte ones
 constexpr size_t kWideBeams = 16;
+constexpr size_t kMaxUnits = (1 << 24) - 1;  // 256 threads each, fewer than 2^32 in a launch
 
 struct Entry {
     const uint8_t* in;
@@ -136,7 +137,7 @@ extern "C" int state_list_create_hip(void** list, void* const* states, void* con
         const size_t cols = (e.row + sr::NT * e.width - 1) / (sr::NT * e.width);
         units += cols * batch;
         e.cols = (uint32_t)cols;
-        if (units > 0x7FFFFFFFull) rc = kInvalidConfiguration;
+        if (units > sr::kMaxUnits) rc = kInvalidConfiguration;
         const size_t all = batch * beams * e.row;
         if (all == 0) continue;
         spans[n++] = sr::Span{(uintptr_t)e.in, (uintptr_t)e.in + all};

@@ -171,7 +171,8 @@ class StateList:
 def reorder(states: StateList, parents: torch.Tensor) -> None:
     """Row (b, j) of every state becomes what row (b, parents[b, j]) was: the beams' states in
     the order that ``nn.beam_select`` left them.  parents (batch, beams) int32; one outside of
-    0 .. beams - 1 leaves its row as it is.  In place, rows that stay are not touched."""
+    0 .. beams - 1 leaves its row as it is; parents is not one of the list's tensors.  In place,
+    rows that stay are not touched."""
     if not isinstance(states, StateList):
         raise TypeError("states must be a StateList")
     efla._require(parents, "parents", torch.int32, states.device)

@@ -675,8 +675,9 @@ int preference_loss_forward_backward_hip(
  * beam's place and the others in the free places, so that most states stay where they are.
  * 1 .. 64 beams, select 1 .. 64 and no more than beams * vocab_size.
  * Workspace (8-byte aligned) of at least beam_select_workspace_size() bytes (0: none, or
- * arguments out of range), or NULL: the library's cached one for `stream`.  Invalid arguments -> 1, sizes
- * out of range (vocab_size or rows past 2^30 or 2^31) -> 9; batch == 0 -> 0.
+ * arguments out of range), or NULL: the library's cached one for `stream`.  Invalid
+ * arguments -> 1, sizes out of range (vocab_size of 2^30, batch of 2^22 and more) -> 9;
+ * batch == 0 -> 0.
  */
 size_t beam_select_workspace_size(size_t batch, size_t beams, size_t vocab_size, size_t select);
 int beam_select_hip(const void* logits, const float* scores, const uint8_t* finished,
@@ -690,9 +691,11 @@ int beam_select_hip(const void* logits, const float* scores, const uint8_t* fini
  * tensor i's of row_bytes[i] bytes, at states[i]; outs[i] of the same shape, or outs NULL:
  * in place.  The list keeps the addresses in a device table (made by a copy to the device,
  * freed by state_list_destroy_hip, which waits for it) on the current device; the
- * memory stays the caller's.  No two tensors may overlap (-> 1).  1 .. 64 beams.
+ * memory stays the caller's.  No two tensors may overlap (-> 1).  1 .. 64 beams; more than
+ * 2^24 pieces of 256 columns of 16 bytes (4 past 16 beams, 4 or 1 as rows are aligned) -> 9.
  * state_reorder_hip: row (b, j) of each output is row (b, parents[b][j]) of its state, as
- * all rows were before the call; parents (batch, beams) int32 on the device.  A parent outside
+ * all rows were before the call; parents (batch, beams) int32 on the device, none of the
+ * list's memory.  A parent outside
  * of 0 .. beams - 1 stands for j itself.  One launch; in place, rows that stay are not
  * touched.  The current device has to be the list's (-> 101); one call at a time may use
  * memory that another writes, as for any kernel.
@@ -707,7 +710,8 @@ int state_reorder_hip(const void* list, const int32_t* parents, hipStream_t stre
  *   scale_n = max_k |w_kn| / 127 in fp32, q_kn = w_kn / scale_n to the nearest, ties to even.
  * int8_weight_size: bytes of the packed form (0: k or n out of range); `packed` is
  * 128-byte aligned.  weight: F32, F16 or BF16, row stride ld.  A column with a NaN or an
- * infinity has scale NaN.  k is at most 131072 (-> 9), so that sums stay below 2^31.
+ * infinity has scale NaN.  k is at most 131072, so that sums stay below 2^31, and n below
+ * 2^29 (-> 9).
  */
 size_t int8_weight_size(size_t k, size_t n);
 int int8_weight_pack_hip(const void* weight, size_t ld, void* packed, size_t k, size_t n,
@@ -721,8 +725,9 @@ int int8_weight_pack_hip(const void* weight, size_t ld, void* packed, size_t k, 
  * (F32, F16 or BF16), whatever the packed weight was made from; any row strides and element
  * alignment; output may be residual itself, x neither.  A row of x with a NaN or an infinity
  * gives a row of NaN.  Workspace (16-byte aligned) of at least linear_int8_workspace_size()
- * bytes (0: none, or arguments out of range), or NULL: the library's cached one for `stream`.  Calls with the same row of x give
- * the same bits in that row, whatever m is.  Codes as above; m == 0 -> 0.
+ * bytes (0: none, or arguments out of range), or NULL: the library's cached one for `stream`.
+ * Calls with the same row of x give the same bits in that row, whatever m is.  m is below
+ * 2^24 (-> 9).  Codes as above; m == 0 -> 0.
  */
 size_t linear_int8_workspace_size(size_t m, size_t k, size_t n, int dtype);
 int linear_int8_hip(const void* x, size_t ldx, const void* packed, const void* bias,

@@ -63,6 +63,21 @@ def test_select_workspace_holds_every_cut(L):
     assert size(BIG, 3, 100, 3) == 0
 
 
+def test_more_threads_than_a_launch_has(L):
+    """A launch has fewer than 2^32 threads in a dimension: refused before any of them."""
+    size = L.beam_select_workspace_size
+    assert _select(L, batch=1 << 22, beams=1, n=1) == 9
+    assert _select(L, batch=1 << 22, beams=1, n=1, vocab=60000, ld=60000) == 9
+    assert size((1 << 22) - 1, 1, 60000, 1) > 0 and size(1 << 22, 1, 60000, 1) == 0
+    assert _create(L, states=(4096,), rows=(4,), batch=1 << 24, beams=1) == 9
+    assert _create(L, states=(4096, 1 << 40), rows=(1, 1), batch=1 << 23, beams=3) == 9
+    assert _linear(L, m=1 << 24) == 9 and _linear(L, n=1 << 29, ldy=1 << 29) == 9
+    assert L.linear_int8_workspace_size((1 << 24) - 1, 32, 16, 14) > 0
+    assert L.linear_int8_workspace_size(1 << 24, 32, 16, 14) == 0
+    assert L.int8_weight_size(1, 1 << 29) == 0 and L.int8_weight_size(1, (1 << 29) - 1) > 0
+    assert _pack(L, n=1 << 29, ld=1 << 29) == 9
+
+
 def _create(L, states=(4096, 1 << 20), outs=None, rows=(64, 8), batch=2, beams=3, count=None):
     h = ctypes.c_void_p(7)
     n = len(states)
