@@ -172,10 +172,16 @@ def chunk_efla_fwd(q, k, v, beta, initial_state=None, output_final_state=False,
         _require(out_state, "out_state", torch.float32, q.device)
         if out_state.shape != (N, H, K, V):
             raise ValueError("out_state must be (N,H,K,V) fp32")
-        if initial_state is not None and out_state.data_ptr() == initial_state.data_ptr() and \
-                (T > STEP_TOKENS or cu_seqlens is not None or workspace is not None):
-            raise ValueError(f"a state in place takes up to {STEP_TOKENS} tokens of equal-length "
-                             "sequences and no workspace")
+        if initial_state is not None:
+            apart = abs(out_state.data_ptr() - initial_state.data_ptr())
+            if apart == 0 and (T > STEP_TOKENS or cu_seqlens is not None or
+                               workspace is not None):
+                raise ValueError(f"a state in place takes up to {STEP_TOKENS} tokens of "
+                                 "equal-length sequences and no workspace")
+            if 0 < apart < 4 * out_state.numel():
+                raise ValueError("out_state overlaps initial_state")
+            if apart == 0 and T == 0:  # nothing changes
+                return torch.empty(B, T, H, V, dtype=q.dtype, device=q.device), out_state
         st = out_state
     o = torch.empty(B, T, H, V, dtype=q.dtype, device=q.device)
     if output_final_state and st is None:

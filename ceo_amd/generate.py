@@ -76,8 +76,8 @@ class Decoder:
     def prefill(self, tokens: torch.Tensor):
         """(logits (B, vocab) behind the last token, states) of (B, T) int32 prompts."""
         B, T = tokens.shape
-        if T == 0:
-            raise ValueError("a prompt has at least one token")
+        if B == 0 or T == 0:
+            raise ValueError("prompts: at least one, of at least one token")
         x, states = self._forward(tokens, None)
         return self._logits(x.view(B, T, -1)[:, -1].contiguous()), states
 

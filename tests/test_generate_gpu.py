@@ -148,6 +148,34 @@ def test_states_in_place_are_the_same_bits():
         efla.chunk_efla_fwd(q, k, v, beta, mine, out_state=mine[:3])
 
 
+def test_states_in_place_without_a_token_and_overlapping():
+    from ceo_amd import efla
+
+    q = torch.zeros(3, 0, 2, 64, device="cuda").bfloat16()
+    flat = torch.randn(4 * 2 * 64 * 64, device="cuda")
+    st = flat[:3 * 2 * 64 * 64].view(3, 2, 64, 64)
+    was = st.clone()
+    o, got = efla.chunk_efla_fwd(q, q, q, q[..., 0], st, out_state=st)
+    assert got is st and o.shape == q.shape and torch.equal(st, was)
+    other = flat[2 * 64 * 64:].view(3, 2, 64, 64)
+    with pytest.raises(ValueError):
+        efla.chunk_efla_fwd(q, q, q, q[..., 0], st, out_state=other)
+    one = torch.zeros(3, 1, 2, 64, device="cuda").bfloat16()
+    with pytest.raises(ValueError):
+        efla.chunk_efla_fwd(one, one, one, one[..., 0].contiguous(), st, out_state=other)
+
+
+def test_prompts_are_refused_empty():
+    from ceo_amd.generate import Decoder, beam_search
+
+    model = _model(5)
+    for shape in ((0, 4), (2, 0)):
+        with pytest.raises(ValueError):
+            beam_search(Decoder(model), torch.zeros(shape, dtype=torch.int32, device="cuda"))
+    text, scores = beam_search(Decoder(model), _prompts(model, 2, 3, 1), 4, 0)
+    assert text.shape == (2, 4, 0) and scores[:, 0].tolist() == [0.0, 0.0]
+
+
 def test_command_counts_on():
     """The command's model: its gradients are those of the training step, tested there; here that
     it runs and that both forms of the products give finite scores."""
