@@ -574,6 +574,67 @@ def test_linear_refusals():
 
 
 # ---------------------------------------------------------------------------
+# offsets past 32 bits
+# ---------------------------------------------------------------------------
+def test_select_past_32_bits():
+    """5 GB of logits: texts at the end as when they are alone."""
+    from ceo_amd import nn
+
+    B, K, V = 2500, 8, 128003
+    z = torch.empty(B * K, V, dtype=torch.float16, device="cuda").normal_(0, 2)
+    scores = -torch.rand(B, K, device="cuda")
+    got = nn.beam_select(z, scores)
+    for b in (0, 2095, 2097, B - 1):  # 2^31 elements are 2097.1 texts
+        alone = nn.beam_select(z[b * K:(b + 1) * K].clone(), scores[b:b + 1])
+        # another cut into slices: sums in another order
+        assert (got[0][b] - alone[0][0]).abs().max().item() <= 2 * LSE + 2 * U * 40
+        assert torch.equal(got[1][b], alone[1][0]) and torch.equal(got[2][b], alone[2][0])
+
+
+@pytest.mark.parametrize("outs", [False, True])
+def test_reorder_past_32_bits(outs):
+    """A state of 5 GB, rows of 640 MB."""
+    from ceo_amd.state import StateList, reorder
+
+    x = torch.arange(8 * 160_000_001, device="cuda", dtype=torch.int32).view(8, -1)
+    y = torch.empty_like(x) if outs else x
+    p = torch.tensor([[1, 0, 3, 3], [2, 9, 0, 1]], dtype=torch.int32, device="cuda")
+    reorder(StateList([x], 4, [y] if outs else None), p)
+    n = x.shape[1]
+    for row, src in enumerate((1, 0, 3, 3, 6, 5, 4, 5)):
+        for at in (0, 1, n // 2, n - 2, n - 1):
+            v = (src * n + at) & 0xFFFFFFFF
+            assert y[row, at].item() == (v - (1 << 32) if v >> 31 else v)
+        d = y[row, 1:] - y[row, :-1]
+        assert bool((d == 1).all())
+
+
+@pytest.mark.parametrize("m,k,n", [(70001, 65536, 24), (600001, 128, 4096)])
+def test_linear_past_32_bits(m, k, n):
+    """4.6 GB of quantised tokens, 4.9 GB of output: rows as when they are alone."""
+    from ceo_amd import nn
+
+    x = torch.empty(m, k, dtype=torch.bfloat16, device="cuda").normal_()
+    wt = nn.Int8Weight(torch.randn(k, n, device="cuda").bfloat16())
+    y = nn.linear_int8(x, wt)
+    for r in (0, 32767, 32769, 65535, 65537, m // 2, m - 300, m - 1):
+        assert torch.equal(y[r:r + 1], nn.linear_int8(x[r:r + 1], wt))
+    assert torch.equal(y[m - 300:], nn.linear_int8(x[m - 300:], wt))
+
+
+def test_weight_past_32_bits():
+    """A packed weight of 4.4 GB."""
+    from ceo_amd import nn
+
+    k, n = 131072, 33600
+    w = torch.empty(k, n, dtype=torch.bfloat16, device="cuda").normal_()
+    x = torch.randn(40, k, device="cuda").bfloat16()
+    y = nn.linear_int8(x, nn.Int8Weight(w))
+    for c in (0, 16384, n - 8):
+        assert torch.equal(y[:, c:c + 8], nn.linear_int8(x, nn.Int8Weight(w[:, c:c + 8])))
+
+
+# ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
 def test_captured_and_replayed():
