@@ -105,6 +105,29 @@ def test_search_against_a_plain_one(beams, end, int8):
         assert text[b].tolist() == [t for _, t, _ in want[b]]
 
 
+@pytest.mark.parametrize("beams,end", [(1, None), (4, 7), (8, None)])
+def test_search_from_a_graph(beams, end):
+    """The same bits as without, from searches one after another, other work in between, and on
+    another stream."""
+    from ceo_amd.generate import GRAPH_TOKENS, Decoder, beam_search
+
+    model = _model(6, scale=6.0)
+    dec = Decoder(model)
+    n = GRAPH_TOKENS + 9
+    side = torch.cuda.Stream()
+    for seed in (1, 2):
+        prompts = _prompts(model, 3, 9, seed)
+        want = beam_search(dec, prompts, beams, n, end, graph=False)
+        got = beam_search(dec, prompts, beams, n, end)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = beam_search(dec, prompts, beams, n, end)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.isfinite(got[1]).all()
+
+
 def test_search_finds_the_best_of_all():
     """As many beams as there are prefixes: the search is exhaustive."""
     from ceo_amd.generate import Decoder, beam_search
