@@ -20,13 +20,19 @@ static size_t dtype_size(int d) {
 }
 static size_t scales_bytes(size_t n) { return (size_t)up_to((long)(n * sizeof(float)), kLine); }
 
-// Whether the weights are streamed past few tokens (few_kernel) or go through tiles.  Up to 64
-// tokens, but for wide outputs, whose tiles fill half the chip, 32: a wave reads all tokens
-// for its 16 channels.  Measured (few / 128-tiles, us; 48 tokens, k x n): 1024 x 4096 7.3 / 8.0,
-// 4096 x 4096 12.8 / 19.1, 1024 x 32000 21.5 / 10.4, 1024 x 128000 70 / 36.
-static bool few(long m, long n) {
+static long tiles(long m, long n, long ts) { return ((m + ts - 1) / ts) * ((n + ts - 1) / ts); }
+
+// Up to here the weights are streamed past the tokens (few_kernel).  Measured, few_kernel / mid_kernel,
+// us: 32 x 4096 x 1024 6.6 / 8.0, 64 x 4096 x 1024 10.0 / 8.3, 64 x 1024 x 4096 6.6 / 4.9.
+constexpr long kFewRows = 32;
+
+// Whether mid_kernel has the tiles: one to a compute unit, or two where k is long, since lone_tile_kernel
+// has longer rounds (mid_kernel / lone_tile_kernel, us: 128 x 1024 x 1024 5.0 / 8.4, 512 x 4096 x 1024
+// 9.1 / 18.7, 512 x 4096 x 4096 17.6 / 22.4; two rounds of short ones 512 x 1024 x 4096 9.1 / 9.0;
+// four 1024 x 4096 x 4096 34 / 27).
+static bool mid(long m, long n, long kp) {
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    return m <= 32 || (m <= 64 && (n + 127) / 128 < cus / 2);
+    return m > kFewRows && tiles(m, n, kMid) <= (kp > 1024 ? 2 : 1) * cus;
 }
 
 // Fewer rows than this are quantised by a workgroup each, more by a wave, unless a wave's registers
@@ -37,6 +43,7 @@ constexpr long kWaveRows = 2048;
 // every workgroup, while rows are short, or the tokens 8 and the weights small (4 x 4096 x 1024
 // 9.0 us, apart 6.5 + 3.4 and the second launch).  What a wave's registers and 64 KiB of
 // LDS hold: 16-bit tokens, 32 of 1024 or 8 of 4096 values.
+// No more than kFewRows: other kernels need quantised tokens.
 static bool fused(size_t m, size_t n, size_t kp, size_t size) {
     if (kp <= 1024) return m <= (size == 2 ? 32 : 16);
     return size == 2 && m <= 8 && kp <= 4096 && n <= 16384;
@@ -60,8 +67,6 @@ static void few_launch(const T* x, long ldx, const uint8_t* xq, const float* xs,
                     xq, xs, wq, (int)m, (int)n, k, kp, (int)kw, o);
 }
 
-static long tiles(long m, long n, long ts) { return ((m + ts - 1) / ts) * ((n + ts - 1) / ts); }
-
 // Whether 256-tiles, one to a compute unit, are the faster ones, 128-tiles two: rounds of what the
 // chip holds, of 1.67 / 1.0 us a block of k and 7.3 / 4.4 us for the epilogue and the
 // first block.  (Measured with either, us: 16384 x 1024 x 1024 24.5 / 27.7, 16384 x 2048 x 1024 38 / 44,
@@ -80,7 +85,8 @@ static void tile_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, l
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const long items = tiles(m, n, TS);
     const dim3 grid((unsigned)std::min(items, TS == 256 ? cus : 2 * cus));
-    const gf::Opnd A{(const char*)xq, kp / 2, (int)m}, B{(const char*)wq, kp / 2, (int)n};
+    const gf::Opnd A{(const char*)xq, kp / 2, (int)m};
+    const Weight B{(const char*)wq, kp, (int)((n + 15) / 16)};
     EFLA_LAUNCH("linear_int8", (tile_kernel<T, TS, FORM>), grid, dim3(64 * gf::tile_waves<TS>()),
                 st, A, B, m, n, (int)(kp / kLine), xs, o);
 }
@@ -88,14 +94,22 @@ static void tile_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, l
 template <typename T, int FORM>
 static void lone_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
                         long kp, const Out<T>& o, hipStream_t st) {
-    const gf::Opnd A{(const char*)xq, kp / 2, (int)m}, B{(const char*)wq, kp / 2, (int)n};
+    const gf::Opnd A{(const char*)xq, kp / 2, (int)m};
+    const Weight B{(const char*)wq, kp, (int)((n + 15) / 16)};
     EFLA_LAUNCH("linear_int8", (lone_tile_kernel<T, FORM>), dim3((unsigned)tiles(m, n, 128)),
                 dim3(512), st, A, B, m, n, (int)(kp / kLine), xs, o);
 }
 
+template <typename T, int FORM>
+static void mid_launch(const uint8_t* xq, const float* xs, const uint8_t* wq, long m, long n,
+                       long kp, const Out<T>& o, hipStream_t st) {
+    EFLA_LAUNCH("linear_int8", (mid_kernel<T, FORM>), dim3((unsigned)tiles(m, n, kMid)), dim3(512),
+                st, xq, xs, wq, m, n, kp, o);
+}
+
 static size_t scratch(size_t m, size_t k, size_t n, size_t size) {
     const size_t kp = (size_t)up_to((long)k, kLine);
-    return fused(m, n, kp, size) ? 0 : scales_bytes(m) + m * kp;
+    return fused(m, n, kp, size) ? 0 : scales_bytes(m) + (m + 15) / 16 * 16 * kp;
 }
 
 template <typename T>
@@ -108,13 +122,14 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     const Out<T> o{y, ldy, bias, residual, ldr, sw, gelu};
     float* xs = nullptr;
     uint8_t* xq = nullptr;
+    const bool pieces = m <= kFewRows || mid(m, n, kp);
     if (!fused((size_t)m, (size_t)n, (size_t)kp, sizeof(T))) {
         xs = (float*)ws;
         xq = ws + scales_bytes((size_t)m);
 #define I8_QUANT(LPR, HOLD)                                                                      \
     EFLA_LAUNCH("quantize_rows", (quantize_rows_kernel<T, LPR, HOLD>),                            \
-                dim3((unsigned)(LPR == 64 ? (m + 3) / 4 : m)), dim3(256), st, x, ldx, m, k, kp, xq, \
-                xs)
+                dim3((unsigned)(LPR == 64 ? (m + 3) / 4 : m)), dim3(256), st, x, ldx, m, k, kp, pieces, \
+                xq, xs)
         if (kp > 4096) I8_QUANT(256, 8);
         else if (m < kWaveRows && kp > 512) I8_QUANT(256, 2);
         else if (kp <= 1024) I8_QUANT(64, 2);
@@ -122,7 +137,16 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
 #undef I8_QUANT
         EFLA_CHECK(hipPeekAtLastError());
     }
-    if (few(m, n)) {
+    const size_t a = 8 * sizeof(T);
+    const bool whole = n % 8 == 0 && (uintptr_t)y % a == 0 && ldy % 8 == 0 &&
+                       (!bias || (uintptr_t)bias % a == 0) &&
+                       (!residual || ((uintptr_t)residual % a == 0 && ldr % 8 == 0));
+    if (mid(m, n, kp)) {
+        if (whole) mid_launch<T, kWhole>(xq, xs, wq, m, n, kp, o, st);
+        else mid_launch<T, kRagged>(xq, xs, wq, m, n, kp, o, st);
+        return (int)hipPeekAtLastError();
+    }
+    if (m <= kFewRows) {
 #define I8_FEW(MT, LPR, HOLD) \
     few_launch<T, MT, LPR, HOLD>(x, ldx, xq, xs, wq, m, n, k, kp, o, st)
         if (!xq && kp > 1024) {
@@ -133,18 +157,12 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
             if constexpr (sizeof(T) == 2) I8_FEW(2, 32, 4);
         } else if (m <= 16) {
             I8_FEW(1, 32, 0);
-        } else if (m <= 32) {
-            I8_FEW(2, 32, 0);
         } else {
-            I8_FEW(4, 32, 0);
+            I8_FEW(2, 32, 0);
         }
 #undef I8_FEW
         return (int)hipPeekAtLastError();
     }
-    const size_t a = 8 * sizeof(T);
-    const bool whole = n % 8 == 0 && (uintptr_t)y % a == 0 && ldy % 8 == 0 &&
-                       (!bias || (uintptr_t)bias % a == 0) &&
-                       (!residual || ((uintptr_t)residual % a == 0 && ldr % 8 == 0));
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const bool lone = tiles(m, n, 128) <= cus, large = !lone && large_tiles(m, n, kp);
     // past the L2s from their 32 MB on (16384 x 1024 x 4096 with a residual 113 -> 104 us, without
@@ -186,7 +204,7 @@ using namespace efla;
 
 extern "C" size_t int8_weight_size(size_t k, size_t n) {
     if (k == 0 || k > i8::kMaxK || n == 0 || n > i8::kMaxN) return 0;
-    return i8::scales_bytes(n) + n * (size_t)i8::up_to((long)k, i8::kLine);
+    return i8::scales_bytes(n) + (n + 15) / 16 * 16 * (size_t)i8::up_to((long)k, i8::kLine);
 }
 
 extern "C" int int8_weight_pack_hip(const void* weight, size_t ld, void* packed, size_t k,

@@ -6,8 +6,11 @@
 //   y_mn = act((sum_k qx_mk qw_kn) sx_m sw_n + bias_n) + residual_mn, rounded once
 //
 // The sums are whole and exact (k <= 131072: below 2^31), so nothing depends on how they
-// are split.  A packed weight is one row of whole 128-byte lines per channel, zero
-// behind k, after the scales; quantised tokens are rows of the same length.
+// are split.  k is filled up with zeros to whole blocks of 128.  A packed weight lies, after
+// the scales, in the order in which a wave's lanes load it: pieces of 16 channels by 64 k, of
+// which lane l = 16 g + r has channel r, k 16 g .. + 15, one behind the other.  (In rows a load takes
+// 16 lines of 16 lanes, at a quarter of the rate: mid_kernel for 128 x 4096 x 1024 19 us, 8.6 so.)
+// Quantised tokens are the same or rows, whichever the product's kernel reads.
 #pragma once
 #include "common.hpp"
 #include "gemm_fast.hpp"
@@ -20,6 +23,11 @@ typedef __attribute__((__vector_size__(16 * sizeof(int)))) int int16v;
 
 constexpr long kLine = 128;
 inline __host__ __device__ long up_to(long x, long m) { return (x + m - 1) / m * m; }
+constexpr int kPiece = 1024;  // bytes of 16 rows by 64 k
+// where in 16 rows' pieces row r's 8 values from k = c on lie (c % 8 == 0)
+__device__ __forceinline__ long piece_at(int r, long c) {
+    return (c >> 6) * kPiece + ((c >> 4) & 3) * 256 + 16 * r + (c & 8);
+}
 
 // --- quantising -----------------------------------------------------------------
 // A row's (column's) scale from its largest magnitude.  NaN where that is not finite: the
@@ -150,9 +158,10 @@ struct Row {
         for (long c = kHeld + 8 * lr; c < k; c += 8 * LPR) m.add(at(x, c, k));
         return m.get();
     }
-    // q: kp bytes, zero behind k
+    // kp bytes, zero behind k; q(c) is where the eight from c on go
+    template <typename At>
     __device__ __forceinline__ void store(const T* x, long k, long kp, int lr, float scale,
-                                          uint8_t* q) {
+                                          At q) {
         // Below the normal range's reciprocals (never in fp16) everything is taken 2^64 times as
         // large, which is exact.  A scale with few bits may leave more than 127 steps: cut off.
         if (scale < 0x1p-100f && scale > 0.f) {
@@ -169,7 +178,7 @@ struct Row {
             for (long c = kHeld + 8 * lr; c < kp; c += 8 * LPR) {
                 Vec y = at(x, c, k);
                 up(y);
-                *reinterpret_cast<uint2*>(q + c) = qz(y);
+                *reinterpret_cast<uint2*>(q(c)) = qz(y);
             }
             scale *= 0x1p64f;
             kp = kp < kHeld ? kp : kHeld;
@@ -178,19 +187,20 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
             const long c = 8 * (lr + LPR * i);
-            if (c < kp) *reinterpret_cast<uint2*>(q + c) = qz(v[i]);
+            if (c < kp) *reinterpret_cast<uint2*>(q(c)) = qz(v[i]);
         }
         for (long c = kHeld + 8 * lr; c < kp; c += 8 * LPR)
-            *reinterpret_cast<uint2*>(q + c) = qz(at(x, c, k));
-        if (k % 8 && lr == k / 8 % LPR) *reinterpret_cast<uint2*>(q + k / 8 * 8) = qz(last);
+            *reinterpret_cast<uint2*>(q(c)) = qz(at(x, c, k));
+        if (k % 8 && lr == k / 8 % LPR) *reinterpret_cast<uint2*>(q(k / 8 * 8)) = qz(last);
     }
 };
 
 // LPR threads to a row: a wave, four rows to a workgroup, or (few rows) the whole workgroup,
-// where one wave's chain of instructions is what a row takes.  Bound by memory.
+// where one wave's chain of instructions is what a row takes.  Bound by memory.  Rows of kp
+// bytes, or pieces.
 template <typename T, int LPR, int HOLD>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ldx,
-                                                            long m, long k, long kp,
+                                                            long m, long k, long kp, int pieces,
                                                             uint8_t* __restrict__ q,
                                                             float* __restrict__ scales) {
     __shared__ float part[4];
@@ -207,7 +217,9 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
         a = amax2(amax2(part[0], part[1]), amax2(part[2], part[3]));
     }
     const float s = scale_of(a);
-    r.store(x, k, kp, lr, s, q + row * kp);
+    q += pieces ? row / 16 * 16 * kp : row * kp;
+    const int r16 = (int)(row & 15);
+    r.store(x, k, kp, lr, s, [&](long c) { return q + (pieces ? piece_at(r16, c) : c); });
     if (lr == 0) scales[row] = s;
 }
 
@@ -222,7 +234,7 @@ __global__ void __launch_bounds__(256) column_amax_kernel(const T* __restrict__ 
     atomicMax(amax + c, __float_as_uint(m));
 }
 
-// 64 x 64 tiles of the weight, turned through LDS and quantised: a row of q per channel.
+// 64 x 64 tiles of the weight, turned through LDS and quantised into pieces.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_weight_kernel(const T* __restrict__ w, long ld, long k,
                                                           long n, long kp,
@@ -248,7 +260,8 @@ __global__ void __launch_bounds__(256) pack_weight_kernel(const T* __restrict__ 
                 if (tiny) v[e] = fminf(fmaxf(v[e], -127.f * s), 127.f * s) * 0x1p64f;
             }
             const Quantizer qz(tiny ? s * 0x1p64f : s);
-            *reinterpret_cast<uint2*>(q + col * kp + k0 + 8 * (i & 7)) = qz(v);
+            *reinterpret_cast<uint2*>(q + col / 16 * 16 * kp +
+                                      piece_at((int)(col & 15), k0 + 8 * (i & 7))) = qz(v);
         }
         __syncthreads();
     }
@@ -294,8 +307,7 @@ __device__ __forceinline__ void scaled(float (&v)[N], const Acc& acc, float sx, 
 // once, LPR lanes to a row (8 HOLD elements of each lane in registers).  Loads return in
 // the order in which they are issued, so the tokens are asked for before the weights and
 // quantised while those are on their way, and what the epilogue needs right behind.  HOLD 0:
-// the tokens are read quantised (32 channels a wave, so that they are read half as often: 48 x 4096
-// x 1024 16.1 us, 11.9 with 16).
+// the tokens are read quantised, in pieces.
 constexpr int kAhead = 8;  // 64-byte steps of k whose weights a wave has in flight
 // waves of a workgroup: enough that 32 lanes have a row
 template <int MT, int LPR, int HOLD>
@@ -316,7 +328,7 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
     const int cw = NW / kw, wk = w % kw;
     const long n0 = ((long)blockIdx.x * cw + w / kw) * 16;
     const int steps = (int)(kp / 64), s0 = steps * wk / kw, s1 = steps * (wk + 1) / kw;
-    const uint8_t* wp = wq + (n0 + r < N ? n0 + r : N - 1) * kp + 16 * g;
+    const uint8_t* wp = wq + (n0 < N ? n0 : 0) * kp + 16 * l;
     const int own = threadIdx.x / LPR, lr = threadIdx.x % LPR;
     Row<T, LPR, FUSED ? HOLD : 1> row;
     if constexpr (FUSED) row.load(x + own * ldx, own < M ? k : 0, lr);
@@ -324,7 +336,7 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
         const int s = s0 + i < s1 ? s0 + i : s0;
-        a[i] = *reinterpret_cast<const int4v*>(wp + 64L * s);
+        a[i] = *reinterpret_cast<const int4v*>(wp + (long)kPiece * s);
     }
     // lane l ends up with rows 16 t + r, channels n .. n + 3
     const long n = n0 + 4 * g;
@@ -339,12 +351,12 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
             if (o.residual && 16 * t + r < M)
                 res[t] = P::load(o.residual + (16 * t + r) * o.ldr + n, N - n);
     }
-    const long ldq = FUSED ? kp + 16 : kp;
+    const long ldq = kp + 16;
     float* sc = reinterpret_cast<float*>(lds);  // 16 MT scales
     uint8_t* rows = lds + 64 * MT;
     if constexpr (FUSED) {
         const float s = scale_of(lanes_amax<LPR>(row.amax(x, 0, lr)));
-        row.store(x, own < M ? k : 0, kp, lr, s, rows + own * ldq);
+        row.store(x, own < M ? k : 0, kp, lr, s, [&](long c) { return rows + own * ldq + c; });
         if (lr == 0) sc[own] = s;
         __syncthreads();
     }
@@ -354,21 +366,20 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
     // (64 lanes a row: LDS has 8 rows, whose products rows 8 to 15 repeat)
     const uint8_t* bp[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = 16 * t + r;
-        bp[t] = (FUSED ? rows + (LPR == 64 ? r & 7 : m) * ldq : xq + (m < M ? m : M - 1) * ldq) +
-                16 * g;
-    }
+    for (int t = 0; t < MT; ++t)
+        bp[t] = FUSED ? rows + (LPR == 64 ? r & 7 : 16 * t + r) * ldq + 16 * g
+                      : xq + (16 * t < M ? 16 * t : 0) * kp + 16 * l;
+    constexpr long kStep = FUSED ? 64 : kPiece;
     for (int s = s0; s < s1; s += kAhead) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (s + i >= s1) break;
             const int4v wa = a[i];
             if (s + i + kAhead < s1)
-                a[i] = *reinterpret_cast<const int4v*>(wp + 64L * (s + i + kAhead));
+                a[i] = *reinterpret_cast<const int4v*>(wp + (long)kPiece * (s + i + kAhead));
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const int4v b = *reinterpret_cast<const int4v*>(bp[t] + 64L * (s + i));
+                const int4v b = *reinterpret_cast<const int4v*>(bp[t] + kStep * (s + i));
                 acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wa, b, acc[t], 0, 0, 0);
             }
         }
@@ -416,33 +427,38 @@ struct Columns {
     typedef gf::Piece<8, float, RAGGED> F;
     long n, cnt;
     float sw[8], bias[8];
-    __device__ __forceinline__ Columns(const Out<T>& o, long n, long N) : n(n), cnt(N - n) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sw[e] = bias[e] = 0.f;
-        if (cnt <= 0) return;
-        const typename F::vec s = F::load(o.sw + n, cnt);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sw[e] = s[e];
-        if (!o.bias) return;
-        const typename P::vec b = P::load(o.bias + n, cnt);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bias[e] = (float)b[e];
-    }
-    struct Rows {  // rows m0, m0 + 8, + 16, + 24
-        float sx[4];
-        typename P::vec res[4];
-        __device__ __forceinline__ void load(const Out<T>& o, const Columns& c,
-                                             const float* __restrict__ xs, long m0, long M) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) sx[s] = xs[min(m0 + 8 * s, M - 1)];
-            if (!o.residual || c.cnt <= 0) return;
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-                res[s] = P::load(o.residual + min(m0 + 8 * s, M - 1) * o.ldr + c.n, c.cnt);
+    struct Read {  // as loaded: converting would wait for it
+        typename F::vec sw{};
+        typename P::vec bias{};
+        __device__ __forceinline__ Read(const Out<T>& o, long n, long N) {
+            if (n < N) sw = F::load(o.sw + n, N - n);
+            if (n < N && o.bias) bias = P::load(o.bias + n, N - n);
         }
     };
+    __device__ __forceinline__ Columns(const Read& r, long n, long N) : n(n), cnt(N - n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sw[e] = r.sw[e];
+            bias[e] = (float)r.bias[e];
+        }
+    }
+    template <int S>
+    struct Rows {  // rows m0, m0 + 8, + 16, ..
+        float sx[S];
+        typename P::vec res[S];
+        __device__ __forceinline__ void load(const Out<T>& o, long n, long N,
+                                             const float* __restrict__ xs, long m0, long M) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) sx[s] = xs[min(m0 + 8 * s, M - 1)];
+            if (!o.residual || n >= N) return;
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                res[s] = P::load(o.residual + min(m0 + 8 * s, M - 1) * o.ldr + n, N - n);
+        }
+    };
+    template <int S>
     __device__ __forceinline__ void finish(const Out<T>& o, long m, const int (&acc)[8],
-                                           const Rows& r, int s) const {
+                                           const Rows<S>& r, int s) const {
         float v[8];
         scaled<T>(v, acc, r.sx[s], sw, bias);
         if (o.gelu) {
@@ -464,9 +480,98 @@ struct Columns {
     }
 };
 
+// --- some rows ------------------------------------------------------------------------
+// 64 x 64 tiles, eight waves that split k, for outputs of few tiles: nothing waits for another
+// wave until the sums meet in LDS, 16 KB a wave, and each wave finishes eight rows.  A wave reads
+// its blocks of 128 straight from memory, one ahead, the weights as A operand like few_kernel.
+// Bound by its start, one block's latency and the joining for short k (128 x 1024 x 1024 5.0 us) and
+// by what a compute unit loads, 64 bytes a clock, for long (8192 more of k 11 us).
+constexpr int kMid = 64;
+
+template <typename T, int FORM>
+__global__ void __launch_bounds__(512, 2)
+mid_kernel(const uint8_t* __restrict__ xq, const float* __restrict__ xs,
+           const uint8_t* __restrict__ wq, long M, long N, long kp, Out<T> o) {
+    constexpr int W = 8, G = kMid / 16;
+    __shared__ __attribute__((aligned(16))) int4v part[W][G * G * 64];
+    const int w = mf::wave(), l = lane_id();
+    // bands of tiles for the XCDs, tokens first
+    const long items = gridDim.x, tm = (M + kMid - 1) / kMid;
+    long id = blockIdx.x;
+    if (items % 8 == 0) id = (id % 8) * (items / 8) + id / 8;
+    const long m0 = id % tm * kMid, n0 = id / tm * kMid;
+    const int blocks = (int)(kp / kLine), b0 = blocks * w / W, b1 = blocks * (w + 1) / W;
+    const uint8_t *wp[G], *xp[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        wp[i] = wq + (n0 + 16 * i < N ? n0 + 16 * i : n0) * kp;
+        xp[i] = xq + (m0 + 16 * i < M ? m0 + 16 * i : m0) * kp;
+    }
+    const unsigned lo = 16 * l;
+    int4v a[2][2][G], b[2][2][G];
+    auto load = [&](int c, int blk) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                const long at = (long)kPiece * (2 * blk + s);
+                a[c][s][i] = *reinterpret_cast<const int4v*>(wp[i] + at + lo);
+                b[c][s][i] = *reinterpret_cast<const int4v*>(xp[i] + at + lo);
+            }
+    };
+    int4v acc[G][G];
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int t = 0; t < G; ++t) acc[i][t] = int4v{};
+    auto mma = [&](int c) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int t = 0; t < G; ++t)
+                    acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[c][s][i], b[c][s][t],
+                                                                      acc[i][t], 0, 0, 0);
+    };
+    if (b0 < b1) load(0, b0);
+    // what the epilogue needs: row 8 w + (l & 7) of the tile, columns 8 (l >> 3) ..
+    const long row = m0 + 8 * w + (l & 7);
+    typedef Columns<T, FORM> Col;
+    const long n = n0 + 8 * (l >> 3);
+    const typename Col::Read read(o, n, N);
+    typename Col::template Rows<1> rows;
+    rows.load(o, n, N, xs, row, M);
+    int blk = b0;
+    for (; blk + 2 <= b1; blk += 2) {
+        load(1, blk + 1);
+        __builtin_amdgcn_sched_barrier(0);  // (the loads would be put behind the products)
+        mma(0);
+        if (blk + 2 < b1) load(0, blk + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(1);
+    }
+    if (blk < b1) mma(0);
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int t = 0; t < G; ++t) part[w][(i * G + t) * 64 + l] = acc[i][t];
+    __syncthreads();
+    // tokens 16 t + r are lane 16 g + r's, channels 16 i + 4 g ..
+    const int at = (((l >> 3) / 2) * G + w / 2) * 64 + ((l >> 3) % 2) * 32 + 8 * (w % 2) + (l & 7);
+    int4v v0{}, v1{};
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        v0 += part[j][at];
+        v1 += part[j][at + 16];
+    }
+    const int v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+    if (row < M && n < N) Col(read, n, N).finish(o, row, v, rows, 0);
+}
+
 // --- many rows ------------------------------------------------------------------------
-// The tiles of gemm_fast.hpp with both operands k-contiguous and two 8-bit integers in the
-// place of each 16-bit element: 256 x 256 x 128 (eight waves of 128 x 64) or 128 x 128 x 128
+// The tiles of gemm_fast.hpp, the tokens k-contiguous with two 8-bit integers in the
+// place of each 16-bit element, the weights in pieces: 256 x 256 x 128 (eight waves of 128 x 64) or 128 x 128 x 128
 // (four of 64 x 64, two workgroups to a CU), copied straight into LDS one block ahead,
 // MFMA 32 x 32 x 32.  Rows are padded to whole blocks, so there is no tail in k.
 
@@ -477,11 +582,13 @@ template <typename T, int FORM, int TMJ>
 __device__ __forceinline__ void tile_epilogue(const Out<T>& o, const int16v (&acc)[2][TMJ],
                                               const float* __restrict__ xs, long mw, long nw,
                                               long M, long N, int l, char* wp) {
-    const Columns<T, FORM> col(o, nw + 8 * (l & 7), N);
+    typedef Columns<T, FORM> Col;
+    const long n = nw + 8 * (l & 7);
+    const Col col(typename Col::Read(o, n, N), n, N);
     // (fp32 residuals and ragged ones leave no registers to read a pass ahead in)
     constexpr bool AHEAD = sizeof(T) == 2 && FORM != kRagged;
-    typename Columns<T, FORM>::Rows rows[2];
-    if (AHEAD && mw < M) rows[0].load(o, col, xs, mw + (l >> 3), M);
+    typename Col::template Rows<4> rows[2];
+    if (AHEAD && mw < M) rows[0].load(o, n, N, xs, mw + (l >> 3), M);
 #pragma unroll
     for (int j = 0; j < TMJ; ++j) {
         const long r0 = mw + 32 * j;
@@ -496,8 +603,8 @@ __device__ __forceinline__ void tile_epilogue(const Out<T>& o, const int16v (&ac
         // the next pass's scales and residual are on their way while this one is
         // finished: its accumulators have left their registers
         if (AHEAD && j + 1 < TMJ && r0 + 32 < M)
-            rows[(j + 1) & 1].load(o, col, xs, r0 + 32 + (l >> 3), M);
-        if (!AHEAD) rows[j & 1].load(o, col, xs, r0 + (l >> 3), M);
+            rows[(j + 1) & 1].load(o, n, N, xs, r0 + 32 + (l >> 3), M);
+        if (!AHEAD) rows[j & 1].load(o, n, N, xs, r0 + (l >> 3), M);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int row = 8 * s + (l >> 3), c = 8 * (l & 7);
@@ -509,6 +616,31 @@ __device__ __forceinline__ void tile_epilogue(const Out<T>& o, const int16v (&ac
     }
 }
 
+// TS channels of a block of k, in the order in which they lie, by the waves of a tile
+struct Weight {
+    const char* base;
+    long kp;
+    int groups;  // of 16 channels
+};
+template <int TS>
+__device__ __forceinline__ void copy_weight(const Weight& B, int n0, int blk, char* tile, int w,
+                                            int l) {
+    constexpr int NW = gf::tile_waves<TS>();
+    const int g0 = n0 >> 4;
+    const char* base = B.base + (long)g0 * 16 * B.kp + 2L * kPiece * blk;
+#pragma unroll
+    for (int i = 0; i < TS / 8 / NW; ++i) {
+        const int q = NW * i + w, group = min(q >> 1, B.groups - 1 - g0);
+        mf::dma16(base, (unsigned)(group * (int)(16 * B.kp) + (q & 1) * kPiece + 16 * l),
+                  tile + kPiece * q);
+    }
+}
+// channels n .. n + 31 of it, k step ks
+__device__ __forceinline__ int4v weight_frag(const char* tile, int n, int ks, int l) {
+    const int group = (n >> 4) + ((l >> 4) & 1), lane = 16 * (2 * (ks & 1) + (l >> 5)) + (l & 15);
+    return *reinterpret_cast<const int4v*>(tile + kPiece * (2 * group + (ks >> 1)) + 16 * lane);
+}
+
 // Fragments and products of one 32-deep step of a tile's block, reads of the next between them
 template <int TS, int TMJ>
 struct Steps {
@@ -517,7 +649,7 @@ struct Steps {
                                          int ks, int l) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            fb[c][i] = __builtin_bit_cast(int4v, gf::frag<true, TS>(bs, wn + 32 * i, ks, l));
+            fb[c][i] = weight_frag(bs, wn + 32 * i, ks, l);
 #pragma unroll
         for (int j = 0; j < TMJ; ++j)
             fa[c][j] = __builtin_bit_cast(int4v, gf::frag<true, TS>(as, wm + 32 * j, ks, l));
@@ -542,7 +674,7 @@ struct Steps {
 
 template <typename T, int TS, int FORM>
 __global__ void __launch_bounds__(64 * gf::tile_waves<TS>(), TS == 128 ? 2 : 1)
-tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
+tile_kernel(gf::Opnd A, Weight B, long M, long N, int niter, const float* __restrict__ xs,
             Out<T> o) {
     constexpr int TILE = gf::tile_bytes<TS>(), TNI = 2, TMJ = TS / 64, KS = 4;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
@@ -569,7 +701,7 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
     auto fetch = [&](int b, int l) {
         if (!fmore) return;
         gf::copy_tile<true, TS>(A, fm0, (long)fkt * gf::BK, As(b), w, l);
-        gf::copy_tile<true, TS>(B, fn0, (long)fkt * gf::BK, Bs(b), w, l);
+        copy_weight<TS>(B, fn0, fkt, Bs(b), w, l);
         if (++fkt == niter) {
             fkt = 0;
             fit += gridDim.x;
@@ -628,15 +760,14 @@ tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __re
     }
 }
 
-// The same for outputs of no more 128 x 128 tiles than there are compute units, each of which has
-// one alone: eight waves in two groups of four that take the blocks of k in turn, two
+// The same for outputs of no more 128 x 128 tiles than there are compute units and too many for
+// mid_kernel: each has one alone, eight waves in two groups of four that take the blocks of k in turn, two
 // buffers each, and add up in LDS.  A lone tile waits for its one wave a SIMD, not for its
 // loads: four waves with two buffers, with three blocks under way, and this, us:
-//   65 x 1024 x 1024 10.2 / 9.3 / 7.9   65 x 4096 x 1024 24.2 / 22.4 / 18.3
 //   65 x 1024 x 32000 11.9 / 11.1 / 10.8   517 x 1001 x 3088 fp16 11.4 / 10.6 / 9.4
 template <typename T, int FORM>
 __global__ void __launch_bounds__(512, 2)
-lone_tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float* __restrict__ xs,
+lone_tile_kernel(gf::Opnd A, Weight B, long M, long N, int niter, const float* __restrict__ xs,
                  Out<T> o) {
     constexpr int TS = 128, TMJ = 2, KS = 4, TILE = gf::tile_bytes<TS>();
     __shared__ __attribute__((aligned(1024))) char smem[4 * 2 * TILE];
@@ -652,7 +783,7 @@ lone_tile_kernel(gf::Opnd A, gf::Opnd B, long M, long N, int niter, const float*
         const long k0 = (2L * i + group) * gf::BK;
         char* to = base + (i & 1) * 2 * TILE;
         gf::copy_tile<true, TS>(A, m0, k0, to, w, l);
-        gf::copy_tile<true, TS>(B, n0, k0, to + TILE, w, l);
+        copy_weight<TS>(B, n0, 2 * i + group, to + TILE, w, l);
     };
     fetch(0);
     int16v acc[2][TMJ];

@@ -121,8 +121,8 @@ def _linear(L, x=P, ldx=32, p=Q, b=NULL, r=NULL, ldr=0, y=P, ldy=16, m=100, k=32
 def test_weight_refusals(L):
     assert L.int8_weight_size(0, 4) == 0 and L.int8_weight_size(4, 0) == 0
     assert L.int8_weight_size(131073, 4) == 0 and L.int8_weight_size(4, 1 << 30) == 0
-    assert L.int8_weight_size(1, 1) == 256                       # a line of scales, one of k
-    assert L.int8_weight_size(129, 33) == 256 + 33 * 256
+    assert L.int8_weight_size(1, 1) == 128 + 16 * 128            # a line of scales, 16 channels
+    assert L.int8_weight_size(129, 33) == 256 + 48 * 256
     assert _pack(L, w=NULL) == 1 and _pack(L, p=NULL) == 1
     assert _pack(L, k=0) == 1 and _pack(L, n=0) == 1 and _pack(L, ld=15) == 1
     assert _pack(L, w=ctypes.c_void_p(4097)) == 1 and _pack(L, p=ctypes.c_void_p(4096 + 64)) == 1

@@ -459,6 +459,15 @@ def test_linear_weight_types_and_strides(m, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(500, 1100, 4000), (520, 1024, 4096), (33, 3000, 1000),
+                                   (1000, 136, 2040), (64, 200, 16385), (512, 4096, 1024)])
+def test_linear_in_between(m, k, n, dtype):
+    """Outputs of few tiles: one or two of 64 x 64 to a compute unit, or one of 128 x 128."""
+    x, w, b, r = operands(m, k, n, dtype)
+    check_linear(x, w, b, r, gelu=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_linear_large(dtype):
     x, w, b, r = operands(2100, 1024, 3088, dtype)
     check_linear(x, w, b, r, gelu=True)
