@@ -40,7 +40,7 @@ __device__ __forceinline__ float scale_of(float amax) {
 // eight of them, a byte each.  A fused multiply and add of 1.5 2^23 rounds x inv to a whole
 // number that its low byte holds.  inv is 1 / scale rounded, so x inv is off by 127 * 2^-23 at
 // most, and the whole number by one at most, next to a half: what lies within 2^-14 of one
-// (one vector in sixty) is looked at again.  There x - r scale, which one fused operation gives
+// (one vector in a thousand) is looked at again.  There x - r scale, which one fused operation gives
 // without rounding (x and scale have 24 bits, r 7, and the difference is below scale),
 // says on which side of the half x lies.
 // A row of zeros, or one that holds NaN or an infinity, has inv 0: 0 everywhere.
