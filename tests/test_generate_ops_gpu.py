@@ -582,6 +582,42 @@ def test_linear_refusals():
                        nn.linear_int8(x, wt, None, r[:1].repeat(4, 1)))
 
 
+def test_library_workspace_on_two_streams():
+    """The C entries without a workspace: the library's, one for each stream, calls of both kinds
+    sharing it in turn."""
+    from ceo_amd import _lib, nn
+
+    L = _lib.lib()
+    B, K, V, n = 5, 4, 50257, 7
+    g = torch.Generator(device="cuda").manual_seed(4)
+    z = torch.randn(B * K, V, generator=g, device="cuda").half()
+    scores = -torch.rand(B, K, generator=g, device="cuda")
+    x = torch.randn(300, 1000, generator=g, device="cuda").bfloat16()
+    wt = nn.Int8Weight(torch.randn(1000, 520, generator=g, device="cuda").bfloat16())
+    want = nn.beam_select(z, scores, n)
+    want_y = nn.linear_int8(x, wt)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(3):
+        for st in streams:
+            with torch.cuda.stream(st):
+                s = torch.empty(B, n, device="cuda")
+                p, t = (torch.empty(B, n, dtype=torch.int32, device="cuda") for _ in range(2))
+                y = torch.empty_like(want_y)
+            h = st.cuda_stream
+            assert L.beam_select_hip(z.data_ptr(), scores.data_ptr(), None, s.data_ptr(),
+                                     p.data_ptr(), t.data_ptr(), None, B, K, V, V, n, -1, 0, 2, None,
+                                     0, h) == 0
+            assert L.linear_int8_hip(x.data_ptr(), 1000, wt.packed.data_ptr(), None, None, 0,
+                                     y.data_ptr(), 520, 300, 1000, 520, 0, 14, None, 0, h) == 0
+            outs.append((s, p, t, y))
+    torch.cuda.synchronize()
+    for s, p, t, y in outs:
+        assert torch.equal(s, want[0]) and torch.equal(p, want[1]) and torch.equal(t, want[2])
+        assert torch.equal(y, want_y)
+
+
 # ---------------------------------------------------------------------------
 # offsets past 32 bits
 # ---------------------------------------------------------------------------
