@@ -151,6 +151,8 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     few_launch<T, MT, LPR, HOLD>(x, ldx, xq, xs, wq, m, n, k, kp, o, st)
         if (!xq && kp > 1024) {
             if constexpr (sizeof(T) == 2) I8_FEW(1, 64, 8);
+        } else if (!xq && m <= 8) {
+            I8_FEW(1, 64, 2);
         } else if (!xq && m <= 16) {
             I8_FEW(1, 32, 4);
         } else if (!xq) {
