@@ -41,7 +41,7 @@ constexpr long kWaveRows = 2048;
 
 // Whether few_kernel quantises the tokens itself: a second launch is longer than what it takes
 // every workgroup, while rows are short, or the tokens 8 and the weights small (4 x 4096 x 1024
-// 9.0 us, apart 6.5 + 3.4 and the second launch).  What a wave's registers and 64 KiB of
+// 7.9 us, apart 6.2 + 3.4 and the second launch).  What a wave's registers and 64 KiB of
 // LDS hold: 16-bit tokens, 32 of 1024 or 8 of 4096 values.
 // No more than kFewRows: other kernels need quantised tokens.
 static bool fused(size_t m, size_t n, size_t kp, size_t size) {
@@ -62,7 +62,7 @@ static void few_launch(const T* x, long ldx, const uint8_t* xq, const float* xs,
     const dim3 grid((unsigned)((cols + cw - 1) / cw)), block(64 * NW);
     const size_t parts = kw > 1 ? (size_t)NW * MT * 64 * 16 : 0;
     const size_t rows = HOLD ? (size_t)(64 * NW / LPR) * (size_t)(kp + 16) : 0;
-    const size_t lds = 64 * MT + std::max(parts, rows);
+    const size_t lds = kFewFront<MT, LPR> + std::max(parts, rows);
     EFLA_LAUNCH_LDS("linear_int8", (few_kernel<T, MT, LPR, HOLD>), grid, block, lds, st, x, ldx,
                     xq, xs, wq, (int)m, (int)n, k, kp, (int)kw, o);
 }
@@ -150,7 +150,7 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
 #define I8_FEW(MT, LPR, HOLD) \
     few_launch<T, MT, LPR, HOLD>(x, ldx, xq, xs, wq, m, n, k, kp, o, st)
         if (!xq && kp > 1024) {
-            if constexpr (sizeof(T) == 2) I8_FEW(1, 64, 8);
+            if constexpr (sizeof(T) == 2) I8_FEW(1, 128, 4);
         } else if (!xq && m <= 8) {
             I8_FEW(1, 64, 2);
         } else if (!xq && m <= 16) {

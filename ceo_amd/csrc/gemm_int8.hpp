@@ -30,10 +30,10 @@ __device__ __forceinline__ long piece_at(int r, long c) {
 }
 
 // --- quantising -----------------------------------------------------------------
-// A row's (column's) scale from its largest magnitude.  NaN where that is not finite: the
+// A row's (column's) scale from its largest magnitude, times 1 / 127 rounded to fp32.  NaN where that is not finite: the
 // row's products are NaN then.
 __device__ __forceinline__ float scale_of(float amax) {
-    return amax < INFINITY ? amax / 127.f : NAN;
+    return amax < INFINITY ? amax * (1.f / 127.f) : NAN;
 }
 
 // x / scale to the nearest whole number, ties to even, as an exact quotient would round:
@@ -306,12 +306,16 @@ __device__ __forceinline__ void scaled(float (&v)[N], const Acc& acc, float sx, 
 // sums meet in LDS.  HOLD > 0: the workgroup quantises the tokens into LDS itself, all rows at
 // once, LPR lanes to a row (8 HOLD elements of each lane in registers).  Loads return in
 // the order in which they are issued, so the tokens are asked for before the weights and
-// quantised while those are on their way, and what the epilogue needs right behind.  HOLD 0:
-// the tokens are read quantised, in pieces.
+// quantised while those are on their way, and what the epilogue needs right behind.  Up to 8
+// tokens have a wave a row (4 x 1024 x 4096 5.4 us, with 32 lanes 6.2, with two waves 5.9), long
+// ones two (4 x 4096 x 1024 7.7, with one 8.8).  HOLD 0: the tokens are read quantised, in pieces.
 constexpr int kAhead = 8;  // 64-byte steps of k whose weights a wave has in flight
-// waves of a workgroup: enough that 32 lanes have a row
+// waves of a workgroup: enough that LPR lanes have a row, 8 rows where that is a wave or two
 template <int MT, int LPR, int HOLD>
-constexpr int kFewWaves = HOLD > 0 && LPR == 32 ? 8 * MT : 8;
+constexpr int kFewWaves = HOLD == 0 ? 8 : LPR == 32 ? 8 * MT : LPR / 8;
+// LDS in front of the rows: their scales, and two waves' halves of a largest magnitude
+template <int MT, int LPR>
+constexpr int kFewFront = LPR > 64 ? 128 : 64 * MT;
 
 template <typename T, int MT, int LPR, int HOLD>
 __global__ void __launch_bounds__((64 * kFewWaves<MT, LPR, HOLD>),
@@ -353,9 +357,16 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
     }
     const long ldq = kp + 16;
     float* sc = reinterpret_cast<float*>(lds);  // 16 MT scales
-    uint8_t* rows = lds + 64 * MT;
+    uint8_t* rows = lds + kFewFront<MT, LPR>;
     if constexpr (FUSED) {
-        const float s = scale_of(lanes_amax<LPR>(row.amax(x, 0, lr)));
+        float m = lanes_amax<LPR < 64 ? LPR : 64>(row.amax(x, 0, lr));
+        if constexpr (LPR > 64) {
+            float* part = sc + 16;
+            if (l == 0) part[w] = m;
+            __syncthreads();
+            m = amax2(m, part[w ^ 1]);
+        }
+        const float s = scale_of(m);
         row.store(x, own < M ? k : 0, kp, lr, s, [&](long c) { return rows + own * ldq + c; });
         if (lr == 0) sc[own] = s;
         __syncthreads();
@@ -363,11 +374,11 @@ few_kernel(const T* __restrict__ x, long ldx, const uint8_t* __restrict__ xq,
     int4v acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = int4v{};
-    // (64 lanes a row: LDS has 8 rows, whose products rows 8 to 15 repeat)
+    // (64 or more lanes a row: LDS has 8 rows, whose products rows 8 to 15 repeat)
     const uint8_t* bp[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
-        bp[t] = FUSED ? rows + (LPR == 64 ? r & 7 : 16 * t + r) * ldq + 16 * g
+        bp[t] = FUSED ? rows + (LPR >= 64 ? r & 7 : 16 * t + r) * ldq + 16 * g
                       : xq + (16 * t < M ? 16 * t : 0) * kp + 16 * l;
     constexpr long kStep = FUSED ? 64 : kPiece;
     for (int s = s0; s < s1; s += kAhead) {

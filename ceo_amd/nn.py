@@ -700,7 +700,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, select=None, finishe
 
 class Int8Weight:
     """A (k, n) weight in 8-bit integers with an fp32 scale for each of its n channels, laid
-    out once for ``linear_int8``: ``scale = max |w| / 127`` over a column, ``w / scale`` to the
+    out once for ``linear_int8``: ``scale = max |w| * (1 / 127)`` in fp32 over a column, ``w / scale`` to the
     nearest (ties to even).  From bf16, fp16 or fp32 (a row stride is fine); k up to 131072.
     A column with a NaN or an infinity gives NaN."""
 

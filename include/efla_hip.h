@@ -707,7 +707,7 @@ int state_reorder_hip(const void* list, const int32_t* parents, hipStream_t stre
 
 /*
  * A weight (k, n) in 8-bit integers with a scale per channel (column):
- *   scale_n = max_k |w_kn| / 127 in fp32, q_kn = w_kn / scale_n to the nearest, ties to even.
+ *   scale_n = max_k |w_kn| (1 / 127), both rounded to fp32, q_kn = w_kn / scale_n to the nearest, ties to even.
  * int8_weight_size: bytes of the packed form (0: k or n out of range); `packed` is
  * 128-byte aligned.  weight: F32, F16 or BF16, row stride ld.  A column with a NaN or an
  * infinity has scale NaN.  k is at most 131072, so that sums stay below 2^31, and n below

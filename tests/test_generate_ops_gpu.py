@@ -373,7 +373,7 @@ def test_reorder_refusals():
 def quantized(x):
     """(whole numbers, scales) of the rows, float64."""
     x = x.double()
-    s = (x.abs().amax(1).float() / 127.0).double()
+    s = (x.abs().amax(1).float() * (torch.ones(()) / 127.0)).double()
     s = torch.where(torch.isfinite(s), s, torch.full_like(s, math.nan))
     q = torch.where(s[:, None] > 0, (x / s[:, None]).round().clamp(-127, 127), torch.zeros_like(x))
     return torch.nan_to_num(q), s
@@ -517,7 +517,7 @@ def test_linear_quotients_on_halves(m):
     weight is one 127 a channel, so an output is 127 times the whole number times the scales."""
     k = 2048
     for scale in (1.0, 0.37, 3.1e-5):
-        s = torch.tensor(127.0 * scale) / 127.0
+        s = torch.tensor(127.0 * scale) * (torch.ones(()) / 127.0)
         steps = torch.arange(k).sub(k // 2).remainder(254).sub(127).double() + 0.5
         x = (steps * s.double()).float()
         i = torch.arange(k)
