@@ -89,7 +89,7 @@ class Decoder:
 
 
 # From this many tokens on a search captures one.  The decoder LM of 24 layers, 4 beams: a token is
-# 2.3 ms of launches and 1.0 ms from a graph, whose capture takes 3 to 7 ms.
+# 2.2 ms of launches and 0.9 ms from a graph, whose capture takes 3 to 7 ms.
 GRAPH_TOKENS = 8
 
 
