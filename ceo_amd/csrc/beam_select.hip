@@ -10,7 +10,7 @@
 // The logits are read once and nothing of their size is written.  Two launches (or one where a
 // text is small, text_kernel):
 //
-// slice_kernel: a workgroup takes a slice of one row, 1 to 4 16-byte vectors a thread, in
+// slice_kernel: a workgroup takes a slice of one row, 1 to 8 16-byte vectors a thread, in
 // registers.  Maximum and sum of exponentials are each thread's own first (no barrier
 // stands between load and exponentials), then joined.  For the best n of the slice each
 // wave finds the n-th largest of its 64 lanes' maxima, bit by bit with one ballot a
@@ -140,6 +140,9 @@ __device__ __forceinline__ float exp_diff(float d) {  // e^d
     return __builtin_amdgcn_exp2f(d * kLog2e);
 }
 
+// c = m log2 e up to here is rounded by 2^20 1.45 / 2^24 at most.
+constexpr float kNear = 0x1p20f;
+
 // A row's vectors start at cache lines: element i of the row is at i + shift, shift its
 // first element's place in its line, and slice s holds [s L, (s + 1) L) of that.
 template <typename T, int VPT>
@@ -190,22 +193,27 @@ slice_kernel(const T* __restrict__ logits, long ld, int V, int n,
         vm[i] = fmaxf(vm[i], -INFINITY) + 0.f;  // no NaN, and -0 is 0
         m = fmaxf(m, vm[i]);
     }
-    // The sum of 2^(z log2 e - c), c = m log2 e rounded: one fused operation and one exponential
-    // an element; what the rounding of c left out is taken back at the end, so that only
-    // z - m meets the constant's own error.  A thread without a logit above -inf: 0, or NaN
-    // from a NaN.  Where m log2 e would overflow (masks of the type's lowest value), floats are
-    // so far apart that any positive factor gives 1 for z = m and 0 below.
+    // Up to kNear the sum of 2^(z log2 e - c), c = m log2 e rounded: one fused operation and one
+    // exponential an element; what the rounding of c left out, an exponent of 0.1 at most, is
+    // taken back at the end, so that only z - m meets the constant's own error.  Further from zero it
+    // would be hundreds, and z - m comes first.  A thread without a logit above -inf: 0, or NaN from a NaN.
     const float m0 = m == -INFINITY ? 0.f : m;
-    const float f = fabsf(m0) > 0x1p126f ? 0x1p-64f : kLog2e, c0 = m0 * f;
     float s = 0.f;
+    auto sum = [&](auto term) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        asm volatile("" : "+v"(x[i]));  // converted again: the fp32 values take four times the registers
+        for (int i = 0; i < VPT; ++i) {
+            asm volatile("" : "+v"(x[i]));  // converted again: the fp32 values take four times the registers
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            s += __builtin_amdgcn_exp2f(fmaf(to_f(x[i][j]), f, -c0));
+            for (int j = 0; j < N; ++j) s += term(to_f(x[i][j]));
+        }
+    };
+    if (__is_same(T, f16) || fabsf(m0) <= kNear) {  // (fp16's largest value is nearer)
+        const float c0 = m0 * kLog2e;
+        sum([&](float z) { return __builtin_amdgcn_exp2f(fmaf(z, kLog2e, -c0)); });
+        s *= __builtin_amdgcn_exp2f(-fmaf(m0, kLog2e, -c0));
+    } else {
+        sum([&](float z) { return exp_diff(z - m0); });
     }
-    s *= __builtin_amdgcn_exp2f(-fmaf(m0, f, -c0));
     const float M = wave_max(m), M0 = M == -INFINITY ? 0.f : M;
     s = wave_sum(s * exp_diff(fminf(m0 - M0, 0.f)));
     if (lane_id() == 0) {

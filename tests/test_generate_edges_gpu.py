@@ -1,0 +1,92 @@
+"""Beam selection where it can go wrong: logits far from zero.
+
+Tolerance of a selection's scores, in units of 2^-24: a sum of exponentials has at most 64 terms added one by one
+in a thread (8 vectors of 8; in the one-launch form at most 32 between two rescalings of 5 units, 4 of
+them, or 16 and 7), 6 + 3 steps of a wave and a workgroup, and four exponentials on a term's way (its
+own and three rescalings) of 1 each, 3 roundings of an argument d that e^d weighs (|d| e^d <= 0.37)
+and a product's 1: 63 + 9 + 4 * 3.2 < 128.  The score's own rounding is half a unit of it.  Within a
+beam the order is that of the logits, whatever the sum."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import announce
+from test_generate_ops_gpu import dev_rows
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+LSE = 128 * U
+
+
+def values(z, scores):
+    """(beams * vocab,) float64 of one text: score + ((z - max z) - log sum exp(z - max z)); a beam without a
+    finite sum or score: -inf."""
+    z = z.double()
+    m = z.max(1, keepdim=True).values
+    d = z - m
+    v = (d - d.exp().sum(1, keepdim=True).log()) + scores.double()[:, None]
+    v[~torch.isfinite(scores) | ~torch.isfinite(m[:, 0]) | torch.isnan(z).any(1)] = -math.inf
+    return v.reshape(-1).numpy()
+
+
+def check(z, scores, n):
+    """Against `values`, text by text; each beam's tokens are the first of its order by logit and token."""
+    from ceo_amd import nn
+
+    B, K = scores.shape
+    V = z.shape[1]
+    s, p, t = (x.cpu().numpy() for x in nn.beam_select(dev_rows(z, z.dtype), scores.cuda(), n)[:3])
+    for b in range(B):
+        zb = z[b * K:(b + 1) * K]
+        v = values(zb, scores[b])
+        flat = p[b].astype(np.int64) * V + t[b]
+        want = -np.sort(-v)[:n]
+        have = v[flat]
+        assert len(set(flat)) == n
+        inf = np.isneginf(want)
+        assert (np.isneginf(have) == inf).all() and (np.isneginf(s[b]) == inf).all()
+        off = np.abs(s[b][~inf] - have[~inf])
+        assert (off <= LSE + U * np.abs(have[~inf])).all(), off.max()
+        assert (np.abs(want - have)[~inf] <= 2 * LSE + 4e-16 * np.abs(want[~inf])).all()
+        rest = np.setdiff1d(np.flatnonzero(np.isneginf(v)), flat[~inf])
+        assert (flat[inf] == rest[:inf.sum()]).all()
+        for k in range(K):
+            mine = t[b][~inf][p[b][~inf] == k]
+            row = zb[k].double().numpy() + 0.0
+            order = np.lexsort((np.arange(V), -row))
+            assert (mine == order[:len(mine)]).all(), (k, mine, order[:len(mine)])
+
+
+def text(B, K, V, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    z = (torch.randn(B * K, V, generator=g) * 2.5).to(dtype)
+    return z, -6.0 - 2.0 * torch.randn(B, K, generator=g).abs()
+
+
+# one workgroup a text, and slices: many logits, many beams, many selected
+SHAPES = [(2, 3, 5000, 4), (2, 3, 30011, 4), (1, 17, 700, 17), (1, 4, 9000, 40), (40, 8, 60000, 8)]
+
+
+def masks(dtype):
+    if dtype is torch.float16:
+        return [-6e4, torch.finfo(dtype).min]
+    return [-1e6, -3e7, -1e9, -5e9, -1e10, -1e20, -1e30, -1e32, -1e37, torch.finfo(dtype).min]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K,V,n", SHAPES)
+def test_masked_runs(dtype, B, K, V, n):
+    """Finite masks over runs of tokens and over all but a few."""
+    for mask in masks(dtype):
+        announce(f"masked runs {dtype} {B} {K} {V} {mask}")
+        z, s = text(min(B, 2), K, V, dtype, K + V)
+        z[:, V // 5:V // 2] = mask
+        z[0, 7:] = mask
+        z[1, ::2] = mask
+        z = z.repeat(-(-B * K // z.shape[0]), 1)[:B * K]
+        s = s.repeat(-(-B // s.shape[0]), 1)[:B]
+        check(z, s, n)
