@@ -1,7 +1,9 @@
 // Beam search's selection for gfx950: of all continuations of a text's beams, the best.
 //
 //   value(k, v) = score_k + z_kv - log sum_v exp z_kv      (beam k, token v, logits z)
+//               = (z_kv - max_v z_kv) + (score_k - log sum_v exp (z_kv - max_v z_kv))
 //
+// (the second form keeps the score and the logarithm beside logits of any size)
 // and of a text's beams * vocabulary values the `select` largest, ties to the lowest
 // k * vocabulary + v.  A finished beam offers the end token at its own score and nothing
 // else.  A beam whose score is not finite, or whose logits have no finite sum of
@@ -444,7 +446,8 @@ __global__ void __launch_bounds__(NTJ)
 join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, int slices,
             const float* __restrict__ scores, const uint8_t* __restrict__ finished, int V,
             int beams, int n, int end_token, int keep_slots, Selected out) {
-    __shared__ double offset[kMaxBeams];  // score - log sum exp; -inf: offers nothing
+    __shared__ double offset[kMaxBeams];  // score - log sum exp (z - top)
+    __shared__ float tops[kMaxBeams];     // the largest logit
     __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
     __shared__ Best place[kJoinPlaces];
     __shared__ Best res[kMaxSelect];
@@ -491,11 +494,12 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
-        const double lse = fin ? 0.0 : (double)M + log(s);
+        const double ls = fin ? 0.0 : log(s);
         if (l == 0) {
-            const bool live = ok && fabs(lse) < (double)INFINITY;
+            const bool live = ok && fabs(ls) < (double)INFINITY && (fin || M > -INFINITY);
             state[k] = !live ? 2 : fin ? 1 : 0;
-            offset[k] = live ? (double)score - lse : -(double)INFINITY;
+            offset[k] = (double)score - ls;
+            tops[k] = M;
         }
     }
     __syncthreads();
@@ -505,7 +509,7 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         if (e >= total) return b;
         b.beam = (int)((unsigned)e / (unsigned)per);
         if (state[b.beam] == 0) {
-            if (x.token >= 0) b.value = (double)x.z + offset[b.beam];
+            if (x.token >= 0) b.value = ((double)x.z - (double)tops[b.beam]) + offset[b.beam];
             b.token = x.token;
         } else if (state[b.beam] == 1 && e == b.beam * per) {
             b.value = offset[b.beam];
@@ -566,7 +570,8 @@ text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
             int keep_slots, Selected out) {
     constexpr int N = 16 / sizeof(T), NTJ = kTextThreads, W = NTJ / kWave, U = 4;
     typedef __attribute__((__vector_size__(16))) T Vec;
-    __shared__ double offset[kTextBeams];  // score - log sum exp; -inf: offers nothing
+    __shared__ double offset[kTextBeams];  // score - log sum exp (z - top); -inf: offers nothing
+    __shared__ float tops[kTextBeams];     // the largest logit
     __shared__ Best place[kJoinPlaces];
     __shared__ Best res[kMaxSelect];
     __shared__ Best wbest[W];
@@ -632,11 +637,14 @@ text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
             const float a = wm[k * waves + i], b = ws[k * waves + i];
             S += a < Mb ? (double)b * (double)exp_diff(a - Mb) : (double)b;
         }
-        const double lse = fin ? 0.0 : (double)Mb + log(S);
-        offset[k] = ok && fabs(lse) < (double)INFINITY ? (double)score - lse : -(double)INFINITY;
+        const double ls = fin ? 0.0 : log(S);
+        const bool offers = ok && fabs(ls) < (double)INFINITY && (fin || Mb > -INFINITY);
+        offset[k] = offers ? (double)score - ls : -(double)INFINITY;
+        tops[k] = Mb;
     }
     __syncthreads();
-    const double off = has ? offset[k] : -(double)INFINITY;
+    const double off = has ? offset[k] : -(double)INFINITY, beam_top = has ? tops[k] : 0.f;
+    auto value_of = [&](float z) { return ((double)z - beam_top) + off; };
     // a thread's candidates whose keys are no less than `from`, and some that are; a finished
     // beam has one
     auto each = [&](uint32_t from, auto f) {
@@ -647,14 +655,14 @@ text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
         }
         for (int v = t; v < nv; v += P) {
             const Vec x = q[v];
-            if (key_of((double)(vec_max<T>(x) + 0.f) + off) < from) continue;
+            if (key_of(value_of(vec_max<T>(x))) < from) continue;
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                f(Best{(double)(to_f(x[j]) + 0.f) + off, k, head + v * N + j});
+                f(Best{value_of(to_f(x[j])), k, head + v * N + j});
         }
-        if (t < edges) f(Best{(double)(to_f(p[edge]) + 0.f) + off, k, edge});
+        if (t < edges) f(Best{value_of(to_f(p[edge])), k, edge});
     };
-    const uint32_t mine = fin ? (t == 0 ? key_of(off) : 0u) : key_of((double)m + off);
+    const uint32_t mine = fin ? (t == 0 ? key_of(off) : 0u) : key_of(value_of(m));
     groups[threadIdx.x] = mine;
     __syncthreads();
     uint32_t group = 0;

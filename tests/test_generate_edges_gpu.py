@@ -90,3 +90,31 @@ def test_masked_runs(dtype, B, K, V, n):
         z = z.repeat(-(-B * K // z.shape[0]), 1)[:B * K]
         s = s.repeat(-(-B // s.shape[0]), 1)[:B]
         check(z, s, n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K,V,n", SHAPES[:4])
+def test_masked_rows(dtype, B, K, V, n):
+    """Beams that a finite mask leaves nothing are uniform, at their own score: behind the live ones."""
+    for mask in masks(dtype) + [-m for m in masks(dtype)]:
+        announce(f"masked rows {dtype} {B} {K} {V} {mask}")
+        z, s = text(B, K, V, dtype, K * V)
+        z[0] = mask
+        z[K - 1] = mask
+        check(z, s, n)
+        z[:] = mask
+        check(z, s, n)
+        z[:, 3] = 0.0  # one token far above the rest, or far below
+        check(z, s, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,K,V,n", SHAPES[:4])
+def test_logits_far_from_zero(dtype, B, K, V, n):
+    """Around one large value, and spread over many magnitudes."""
+    for far in (1e3, 1e6, 2e7, 3e8, 1e10, 1e14, 1e16, 1e30):
+        announce(f"far {dtype} {B} {K} {V} {far}")
+        z, s = text(B, K, V, torch.float32, K + n)
+        check((z + far).to(dtype), s, n)
+        check((z - far).to(dtype), s, n)
+        check((z * far).to(dtype), s, n)
