@@ -5,7 +5,7 @@
 //
 // (the second form keeps the score and the logarithm beside logits of any size)
 // and of a text's beams * vocabulary values the `select` largest, ties to the lowest
-// k * vocabulary + v.  A finished beam offers the end token at its own score and nothing
+// k * vocabulary + v.  Two beams' values are compared in 64 bits, one beam's by their logits.  A finished beam offers the end token at its own score and nothing
 // else.  A beam whose score is not finite, or whose logits have no finite sum of
 // exponentials (a NaN, +inf, -inf everywhere), offers nothing: its values are -inf.
 //
@@ -18,7 +18,7 @@
 // wave finds the n-th largest of its 64 lanes' maxima, bit by bit with one ballot a
 // bit: n logits of the slice are no less, so that is a bound, and the largest of the waves'
 // bounds leaves a few tens of a slice's thousands.  Those go to LDS and are ranked by
-// counting how many are better (value, then token: no two are equal, so the order in
+// counting how many are better (logit, then token: no two are equal, so the order in
 // which they arrive does not matter).  Where more pass the bound than LDS has places
 // (many equal logits) the best are taken out one by one.
 //
@@ -324,10 +324,22 @@ struct Best {
     double value;
     int beam, token;
 };
-__device__ __forceinline__ bool better(const Best& a, const Best& b) {
+// With its logit, as `ordered`.  A beam's own order is that of its logits, which 64 bits do not always
+// leave in the values (a score of -1e30 for a beam that does not count, a logit of 1e30).
+struct Candidate : Best {
+    uint32_t z;
+};
+__device__ __forceinline__ bool better(const Candidate& a, const Candidate& b) {
     if (a.value != b.value) return a.value > b.value;
     if (a.beam != b.beam) return a.beam < b.beam;
+    if (a.z != b.z) return a.z > b.z;
     return a.token < b.token;
+}
+// Whether value = (z - top) + offset may be that of another logit of the beam too.  Logits differ by
+// 2^-24 of the larger at least, and the value's two roundings are 2^-52 of |z| + |top| + |offset|
+// together: two of those are less, unless z is this small.  (0 is as far from the others as they from it.)
+__device__ __forceinline__ bool merges(float z, float top, double offset) {
+    return z != 0.f && fabs((double)z) * 0x1p26 < fabs((double)top) + fabs(offset);
 }
 
 // Whole numbers in the values' order, 0: not a candidate.
@@ -343,36 +355,61 @@ struct Selected {
     uint8_t* finished;
 };
 
+// Candidates that reach the bound, in the order in which they arrive.
+struct Places {
+    Best at[kJoinPlaces];
+    uint32_t z[kJoinPlaces];
+    int count, merged;  // whether logits have to be compared
+    __device__ __forceinline__ void clear() { count = merged = 0; }
+    __device__ __forceinline__ void take(const Candidate& c, float top, double offset) {
+        const int i = atomicAdd(&count, 1);
+        if (i < kJoinPlaces) {
+            at[i] = c;
+            z[i] = c.z;
+        }
+        if (merges(unordered(c.z), top, offset)) merged = 1;
+    }
+};
+
 // The n best of the candidates in `place`, or, where it has not held them all (equal values), of
 // those that `each` hands to a function, a thread its own, into `res` in order; all threads.
 template <int NTJ, typename Each>
-__device__ __forceinline__ void rank(int found, int n, int beams, const Best* place, Best* res,
-                                     Best* wbest, Each each) {
+__device__ __forceinline__ void rank(int n, int beams, const Places& place, Best* res,
+                                     Candidate* wbest, Each each) {
+    const int found = place.count;
     if (found <= kJoinPlaces) {
+        const bool merged = place.merged;
         for (int i = threadIdx.x; i < found; i += NTJ) {
-            const Best b = place[i];
+            const Best b = place.at[i];
             int rank = 0;
-            // without branches, so that the reads need not wait for each other
+            if (merged) {
+                const Candidate c{b, place.z[i]};
+                for (int k = 0; k < found; ++k)
+                    rank += better(Candidate{place.at[k], place.z[k]}, c);
+            } else {
+                // without branches, so that the reads need not wait for each other
 #pragma unroll 4
-            for (int k = 0; k < found; ++k) {
-                const Best x = place[k];
-                const bool before = (x.beam < b.beam) | ((x.beam == b.beam) & (x.token < b.token));
-                rank += (x.value > b.value) | ((x.value == b.value) & before);
+                for (int k = 0; k < found; ++k) {
+                    const Best x = place.at[k];
+                    const bool before =
+                        (x.beam < b.beam) | ((x.beam == b.beam) & (x.token < b.token));
+                    rank += (x.value > b.value) | ((x.value == b.value) & before);
+                }
             }
             if (rank < n) res[rank] = b;
         }
     } else {
         // the best, then the best behind it, n times
-        Best last{(double)INFINITY, -1, -1};
+        Candidate last{{(double)INFINITY, -1, -1}, 0};
         for (int r = 0; r < n; ++r) {
-            Best b{-(double)INFINITY, beams, 0};
-            each([&](const Best& x) {
+            Candidate b{{-(double)INFINITY, beams, 0}, 0};
+            each([&](const Candidate& x) {
                 if (x.value > -(double)INFINITY && better(last, x) && better(x, b)) b = x;
             });
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) {
-                const Best x{__shfl_xor(b.value, o), __shfl_xor(b.beam, o),
-                             __shfl_xor(b.token, o)};
+                const Candidate x{{__shfl_xor(b.value, o), __shfl_xor(b.beam, o),
+                                   __shfl_xor(b.token, o)}, __shfl_xor(b.z, o)};
                 if (better(x, b)) b = x;
             }
             __syncthreads();  // `wbest` has been read
@@ -449,12 +486,11 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     __shared__ double offset[kMaxBeams];  // score - log sum exp (z - top)
     __shared__ float tops[kMaxBeams];     // the largest logit
     __shared__ int state[kMaxBeams];      // 0: live, 1: finished, 2: offers nothing
-    __shared__ Best place[kJoinPlaces];
+    __shared__ Places place;
     __shared__ Best res[kMaxSelect];
-    __shared__ Best wbest[NTJ / kWave];
+    __shared__ Candidate wbest[NTJ / kWave];
     __shared__ __attribute__((aligned(16))) uint32_t groups[256];
     __shared__ uint32_t exact;
-    __shared__ int count;
     const long text = blockIdx.x, row0 = text * beams;
     const int per = slices * n, total = beams * per;
     const Cand* mine = cands + row0 * per;
@@ -474,7 +510,7 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         from[i] = depth < n ? (j - depth * lists) * n + depth : total;
         head[i] = depth < n ? mine[from[i]] : Cand{0.f, -1};
     }
-    if (threadIdx.x == 0) count = 0, exact = 0;
+    if (threadIdx.x == 0) place.clear(), exact = 0;
     // 16 lanes to a beam
     for (int k = threadIdx.x / 16; k < beams; k += NTJ / 16) {
         const int l = threadIdx.x % 16;
@@ -505,19 +541,20 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
     __syncthreads();
     // entry e from what the slice left; a finished beam has one entry
     auto best_of = [&](int e, const Cand& x) {
-        Best b{-(double)INFINITY, 0, 0};
+        Candidate b{{-(double)INFINITY, 0, 0}, 0};
         if (e >= total) return b;
         b.beam = (int)((unsigned)e / (unsigned)per);
         if (state[b.beam] == 0) {
             if (x.token >= 0) b.value = ((double)x.z - (double)tops[b.beam]) + offset[b.beam];
             b.token = x.token;
+            b.z = ordered(x.z);
         } else if (state[b.beam] == 1 && e == b.beam * per) {
             b.value = offset[b.beam];
             b.token = end_token;
         }
         return b;
     };
-    const Best first = best_of(e0, held);
+    const Candidate first = best_of(e0, held);
     // The bound from the largest of some lists: 64 lanes', in every wave by itself, or 256 threads'.
     uint32_t top = 0;
 #pragma unroll
@@ -537,21 +574,16 @@ join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, in
         least = exact;
     }
     least = max(least, 1u);
-    auto take = [&](const Best& b) {
-        const int at = atomicAdd(&count, 1);
-        if (at < kJoinPlaces) place[at] = b;
+    auto take = [&](const Candidate& b) {
+        if (key_of(b.value) >= least) place.take(b, tops[b.beam], offset[b.beam]);
     };
-    if (key_of(first.value) >= least) take(first);
-    for (int e = e0 + NTJ; e < total; e += NTJ) {
-        const Best b = best_of(e, mine[e]);
-        if (key_of(b.value) >= least) take(b);
-    }
+    take(first);
+    for (int e = e0 + NTJ; e < total; e += NTJ) take(best_of(e, mine[e]));
     __syncthreads();
-    const int found = count;
-    rank<NTJ>(found, n, beams, place, res, wbest, [&](auto f) {
+    rank<NTJ>(n, beams, place, res, wbest, [&](auto f) {
         for (int e = e0; e < total; e += NTJ) f(best_of(e, mine[e]));
     });
-    write(res, found, n, V, text, row0, finished, end_token, keep_slots, out);
+    write(res, place.count, n, V, text, row0, finished, end_token, keep_slots, out);
 }
 
 // A whole text in a workgroup, for texts of few logits (kTextLogits), where a second launch is
@@ -572,14 +604,13 @@ text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
     typedef __attribute__((__vector_size__(16))) T Vec;
     __shared__ double offset[kTextBeams];  // score - log sum exp (z - top); -inf: offers nothing
     __shared__ float tops[kTextBeams];     // the largest logit
-    __shared__ Best place[kJoinPlaces];
+    __shared__ Places place;
     __shared__ Best res[kMaxSelect];
-    __shared__ Best wbest[W];
+    __shared__ Candidate wbest[W];
     __shared__ float wm[W], ws[W];
     __shared__ uint32_t groups[NTJ];
-    __shared__ int count;
     const long text = blockIdx.x, row0 = text * beams;
-    if (threadIdx.x == 0) count = 0;
+    if (threadIdx.x == 0) place.clear();
     const int waves = W / beams, P = waves * kWave;  // a beam's
     const int k = wave_id() / waves, t = (int)threadIdx.x - k * P;
     const bool has = k < beams;
@@ -643,24 +674,28 @@ text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
         tops[k] = Mb;
     }
     __syncthreads();
-    const double off = has ? offset[k] : -(double)INFINITY, beam_top = has ? tops[k] : 0.f;
-    auto value_of = [&](float z) { return ((double)z - beam_top) + off; };
+    const double off = has ? offset[k] : -(double)INFINITY;
+    const float beam_top = has ? tops[k] : 0.f;
+    auto value_of = [&](float z) { return ((double)z - (double)beam_top) + off; };
+    auto best_of = [&](T logit, int token) {
+        const float z = to_f(logit) + 0.f;  // -0 is 0
+        return Candidate{{value_of(z), k, token}, ordered(z)};
+    };
     // a thread's candidates whose keys are no less than `from`, and some that are; a finished
     // beam has one
     auto each = [&](uint32_t from, auto f) {
         if (!(off > -(double)INFINITY)) return;
         if (fin) {
-            if (t == 0) f(Best{off, k, end_token});
+            if (t == 0) f(Candidate{{off, k, end_token}, ordered(0.f)});
             return;
         }
         for (int v = t; v < nv; v += P) {
             const Vec x = q[v];
             if (key_of(value_of(vec_max<T>(x))) < from) continue;
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                f(Best{value_of(to_f(x[j])), k, head + v * N + j});
+            for (int j = 0; j < N; ++j) f(best_of(x[j], head + v * N + j));
         }
-        if (t < edges) f(Best{value_of(to_f(p[edge])), k, edge});
+        if (t < edges) f(best_of(p[edge], edge));
     };
     const uint32_t mine = fin ? (t == 0 ? key_of(off) : 0u) : key_of(value_of(m));
     groups[threadIdx.x] = mine;
@@ -670,15 +705,12 @@ text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
     for (int i = 0; i < W; ++i) group = max(group, groups[lane_id() + i * kWave]);
     const uint32_t least = max(wave_bound<4>(group, n), 1u);
     if (mine >= least)
-        each(least, [&](const Best& b) {
-            if (key_of(b.value) < least) return;
-            const int at = atomicAdd(&count, 1);
-            if (at < kJoinPlaces) place[at] = b;
+        each(least, [&](const Candidate& b) {
+            if (key_of(b.value) >= least) place.take(b, beam_top, off);
         });
     __syncthreads();
-    const int found = count;
-    rank<NTJ>(found, n, beams, place, res, wbest, [&](auto f) { each(1, f); });
-    write(res, found, n, V, text, row0, finished, end_token, keep_slots, out);
+    rank<NTJ>(n, beams, place, res, wbest, [&](auto f) { each(1, f); });
+    write(res, place.count, n, V, text, row0, finished, end_token, keep_slots, out);
 }
 
 static size_t dtype_size(int d) {

@@ -662,8 +662,8 @@ int preference_loss_forward_backward_hip(
 /*
  * Of each text's beams * vocab_size continuations the `select` best, in order:
  *   value(k, v) = scores[k] + logits[k][v] - log sum_v exp logits[k][v],
- * ties to the lowest k * vocab_size + v.  logits (batch * beams, vocab_size), row stride
- * ld, F32, F16 or BF16; scores (batch, beams) fp32; out_scores fp32, out_parents (the beam,
+ * ties to the lowest k * vocab_size + v.  Values of two beams are compared in 64 bits, those of
+ * one by their logits.  logits (batch * beams, vocab_size), row stride ld, F32, F16 or BF16; scores (batch, beams) fp32; out_scores fp32, out_parents (the beam,
  * 0 .. beams - 1) and out_tokens int32, all (batch, select).
  * finished (batch, beams) bytes or NULL: a beam that is marked has one continuation,
  * end_token at the beam's own score, and its logits are not read.  out_finished (batch,

@@ -1,4 +1,4 @@
-"""Beam selection where it can go wrong: logits far from zero.
+"""Beam selection where it can go wrong: logits far from zero, scores far below.
 
 Tolerance of a selection's scores, in units of 2^-24: a sum of exponentials has at most 64 terms added one by one
 in a thread (8 vectors of 8; in the one-launch form at most 32 between two rescalings of 5 units, 4 of
@@ -118,3 +118,33 @@ def test_logits_far_from_zero(dtype, B, K, V, n):
         check((z + far).to(dtype), s, n)
         check((z - far).to(dtype), s, n)
         check((z * far).to(dtype), s, n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K,V,n", SHAPES[:4])
+def test_beams_far_below(dtype, B, K, V, n):
+    """Scores and logits beside which 64 bits do not hold a token's part: the beam's own order stays."""
+    announce(f"far below {dtype} {B} {K} {V}")
+    z, s = text(B, K, V, dtype, 3 * K + n)
+    s[:, 1:] = -1e30
+    check(z, s, n)
+    s[:] = -1e9
+    check(z, s, n)
+    if dtype is not torch.float16:
+        z[:, 11] = 1e30
+        check(z, s, n)
+
+
+@pytest.mark.parametrize("B,K,V,n", SHAPES[:4])
+def test_first_of_more(B, K, V, n):
+    """A selection is the start of a larger one, also where 64 bits do not tell a beam's values apart."""
+    from ceo_amd import nn
+
+    z, s = text(B, K, V, torch.float32, n)
+    z[:, V // 3:] *= 1e-20
+    s[:, 0] = -1e20
+    z, s = z.cuda(), s.cuda()
+    more = nn.beam_select(z, s, 64)
+    for m in (1, 2, n, 31, 33):
+        few = nn.beam_select(z, s, m)
+        assert all(torch.equal(a, b[:, :m]) for a, b in zip(few[1:3], more[1:3])), m
