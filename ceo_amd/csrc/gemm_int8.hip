@@ -43,8 +43,8 @@ constexpr long kWaveRows = 2048;
 // every workgroup, while rows are short, or the tokens 8 and the weights small (4 x 4096 x 1024
 // 7.9 us, apart 6.2 + 3.4 and the second launch).  What a wave's registers and 64 KiB of
 // LDS hold: 16-bit tokens, 32 of 1024 or 8 of 4096 values.
-// No more than kFewRows: other kernels need quantised tokens.
 static bool fused(size_t m, size_t n, size_t kp, size_t size) {
+    if (m > (size_t)kFewRows) return false;  // the other kernels read quantised tokens
     if (kp <= 1024) return m <= (size == 2 ? 32 : 16);
     return size == 2 && m <= 8 && kp <= 4096 && n <= 16384;
 }
@@ -141,11 +141,6 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
     const bool whole = n % 8 == 0 && (uintptr_t)y % a == 0 && ldy % 8 == 0 &&
                        (!bias || (uintptr_t)bias % a == 0) &&
                        (!residual || ((uintptr_t)residual % a == 0 && ldr % 8 == 0));
-    if (mid(m, n, kp)) {
-        if (whole) mid_launch<T, kWhole>(xq, xs, wq, m, n, kp, o, st);
-        else mid_launch<T, kRagged>(xq, xs, wq, m, n, kp, o, st);
-        return (int)hipPeekAtLastError();
-    }
     if (m <= kFewRows) {
 #define I8_FEW(MT, LPR, HOLD) \
     few_launch<T, MT, LPR, HOLD>(x, ldx, xq, xs, wq, m, n, k, kp, o, st)
@@ -163,6 +158,12 @@ static int linear(const T* x, long ldx, const uint8_t* packed, const T* bias, co
             I8_FEW(2, 32, 0);
         }
 #undef I8_FEW
+        return (int)hipPeekAtLastError();
+    }
+    if (!xq) return kInvalidConfiguration;  // what follows reads quantised tokens
+    if (mid(m, n, kp)) {
+        if (whole) mid_launch<T, kWhole>(xq, xs, wq, m, n, kp, o, st);
+        else mid_launch<T, kRagged>(xq, xs, wq, m, n, kp, o, st);
         return (int)hipPeekAtLastError();
     }
     const long cus = device_cu_count() > 0 ? device_cu_count() : 256;

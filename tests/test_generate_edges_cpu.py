@@ -1,0 +1,24 @@
+"""What the entry points for generating text say about their memory, without a GPU."""
+import pytest
+
+from ceo_amd import _lib
+
+DTYPES = {14: 2, 2: 2, 0: 4}
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_products_of_many_rows_have_room_for_their_tokens(L, dt):
+    """Only up to 32 rows are quantised by the product's kernel: more need bytes for each of them and a scale."""
+    for k in (1, 64, 128, 129, 1000, 1024, 1025, 4096, 4097, 8200, 131072):
+        kp = -(-k // 128) * 128
+        for n in (1, 16, 1024, 16384, 16385, 50257):
+            for m in (1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 34, 63, 64, 65, 256, 1000, 16384):
+                size = L.linear_int8_workspace_size(m, k, n, dt)
+                assert size == 0 and m <= 32 or size >= -(-m // 16) * 16 * kp + 4 * m, (m, k, n)
+                if size == 0:
+                    assert m <= (32 if dt else 16) if kp <= 1024 else m <= 8 and dt and kp <= 4096
