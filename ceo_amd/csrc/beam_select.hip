@@ -735,11 +735,20 @@ static bool one_workgroup(size_t beams, size_t vocab, size_t n) {
     return beams <= kTextBeams && n <= kFewSelect && beams * vocab <= kTextLogits;
 }
 
+static size_t slice_bytes(size_t n) { return sizeof(float2) + n * sizeof(Cand); }
+
+// Room for the slices of either element size at any alignment.  vectors() takes fewer than 8 only
+// where twice as many would leave fewer than 4 cus slices in all, so that there are no more than 8 cus / rows
+// + 1 in a row; with 8 the 4-byte logits have the most, and one vector of those is the finest cut.
 static size_t scratch(size_t batch, size_t beams, size_t vocab, size_t n) {
-    if (one_workgroup(beams, vocab, n)) return 0;
-    // whatever the type and the alignment: 4-byte logits, one vector a thread
-    const size_t slices = slices_of(vocab, 4, 1, false);
-    return batch * beams * slices * (sizeof(float2) + n * sizeof(Cand));
+    const size_t rows = batch * beams;
+    if (rows == 0 || one_workgroup(beams, vocab, n)) return 0;
+    const size_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    size_t slices = slices_of(vocab, 4, 8, false);
+    if (slices < 8 * cus / rows + 1) slices = 8 * cus / rows + 1;
+    const size_t finest = slices_of(vocab, 4, 1, false);
+    if (slices > finest) slices = finest;
+    return rows * slices * slice_bytes(n);
 }
 
 template <typename T>
@@ -821,6 +830,7 @@ extern "C" int beam_select_hip(const void* logits, const float* scores, const ui
     const int vpt = bs::vectors(rows, vocab_size, size);
     const bool lines = (uintptr_t)logits % 128 == 0 && ld * size % 128 == 0;
     const size_t slices = bs::slices_of(vocab_size, size, vpt, lines);
+    if (rows * slices * bs::slice_bytes(select) > need) return kInvalidConfiguration;
     if (dtype == kDtypeBF16)
         bs::launch<bf16>(logits, scores, finished, (const uint8_t*)ws, rows, vocab_size, ld,
                          select, vpt, slices, stream);

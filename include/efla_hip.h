@@ -674,8 +674,8 @@ int preference_loss_forward_backward_hip(
  * keep_slots (select == beams): not in order, but the best continuation of a beam in that
  * beam's place and the others in the free places, so that most states stay where they are.
  * 1 .. 64 beams, select 1 .. 64 and no more than beams * vocab_size.
- * Workspace (8-byte aligned) of at least beam_select_workspace_size() bytes (0: none, or
- * arguments out of range), or NULL: the library's cached one for `stream`.  Invalid
+ * Workspace (8-byte aligned) of at least beam_select_workspace_size() bytes on the same
+ * device (0: none, or arguments out of range), or NULL: the library's cached one for `stream`.  Invalid
  * arguments -> 1, sizes out of range (vocab_size of 2^30, batch of 2^22 and more) -> 9;
  * batch == 0 -> 0.
  */

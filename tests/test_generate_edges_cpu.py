@@ -22,3 +22,14 @@ def test_products_of_many_rows_have_room_for_their_tokens(L, dt):
                 assert size == 0 and m <= 32 or size >= -(-m // 16) * 16 * kp + 4 * m, (m, k, n)
                 if size == 0:
                     assert m <= (32 if dt else 16) if kp <= 1024 else m <= 8 and dt and kp <= 4096
+
+
+def test_selection_asks_for_what_it_uses(L):
+    """A slice is 16384 logits of 2 bytes or 8192 of 4 where there are many rows, with a place for each selected of 8
+    bytes and 8 more; a few rows' slices are 8 to a compute unit at most."""
+    size = L.beam_select_workspace_size
+    assert size(2500, 8, 128003, 64) <= 20000 * (128003 // 8192 + 2) * (8 + 8 * 64)
+    assert size(64, 8, 50257, 8) <= 512 * (50257 // 8192 + 2) * 72
+    for batch in (1, 3, 100):
+        assert size(batch, 4, 1 << 20, 4) <= (4 * batch * 130 + 8 * 512 + 4 * batch) * 40
+    assert size(0, 4, 50257, 4) == 0

@@ -148,3 +148,35 @@ def test_first_of_more(B, K, V, n):
     for m in (1, 2, n, 31, 33):
         few = nn.beam_select(z, s, m)
         assert all(torch.equal(a, b[:, :m]) for a, b in zip(few[1:3], more[1:3])), m
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,n", [(4, 4), (17, 3), (8, 64)])
+def test_workspace_of_the_size_asked_for(dtype, K, n):
+    """Rows and vocabularies on both sides of where a thread takes 1, 2, 4 or 8 vectors: the same results, and nothing
+    is written behind the workspace."""
+    from ceo_amd import _lib, nn
+
+    L = _lib.lib()
+    code = {torch.bfloat16: 14, torch.float16: 2, torch.float32: 0}[dtype]
+    size = 4 if dtype is torch.float32 else 2
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for rows in (K, 12 * K, 30 * K, 150 * K, 600 * K):
+        for v in (1, 2, 4, 8):
+            slices = max(1, 1024 // rows)
+            for V in {max(slices * 4096 * v // size + d, 50) for d in (-64, -1, 0, 1, 2050)}:
+                if rows * V * size > 1 << 30:
+                    continue
+                announce(f"workspace {dtype} {rows} {K} {V} {n}")
+                z = torch.empty(rows * V + 3, dtype=dtype, device="cuda").normal_(generator=g)[3:].view(rows, V)
+                s = -torch.rand(rows // K, K, generator=g, device="cuda")
+                need = L.beam_select_workspace_size(rows // K, K, V, n)
+                ws = torch.full((need + 4096,), 171, dtype=torch.uint8, device="cuda")
+                want = nn.beam_select(z, s, n)
+                a = torch.empty(rows // K, n, device="cuda")
+                p, t = (torch.empty(rows // K, n, dtype=torch.int32, device="cuda") for _ in range(2))
+                assert L.beam_select_hip(z.data_ptr(), s.data_ptr(), None, a.data_ptr(), p.data_ptr(), t.data_ptr(), None,
+                                         rows // K, K, V, V, n, -1, 0, code, ws.data_ptr(), need,
+                                         torch.cuda.current_stream().cuda_stream) == 0
+                assert all(torch.equal(x, y) for x, y in zip((a, p, t), want))
+                assert bool((ws[need:] == 171).all())
