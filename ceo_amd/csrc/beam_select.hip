@@ -425,7 +425,7 @@ __device__ __forceinline__ void rank(int n, int beams, const Places& place, Best
     __syncthreads();
 }
 
-// The selected, the first wave's.
+// The selected, the first wave's.  (Others have read the text's marks in front of a barrier.)
 __device__ __forceinline__ void write(Best* res, int found, int n, int V, long text, long row0,
                                       const uint8_t* finished, int end_token, int keep_slots,
                                       const Selected& out) {
@@ -464,13 +464,16 @@ __device__ __forceinline__ void write(Best* res, int found, int n, int V, long t
             to = __ffsll((unsigned long long)open) - 1;
         }
     }
+    // the marks may be written over those that they come from: all are read before
+    bool ended = b.token == end_token;
+    if (finished) ended |= finished[row0 + b.beam] != 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (r >= n) return;
     const long at = text * n + to;
     out.scores[at] = (float)b.value;
     out.parents[at] = b.beam;
     out.tokens[at] = b.token;
-    if (out.finished)
-        out.finished[at] = (finished && finished[row0 + b.beam]) || b.token == end_token;
+    if (out.finished) out.finished[at] = ended;
 }
 
 constexpr int kHeads = 2;
@@ -481,7 +484,7 @@ constexpr int kHeads = 2;
 template <int NTJ>
 __global__ void __launch_bounds__(NTJ)
 join_kernel(const float2* __restrict__ stats, const Cand* __restrict__ cands, int slices,
-            const float* __restrict__ scores, const uint8_t* __restrict__ finished, int V,
+            const float* __restrict__ scores, const uint8_t* finished, int V,
             int beams, int n, int end_token, int keep_slots, Selected out) {
     __shared__ double offset[kMaxBeams];  // score - log sum exp (z - top)
     __shared__ float tops[kMaxBeams];     // the largest logit
@@ -598,7 +601,7 @@ constexpr size_t kTextLogits = 49152;
 template <typename T>
 __global__ void __launch_bounds__(kTextThreads)
 text_kernel(const T* __restrict__ logits, long ld, int V, int beams, int n,
-            const float* __restrict__ scores, const uint8_t* __restrict__ finished, int end_token,
+            const float* __restrict__ scores, const uint8_t* finished, int end_token,
             int keep_slots, Selected out) {
     constexpr int N = 16 / sizeof(T), NTJ = kTextThreads, W = NTJ / kWave, U = 4;
     typedef __attribute__((__vector_size__(16))) T Vec;

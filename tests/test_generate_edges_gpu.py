@@ -180,3 +180,23 @@ def test_workspace_of_the_size_asked_for(dtype, K, n):
                                          torch.cuda.current_stream().cuda_stream) == 0
                 assert all(torch.equal(x, y) for x, y in zip((a, p, t), want))
                 assert bool((ws[need:] == 171).all())
+
+
+@pytest.mark.parametrize("B,K,V", [(300, 4, 1000), (300, 5, 20000), (3, 64, 3000)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_marks_in_place(B, K, V, keep):
+    from ceo_amd import _lib, nn
+
+    announce(f"marks in place {B} {K} {V}")
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = torch.randn(B * K, V, generator=g, device="cuda").bfloat16()
+    scores = -torch.rand(B, K, generator=g, device="cuda") * 12
+    for _ in range(3):
+        fin = torch.rand(B, K, generator=g, device="cuda") < 0.4
+        want = nn.beam_select(z, scores, finished=fin, end_token=3, keep_slots=keep)
+        s, p, t = (torch.empty_like(x) for x in want[:3])
+        assert _lib.lib().beam_select_hip(z.data_ptr(), scores.data_ptr(), fin.data_ptr(), s.data_ptr(), p.data_ptr(),
+                                          t.data_ptr(), fin.data_ptr(), B, K, V, V, K, 3, int(keep), 14, None, 0,
+                                          torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((s, p, t, fin), want))
