@@ -74,6 +74,7 @@ _SIGS = {
     "efla_affine_state_scan_hip": (i32, [ctypes.POINTER(vp), ctypes.POINTER(vp), sz, sz, sz, sz,
                                          vp]),
     # EFLA, query readout
+    "efla_chunk_step_tokens": (sz, []),
     "efla_chunk_fwd_workspace_size": (sz, [sz, sz, sz, sz, sz, sz, i32]),
     "efla_chunk_bwd_workspace_size": (sz, [sz, sz, sz, sz, sz, sz, i32]),
     "efla_chunk_fwd_hip": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz,

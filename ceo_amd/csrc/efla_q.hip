@@ -1260,6 +1260,8 @@ static size_t ws_size(size_t batch, size_t seq_len, size_t num_seqs, size_t H, s
     return std::max(packed, carve(p));
 }
 
+extern "C" size_t efla_chunk_step_tokens(void) { return (size_t)kStepTokens; }
+
 extern "C" size_t efla_chunk_fwd_workspace_size(size_t batch_size, size_t seq_len,
                                                 size_t num_seqs, size_t num_heads,
                                                 size_t head_dim_k, size_t head_dim_v,
@@ -1329,7 +1331,7 @@ static int chunk_fwd(const void* q, const void* k, const void* v, const void* be
     if (save && workspace == nullptr) return kInvalidValue;
     const size_t sbytes = (size_t)p.N * p.H * p.K * p.V * sizeof(float);
     if (empty) {
-        if (final_state == nullptr) return kSuccess;
+        if (final_state == nullptr || final_state == initial_state) return kSuccess;
         if (initial_state)
             return (int)hipMemcpyAsync(final_state, initial_state, sbytes,
                                        hipMemcpyDeviceToDevice, stream);

@@ -18,6 +18,7 @@ non-zero return code.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -145,7 +146,16 @@ def _q_shapes(q, k, v, beta, cu_seqlens):
 SAVE_STATES = 1  # EFLA_FWD_SAVE_STATES
 
 
-STEP_TOKENS = 6  # continued from a carried state without a workspace: no chunk, fp32 throughout
+@functools.cache
+def _step_tokens() -> int:
+    return lib().efla_chunk_step_tokens()
+
+
+def __getattr__(name):
+    # tokens continued from a carried state without a workspace: no chunk, fp32 throughout
+    if name == "STEP_TOKENS":
+        return _step_tokens()
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def chunk_efla_fwd(q, k, v, beta, initial_state=None, output_final_state=False,
@@ -174,9 +184,9 @@ def chunk_efla_fwd(q, k, v, beta, initial_state=None, output_final_state=False,
             raise ValueError("out_state must be (N,H,K,V) fp32")
         if initial_state is not None:
             apart = abs(out_state.data_ptr() - initial_state.data_ptr())
-            if apart == 0 and (T > STEP_TOKENS or cu_seqlens is not None or
-                               workspace is not None):
-                raise ValueError(f"a state in place takes up to {STEP_TOKENS} tokens of "
+            most = _step_tokens()
+            if apart == 0 and (T > most or cu_seqlens is not None or workspace is not None):
+                raise ValueError(f"a state in place takes up to {most} tokens of "
                                  "equal-length sequences and no workspace")
             if 0 < apart < 4 * out_state.numel():
                 raise ValueError("out_state overlaps initial_state")

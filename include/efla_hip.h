@@ -103,7 +103,10 @@ int efla_chunked_scan_hip(void** chunk_states, size_t num_chunks, size_t num_hea
  * cu_seqlens != NULL the batch must be 1 and `seq_len` is the packed token
  * count; num_seqs gives the number of sequences (cu_seqlens has num_seqs+1
  * entries); otherwise num_seqs must equal batch_size.  initial_state /
- * final_state (num_seqs, H, d_k, d_v) fp32, either may be NULL.
+ * final_state (num_seqs, H, d_k, d_v) fp32, either may be NULL.  They do not overlap,
+ * except that final_state may be initial_state itself, updated in place, for up to
+ * efla_chunk_step_tokens() tokens of equal-length sequences without a caller's workspace
+ * (a call without a token leaves it alone).
  * Supported: chunk_size 64 (0 selects 64); (d_k, d_v) in
  * {64,128} x {64,128,256} for bf16, d_k = d_v = 64 for fp32.
  * Workspace: pass NULL to use the library's cached buffer for `stream`, or
@@ -116,12 +119,16 @@ int efla_chunked_scan_hip(void** chunk_states, size_t num_chunks, size_t num_hea
  * sequence of 16 chunks or more alone (bf16; it may run as several segments at
  * once) and in a packed batch (always one chain); a bf16 workspace smaller than
  * the queried size that still holds one chain's factors (accepted, one chain);
- * and up to 6 tokens from an initial state, which without a caller's workspace
- * keep the state in fp32 throughout and with one run a padded chunk.
+ * and up to efla_chunk_step_tokens() tokens from an initial state, which without a caller's
+ * workspace keep the state in fp32 throughout and with one run a padded chunk.
  * ======================================================================== */
 size_t efla_chunk_fwd_workspace_size(size_t batch_size, size_t seq_len, size_t num_seqs,
                                      size_t num_heads, size_t head_dim_k, size_t head_dim_v,
                                      int dtype);
+
+/* Tokens up to which a continuation of equal-length sequences without a caller's workspace
+ * runs token by token. */
+size_t efla_chunk_step_tokens(void);
 
 /* flags of efla_chunk_fwd_hip */
 /* Also write each chunk's start state (bf16) and, on the bf16 path, its

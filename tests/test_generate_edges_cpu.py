@@ -33,3 +33,12 @@ def test_selection_asks_for_what_it_uses(L):
     for batch in (1, 3, 100):
         assert size(batch, 4, 1 << 20, 4) <= (4 * batch * 130 + 8 * 512 + 4 * batch) * 40
     assert size(0, 4, 50257, 4) == 0
+
+
+def test_states_in_place_take_the_library_s_steps(L):
+    """The wrapper's limit is the library's; without a token nothing is launched and nothing copied."""
+    from ceo_amd import efla
+
+    assert efla.STEP_TOKENS == L.efla_chunk_step_tokens() >= 1
+    st = 1 << 20
+    assert L.efla_chunk_fwd_hip(16, 16, 16, 16, st, 16, st, None, 2, 0, 2, 2, 64, 64, 64, 14, None, 0, 0, None) == 0

@@ -200,3 +200,23 @@ def test_marks_in_place(B, K, V, keep):
                                           torch.cuda.current_stream().cuda_stream) == 0
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((s, p, t, fin), want))
+
+
+@pytest.mark.parametrize("K,V,dtype", [(64, 64, torch.float32), (64, 64, torch.bfloat16), (128, 256, torch.bfloat16)])
+def test_states_in_place_up_to_the_last_step(K, V, dtype):
+    from ceo_amd import efla
+
+    g = torch.Generator(device="cuda").manual_seed(K + V)
+    for T in (1, efla.STEP_TOKENS, efla.STEP_TOKENS + 1):
+        q, k = (torch.randn(3, T, 2, K, generator=g, device="cuda").to(dtype) for _ in range(2))
+        v = torch.randn(3, T, 2, V, generator=g, device="cuda").to(dtype)
+        beta = torch.rand(3, T, 2, generator=g, device="cuda").to(dtype)
+        s0 = torch.randn(3, 2, K, V, generator=g, device="cuda")
+        o, st = efla.chunk_efla_fwd(q, k, v, beta, s0, True)
+        mine = s0.clone()
+        if T > efla.STEP_TOKENS:
+            with pytest.raises(ValueError):
+                efla.chunk_efla_fwd(q, k, v, beta, mine, out_state=mine)
+            continue
+        o2, _ = efla.chunk_efla_fwd(q, k, v, beta, mine, out_state=mine)
+        assert torch.equal(mine, st) and torch.equal(o, o2)
