@@ -1,7 +1,7 @@
 // Products in 8-bit integers with a scale for each token and channel, for gfx950
 // (included by gemm_int8.hip).
 //
-//   sx_m = max_k |x_mk| / 127, qx_mk = x_mk / sx_m to the nearest whole number (ties to even)
+//   sx_m = max_k |x_mk| (1 / 127), qx_mk = x_mk / sx_m to the nearest whole number (ties to even)
 //   sw_n, qw_kn the same over the columns of the weight, once, when it is packed
 //   y_mn = act((sum_k qx_mk qw_kn) sx_m sw_n + bias_n) + residual_mn, rounded once
 //
@@ -223,6 +223,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
     if (lr == 0) scales[row] = s;
 }
 
+// Packing: the weight is read twice, for its columns' scales and for its values, once in its life (a call, bf16:
+// 1024 x 1024 16 us, 4096 x 1024 20, 1024 x 32000 65).
 // Columns' largest magnitudes, as whole numbers, into amax (zero before).
 template <typename T>
 __global__ void __launch_bounds__(256) column_amax_kernel(const T* __restrict__ w, long ld, long k,

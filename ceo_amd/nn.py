@@ -643,7 +643,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, select=None, finishe
     """(scores fp32, parents int32, tokens int32, finished bool or None), each (batch, select):
     of each text's beams * vocab continuations the ``select`` (default: beams) with the largest
     ``scores[b, k] + log softmax(logits)[b * beams + k, v]``, ties to the lowest
-    ``k * vocab + v``; ``parents`` is k and ``tokens`` v.
+    ``k * vocab + v``; ``parents`` is k and ``tokens`` v.  Tokens are ruled out with -inf (never a
+    continuation) or any finite value; -inf is the faster mask over most of a row.
 
     logits (batch * beams, vocab), bf16, fp16 or fp32 (a row stride is fine); scores (batch,
     beams) fp32.  A beam marked in ``finished`` (bool, (batch, beams)) only continues with
@@ -701,7 +702,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, select=None, finishe
 class Int8Weight:
     """A (k, n) weight in 8-bit integers with an fp32 scale for each of its n channels, laid
     out once for ``linear_int8``: ``scale = max |w| * (1 / 127)`` in fp32 over a column, ``w / scale`` to the
-    nearest (ties to even).  From bf16, fp16 or fp32 (a row stride is fine); k up to 131072.
+    nearest (ties to even).  (torch divides a GPU tensor by 127 the same way; on the CPU the last
+    place of a scale may differ.)  From bf16, fp16 or fp32 (a row stride is fine); k up to 131072.
     A column with a NaN or an infinity gives NaN."""
 
     def __init__(self, weight: torch.Tensor):
