@@ -5,9 +5,10 @@
 //
 // (the second form keeps the score and the logarithm beside logits of any size)
 // and of a text's beams * vocabulary values the `select` largest, ties to the lowest
-// k * vocabulary + v.  Two beams' values are compared in 64 bits, one beam's by their logits.  A finished beam offers the end token at its own score and nothing
-// else.  A beam whose score is not finite, or whose logits have no finite sum of
-// exponentials (a NaN, +inf, -inf everywhere), offers nothing: its values are -inf.
+// k * vocabulary + v.  Two beams' values are compared in 64 bits, one beam's by their logits.
+// A finished beam offers the end token at its own score and nothing else.  A beam whose score is
+// not finite, or whose logits have no finite sum of exponentials (a NaN, +inf, -inf everywhere),
+// offers nothing: its values are -inf.
 //
 // The logits are read once and nothing of their size is written.  Two launches (or one where a
 // text is small, text_kernel):
@@ -31,6 +32,8 @@
 // that are not among them, which is what the order above gives.
 #include <hip/hip_runtime.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "../../include/efla_hip.h"
 #include "common.hpp"
@@ -744,18 +747,16 @@ static bool one_workgroup(size_t beams, size_t vocab, size_t n) {
 
 static size_t slice_bytes(size_t n) { return sizeof(float2) + n * sizeof(Cand); }
 
-// Room for the slices of either element size at any alignment.  vectors() takes fewer than 8 only
-// where twice as many would leave fewer than 4 cus slices in all, so that there are no more than 8 cus / rows
-// + 1 in a row; with 8 the 4-byte logits have the most, and one vector of those is the finest cut.
+// Room for the slices of either element size at any alignment, growing with every argument.  vectors()
+// takes fewer than 8 only where twice as many would leave fewer than 4 cus slices in all, so that there are no
+// more than 8 cus and one a row; with 8 the 4-byte logits have the most, and one vector of those is the
+// finest cut.
 static size_t scratch(size_t batch, size_t beams, size_t vocab, size_t n) {
-    const size_t rows = batch * beams;
-    if (rows == 0 || one_workgroup(beams, vocab, n)) return 0;
-    const size_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    size_t slices = slices_of(vocab, 4, 8, false);
-    if (slices < 8 * cus / rows + 1) slices = 8 * cus / rows + 1;
-    const size_t finest = slices_of(vocab, 4, 1, false);
-    if (slices > finest) slices = finest;
-    return rows * slices * slice_bytes(n);
+    if (one_workgroup(beams, vocab, n)) return 0;
+    const size_t cus = device_cu_count() > 0 ? device_cu_count() : 256, rows = batch * beams;
+    const size_t finest = rows * slices_of(vocab, 4, 1, false);
+    const size_t few = 8 * cus + rows, many = rows * slices_of(vocab, 4, 8, false);
+    return std::max(many, std::min(few, finest)) * slice_bytes(n);
 }
 
 template <typename T>

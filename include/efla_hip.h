@@ -670,8 +670,9 @@ int preference_loss_forward_backward_hip(
  * Of each text's beams * vocab_size continuations the `select` best, in order:
  *   value(k, v) = scores[k] + logits[k][v] - log sum_v exp logits[k][v],
  * ties to the lowest k * vocab_size + v.  Values of two beams are compared in 64 bits, those of
- * one by their logits.  logits (batch * beams, vocab_size), row stride ld, F32, F16 or BF16; scores (batch, beams) fp32; out_scores fp32, out_parents (the beam,
- * 0 .. beams - 1) and out_tokens int32, all (batch, select).
+ * one by their logits.  logits (batch * beams, vocab_size), row stride ld, F32, F16 or BF16;
+ * scores (batch, beams) fp32; out_scores fp32, out_parents (the beam, 0 .. beams - 1) and
+ * out_tokens int32, all (batch, select).
  * finished (batch, beams) bytes or NULL: a beam that is marked has one continuation,
  * end_token at the beam's own score, and its logits are not read.  out_finished (batch,
  * select) bytes or NULL: the parent is marked or the token is end_token (it may be
@@ -682,8 +683,8 @@ int preference_loss_forward_backward_hip(
  * beam's place and the others in the free places, so that most states stay where they are.
  * 1 .. 64 beams, select 1 .. 64 and no more than beams * vocab_size.
  * Workspace (8-byte aligned) of at least beam_select_workspace_size() bytes on the same
- * device (0: none, or arguments out of range), or NULL: the library's cached one for `stream`.  Invalid
- * arguments -> 1, sizes out of range (vocab_size of 2^30, batch of 2^22 and more) -> 9;
+ * device (0: none, or arguments out of range; enough for smaller arguments too), or NULL:
+ * the library's cached one for `stream`.  Invalid arguments -> 1, sizes out of range (vocab_size of 2^30, batch of 2^22 and more) -> 9;
  * batch == 0 -> 0.
  */
 size_t beam_select_workspace_size(size_t batch, size_t beams, size_t vocab_size, size_t select);

@@ -42,3 +42,21 @@ def test_states_in_place_take_the_library_s_steps(L):
     assert efla.STEP_TOKENS == L.efla_chunk_step_tokens() >= 1
     st = 1 << 20
     assert L.efla_chunk_fwd_hip(16, 16, 16, 16, st, 16, st, None, 2, 0, 2, 2, 64, 64, 64, 14, None, 0, 0, None) == 0
+
+
+def test_selection_s_workspace_is_enough_for_less(L):
+    """Sized for the most texts, beams, tokens and selected, it is enough for fewer of each."""
+    size = L.beam_select_workspace_size
+    for vocab in (700, 9000, 50257, 128003, 1 << 20):
+        for beams, n in ((1, 1), (4, 4), (4, 40), (17, 3), (64, 64)):
+            last = 0
+            for batch in list(range(1, 700)) + [1000, 1023, 1024, 1025, 2047, 2048, 2049, 5000]:
+                got = size(batch, beams, vocab, n)
+                assert got >= last, (batch, beams, vocab, n)
+                last = got
+    for batch in (1, 3, 16, 64, 700):
+        last = [0] * 3
+        for step in range(1, 65):
+            got = [size(batch, 20, 700 * step * step, 5), size(batch, step, 50257, 5), size(batch, 20, 5000, step)]
+            assert all(a >= b for a, b in zip(got, last)), (batch, step)
+            last = got
